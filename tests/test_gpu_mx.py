@@ -1,0 +1,564 @@
+"""The MX4 operators on the GPU against their definition in 64 bits (mxref.py): formats and rounding bit for
+bit, products exactly where every partial sum is a 24-bit number and within the bound of 32-bit sums
+elsewhere, the expert layer within the bound that follows from its documented roundings."""
+import ctypes as C
+import functools
+import math
+
+import pytest
+import torch
+
+import mxref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mx():
+    from unoq_dsp import mx
+    return mx
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def matrix(rows, k, dtype, seed, pad=0, offset=0):
+    """Values of several magnitudes in a view whose rows are k + pad apart, `offset` elements into it."""
+    g = gen(seed)
+    flat = torch.randn(rows * (k + pad) + offset, generator=g, device="cuda")
+    flat = flat * torch.exp(2 * torch.randn(flat.shape, generator=g, device="cuda"))
+    return flat.to(dtype)[offset:].view(rows, k + pad)[:, :k]
+
+
+def on_gpu(pair):
+    return tuple(t.cuda() for t in pair)
+
+
+@functools.lru_cache(maxsize=16)
+def weights(n, k, seed, batch=None):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn((batch or 1) * n, k, generator=g) / math.sqrt(k)
+    c, s = mxref.stored(w)
+    if batch:
+        return c.view(batch, n, -1), s.view(batch, n, -1)
+    return c, s
+
+
+def assert_within(got, want, bound, what=""):
+    got, want = got.cpu().double(), want.double()
+    assert got.shape == want.shape
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan), what
+    off = (got - want).abs()[~nan]
+    over = off > bound.double()[~nan]
+    assert not over.any(), f"{what}: {int(over.sum())} of {over.numel()} outside, worst {float((off / bound[~nan].clamp(min=1e-300)).max()):.3g} of its bound"
+
+
+SIZES = [(1, 1), (1, 2), (3, 31), (2, 32), (5, 33), (1, 127), (130, 128), (4, 129), (257, 77), (64, 1024), (33, 4099)]
+
+
+# ---- formats -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,k", SIZES)
+def test_quantize_is_the_definition(mx, rows, k, name):
+    for pad, offset in ((0, 0), (1, 0), (8, 8), (5, 3)):
+        x = matrix(rows, k, mxref.TYPES[name], rows * k, pad, offset)
+        c, s = mxref.stored(x)
+        q = mx.quantize(x, layout="stored")
+        assert torch.equal(q.scales.cpu(), s) and torch.equal(q.codes.cpu(), c)
+        o = mx.quantize(x)
+        for dtype in mxref.TYPES.values():
+            want = mxref.values(c, s, k).to(dtype)
+            assert torch.equal(q.dequantize(dtype).cpu(), want) and torch.equal(o.dequantize(dtype).cpu(), want)
+
+
+def test_quantize_operand_bytes(mx):
+    for rows, k in ((128, 128), (256, 384), (128, 200)):
+        x = matrix(rows, k, torch.bfloat16, k)
+        want = mxref.operand(*mxref.stored(x), k)
+        q = mx.quantize(x)
+        assert torch.equal(q.codes.cpu(), want[0]) and torch.equal(q.scales.cpu(), want[1])
+
+
+def test_quantize_borders_and_extremes(mx):
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.99, 0.0, -0.0])
+    ties = torch.cat((ties, -ties, torch.nextafter(ties, torch.tensor(9.0))))
+    x = torch.zeros(12, 64)
+    x[:, :36] = ties
+    x[:, 40] = 7.0
+    x = x * torch.ldexp(torch.ones(12, 1), torch.tensor([[0], [5], [-20], [120], [-120], [-130], [-140], [125], [-149], [1], [-1], [-126]]))
+    x[3] = 0
+    q = mx.quantize(x.cuda(), layout="stored")
+    c, s = mxref.stored(x)
+    assert torch.equal(q.scales.cpu(), s) and torch.equal(q.codes.cpu(), c)
+    assert torch.equal(q.dequantize(torch.float32).cpu().double(), mxref.values(c, s, 64).float().double())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_nonfinite_value_makes_its_block_nan(mx, bad):
+    x = matrix(6, 96, torch.float32, 1)
+    x[1, 40] = bad
+    x[4, 95] = bad
+    for layout in ("stored", "operand"):
+        v = mx.quantize(x, layout=layout).dequantize(torch.float32).cpu()
+        want = mxref.values(*mxref.stored(x), 96)
+        assert torch.equal(torch.isnan(v), torch.isnan(want)) and int(torch.isnan(v).sum()) == 64
+        assert torch.equal(v[~torch.isnan(v)].double(), want[~torch.isnan(want)])
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (2, 33), (130, 77), (256, 128), (129, 4099)])
+def test_pack_is_the_operand_layout(mx, n, k):
+    c, s = weights(n, k, n + k)
+    if k % 2:
+        c = c.clone()
+        c[:, -1] |= 0xF0  # what files hold in the nibble past the last value is not read
+    p = mx.pack(c.cuda(), s.cuda(), k=k)
+    want = mxref.operand(c, s, k)
+    assert torch.equal(p.codes.cpu(), want[0]) and torch.equal(p.scales.cpu(), want[1])
+    assert torch.equal(p.dequantize(torch.float32).cpu().double(), mxref.values(c, s, k))
+
+
+def test_pack_of_paired_matrices(mx):
+    for f, d in ((1, 5), (128, 64), (200, 130)):
+        c, s = weights(2 * f, d, f, batch=3)
+        layer = mx.Experts(torch.zeros(3, d, dtype=torch.bfloat16, device="cuda"), (c.cuda(), s.cuda()),
+                           on_gpu(weights(d, f, 1, batch=3)), 2)
+        parts = [mxref.operand(c[e], s[e], d, paired=True) for e in range(3)]
+        assert torch.equal(layer.gate_up[0].cpu(), torch.cat([p[0] for p in parts]))
+        assert torch.equal(layer.gate_up[1].cpu(), torch.cat([p[1] for p in parts]))
+
+
+def test_dequantize_leaves_the_rest_of_a_wide_output(mx):
+    x = matrix(5, 70, torch.bfloat16, 3)
+    wide = torch.full((6, 90), 7.0, device="cuda", dtype=torch.float16)
+    mx.quantize(x).dequantize(torch.float16, out=wide[:5, :70])
+    assert (wide[5] == 7).all() and (wide[:, 70:] == 7).all()
+    assert torch.equal(wide[:5, :70].cpu(), mxref.values(*mxref.stored(x), 70).to(torch.float16))
+
+
+# ---- products ------------------------------------------------------------------------------------
+
+PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 3, 33), (7, 129, 127), (8, 128, 128), (16, 256, 512), (17, 200, 1000), (65, 130, 257),
+            (128, 256, 384), (129, 384, 640), (200, 1000, 96), (257, 515, 1023), (300, 129, 4100), (1, 4096, 4096),
+            (3, 2049, 8192), (40, 4097, 2080), (600, 700, 300)]
+
+
+def whole(rows, k, seed, narrow):
+    """MX4 values whose products and sums are exact in 32 bits: scales 1 and 2 (or 1)."""
+    g = torch.Generator().manual_seed(seed)
+    c = torch.randint(0, 256, (rows, (k + 1) // 2), generator=g, dtype=torch.uint8)
+    if k % 2:
+        c[:, -1] &= 15
+    s = torch.randint(127, 128 if narrow else 129, (rows, (k + 31) // 32), generator=g, dtype=torch.uint8)
+    return c, s
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_matmul_exact(mx, m, n, k):
+    a, w = whole(m, k, m + k, True), whole(n, k, n * 3 + k, False)
+    want = mxref.values(*a, k) @ mxref.values(*w, k).t()   # multiples of 1/4 below 2^22: exact in 32 bits
+    A, W = mx.pack(*on_gpu(a), k=k), mx.pack(*on_gpu(w), k=k)
+    assert torch.equal(mx.matmul(A, W, dtype=torch.float32).cpu().double(), want)
+    for dtype in (torch.float16, torch.bfloat16):
+        assert torch.equal(mx.matmul(A, W, dtype=dtype).cpu(), want.to(torch.float32).to(dtype))
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_matmul_x16_exact(mx, m, n, k, name):
+    # whole activations up to 255: eight bits, exact in both types, and within 2^-12 of their blocks' largest
+    g = torch.Generator().manual_seed(m + n + k)
+    x = torch.randint(-255, 256, (m, k), generator=g).to(mxref.TYPES[name])
+    c, s = whole(n, k, n + k, True)
+    # products are multiples of 1/2; the sum of magnitudes stays below 2^23 halves
+    want = x.double() @ mxref.values(c, s, k).t()
+    W = mx.pack(c.cuda(), s.cuda(), k=k)
+    bound = torch.zeros_like(want) if float((x.double().abs() @ mxref.values(c, s, k).abs().t()).max()) < 2 ** 22 else \
+        mxref.product_bound(x.double(), mxref.values(c, s, k), want, torch.float32)
+    assert_within(mx.matmul(x.cuda(), W, dtype=torch.float32), want, bound)
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_matmul_of_quantised_activations(mx, m, n, k):
+    x = matrix(m, k, torch.bfloat16, m * n)
+    c, s = weights(n, k, m)
+    a, w = mxref.values(*mxref.stored(x), k), mxref.values(c, s, k)
+    W = mx.pack(c.cuda(), s.cuda(), k=k)
+    for dtype in mxref.TYPES.values():
+        assert_within(mx.matmul(mx.quantize(x), W, dtype=dtype), a @ w.t(), mxref.product_bound(a, w, a @ w.t(), dtype), str(dtype))
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_matmul_x16(mx, m, n, k, name):
+    x = torch.randn(m, k + 3, generator=gen(m + n), device="cuda")
+    x = (x * torch.exp(torch.randn(x.shape, generator=gen(n), device="cuda"))).to(mxref.TYPES[name])[:, :k]
+    c, s = weights(n, k, n)
+    a, w = x.cpu().double(), mxref.values(c, s, k)
+    pieces = (a.abs().amax(1, keepdim=True) * 2.0 ** -21) @ w.abs().sum(1)[None]  # the documented floor of small values
+    W = mx.pack(c.cuda(), s.cuda(), k=k)
+    for dtype in mxref.TYPES.values():
+        assert_within(mx.matmul(x, W, dtype=dtype), a @ w.t(), mxref.product_bound(a, w, a @ w.t(), dtype) + pieces, str(dtype))
+
+
+def test_matmul_x16_wide_range_in_a_block(mx):
+    """Values far below their block's largest: exact down to 2^-12 of it, within 2^-21 of it below."""
+    k = 64
+    c, s = whole(16, k, 5, True)
+    w = mxref.values(c, s, k)
+    for dtype in (torch.bfloat16, torch.float16):
+        for shift in range(0, 24):
+            x = torch.zeros(1, k)
+            x[0, 0] = 96.0
+            x[0, 7] = 1.8359375 * 2.0 ** (6 - shift)   # eight significant bits
+            x[0, 33] = -3.0
+            x = x.to(dtype)
+            want = x.double() @ w.t()
+            got = mx.matmul(x.cuda(), mx.pack(c.cuda(), s.cuda(), k=k), dtype=torch.float32).cpu().double()
+            floor = 0.0 if shift <= 12 else 6 * 96 * 2.0 ** -21
+            # the sum itself: three products in 32 bits
+            bound = floor + 4 * 2.0 ** -23 * (x.double().abs() @ w.abs().t())
+            assert ((got - want).abs() <= bound).all(), (dtype, shift)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -120, 2.0 ** 100])
+def test_matmul_x16_far_magnitudes(mx, scale):
+    x = (torch.randn(3, 256, generator=gen(1), device="cuda") * scale).to(torch.bfloat16)
+    c, s = weights(40, 256, 3)
+    a, w = x.cpu().double(), mxref.values(c, s, 256)
+    # below 2^-108 the last piece's scale byte stops at 0: its grid is 2^-127 * 2^-9, half of that per value
+    low = 2.0 ** -137 * w.abs().sum(1)[None]
+    got = mx.matmul(x, mx.pack(c.cuda(), s.cuda()), dtype=torch.float32)
+    pieces = (a.abs().amax(1, keepdim=True) * 2.0 ** -21) @ w.abs().sum(1)[None]
+    assert_within(got, a @ w.t(), mxref.product_bound(a, w, a @ w.t(), torch.float32) + pieces + low)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_nonfinite_rows_stay_apart(mx, bad):
+    x = torch.randn(20, 300, generator=gen(2), device="cuda").to(torch.bfloat16)
+    x[3, 299] = bad
+    x[17, 0] = bad
+    c, s = weights(140, 300, 2)
+    W = mx.pack(c.cuda(), s.cuda())
+    for a in (x, mx.quantize(x)):
+        y = mx.matmul(a, W)
+        rows = torch.isnan(y).all(1)
+        assert rows.nonzero().flatten().tolist() == [3, 17] and not torch.isnan(y[~rows]).any()
+    s2 = s.clone()
+    s2[9, 1] = 255  # a weight block that is not a number: one column
+    y = mx.matmul(x[:3], mx.pack(c.cuda(), s2.cuda()))
+    assert torch.isnan(y).all(0).nonzero().flatten().tolist() == [9] and not torch.isnan(y[:, :9]).any()
+
+
+def test_zero_rows_and_columns(mx):
+    W = mx.pack(*on_gpu(weights(16, 64, 1)))
+    assert mx.matmul(torch.empty(0, 64, device="cuda", dtype=torch.bfloat16), W).shape == (0, 16)
+    q = mx.quantize(torch.empty(0, 64, device="cuda"))
+    assert q.shape == (0, 64) and q.dequantize().shape == (0, 64) and mx.matmul(q, W).shape == (0, 16)
+    none = mx.quantize(torch.empty(0, 64, device="cuda"))
+    assert mx.matmul(torch.ones(3, 64, device="cuda", dtype=torch.float16), none).shape == (3, 0)
+
+
+def test_matmul_shapes_and_outputs(mx):
+    x = torch.randn(2, 3, 96, generator=gen(4), device="cuda").to(torch.float16)
+    W = mx.pack(*on_gpu(weights(50, 96, 4)))
+    y = mx.matmul(x, W)
+    assert y.shape == (2, 3, 50) and y.dtype == torch.float16
+    assert torch.equal(mx.matmul(x.view(6, 96), W).view(2, 3, 50), y)
+    assert torch.equal(mx.matmul(x[0, 1], W), y[0, 1])
+    t = x.view(6, 96).t().contiguous().t()  # values of a row apart: copied first
+    assert torch.equal(mx.matmul(t, W).view(2, 3, 50), y)
+    one = x[:1, :1].expand(1, 4, 96)        # rows that are one row
+    assert torch.equal(mx.matmul(one, W)[0, 3], y[0, 0])
+    wide = torch.full((8, 64), 3.0, device="cuda", dtype=torch.bfloat16)
+    mx.matmul(x.view(6, 96), W, dtype=torch.bfloat16, out=wide[:6, 5:55])
+    assert torch.equal(wide[:6, 5:55], mx.matmul(x.view(6, 96), W, dtype=torch.bfloat16))
+    rest = torch.ones_like(wide, dtype=torch.bool)
+    rest[:6, 5:55] = False
+    assert (wide[rest] == 3).all()
+
+
+def test_python_refusals(mx):
+    x = torch.randn(4, 64, device="cuda").to(torch.bfloat16)
+    W = mx.pack(*on_gpu(weights(16, 64, 1)))
+    with pytest.raises(ValueError, match="float64"):
+        mx.quantize(x.double())
+    with pytest.raises(ValueError, match="gradient"):
+        mx.quantize(x.float().requires_grad_())
+    with torch.no_grad():
+        mx.quantize(x.float().requires_grad_())
+    with pytest.raises(ValueError, match="at least one"):
+        mx.quantize(x[:, :0])
+    with pytest.raises(ValueError, match="layout"):
+        mx.quantize(x, layout="rows")
+    with pytest.raises(ValueError, match="operand"):
+        mx.matmul(x, mx.quantize(x, layout="stored"))
+    with pytest.raises(ValueError, match="rows of 32"):
+        mx.matmul(x[:, :32], W)
+    with pytest.raises(ValueError):
+        mx.matmul(x.float(), W)
+    with pytest.raises(ValueError, match="dtype"):
+        mx.matmul(x, W, dtype=torch.float64)
+    with pytest.raises(ValueError, match="shape"):
+        mx.matmul(x, W, out=torch.empty(4, 17, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="overlap"):
+        mx.matmul(x[:, :64], W, out=x[:, :16])
+    with pytest.raises(ValueError, match="contiguous rows"):
+        mx.matmul(x, W, out=torch.empty(16, 4, device="cuda", dtype=torch.bfloat16).t())
+    with pytest.raises(ValueError, match="bytes"):
+        mx.MX4(W.codes[:-1], W.scales, 16, 64)
+    with pytest.raises(ValueError, match="code and"):
+        mx.pack(torch.zeros(4, 32, dtype=torch.uint8, device="cuda"), torch.zeros(4, 2, dtype=torch.uint8, device="cuda"), k=66)
+
+
+def test_abi_refuses_host_pointers(native):
+    d = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    h = torch.zeros(1 << 16, dtype=torch.uint8)
+    at = (h.data_ptr() + 255) // 256 * 256
+    assert native.ug_mx4_quantize(at, 0, 1, 32, 32, 0, d.data_ptr(), d.data_ptr() + 4096, None) == 22
+    assert native.ug_mx4_matmul(d.data_ptr(), d.data_ptr(), 1, d.data_ptr(), at, 8, 32, d.data_ptr() + 32768, 0, 8, None) == 22
+    assert native.ug_mx4_check(99) == 2002
+    assert native.ug_mx4_check(0) == 0
+
+
+# ---- the expert layer ------------------------------------------------------------------------------
+
+EXPERTS = [  # tokens, d, f, experts, top_k, normalize, type, bias
+    (1, 1, 1, 1, 1, True, "bf16", False), (1, 64, 64, 4, 2, True, "bf16", False), (1, 512, 256, 32, 4, True, "bf16", True),
+    (3, 130, 70, 5, 5, False, "f16", False), (7, 333, 129, 60, 3, False, "f16", True), (2, 1024, 384, 8, 1, True, "f16", False),
+    (16, 256, 512, 16, 2, True, "bf16", False), (33, 257, 200, 4, 3, True, "bf16", False), (64, 384, 128, 128, 8, True, "bf16", False),
+    (64, 128, 256, 2, 2, False, "f16", False), (128, 200, 136, 256, 16, True, "bf16", True), (128, 256, 128, 3, 1, True, "f16", False),
+    (5, 1447, 999, 12, 4, True, "bf16", False)]
+
+
+def layer_parts(d, f, e, name, bias, seed):
+    g = torch.Generator().manual_seed(seed)
+    router = (torch.randn(e, d, generator=g) / math.sqrt(d)).to(mxref.TYPES[name])
+    return router, weights(2 * f, d, seed + 1, batch=e), weights(d, f, seed + 2, batch=e), \
+        torch.randn(e, generator=g) if bias else None
+
+
+def distinct(x, router, bias, top):
+    """Rows of x whose choice does not hang on the last bits of the logits."""
+    logits = x.cpu().double() @ router.double().t() + (0 if bias is None else bias.double())
+    if logits.shape[1] == top:
+        gap = torch.ones(logits.shape[0])
+    else:
+        s = logits.sort(-1, descending=True).values
+        gap = s[:, top - 1] - s[:, top]
+    order = logits.sort(-1, descending=True).values[:, :top]
+    inner = (order[:, :-1] - order[:, 1:]).amin(-1) if top > 1 else torch.ones(logits.shape[0])
+    return (torch.minimum(gap, inner) > 1e-4).cpu()
+
+
+@pytest.mark.parametrize("t,d,f,e,top,norm,name,with_bias", EXPERTS)
+def test_experts(mx, t, d, f, e, top, norm, name, with_bias):
+    router, gate_up, down, bias = layer_parts(d, f, e, name, with_bias, t + d)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), top, norm, None if bias is None else bias.cuda())
+    x = torch.randn(t, d + 5, generator=gen(d), device="cuda").to(mxref.TYPES[name])[:, :d]
+    y, chosen, p = layer(x, return_choice=True)
+    ok = distinct(x, router, bias, top)
+    assert ok.sum() >= t / 2
+    want, order, weight, bound = mxref.experts(x, router, gate_up, down, top, norm, bias)
+    assert torch.equal(chosen.cpu().long()[ok], order[ok])
+    # softmax weights: 3 times what the logits are off by, and 2^-20 for expf and the division
+    logit_off = (mxref._sum_error(d) + 2.0 ** -22) * (x.cpu().double().abs() @ router.double().abs().t() + 3).amax(1, keepdim=True)
+    assert ((p.cpu().double() - weight).abs()[ok] <= ((3 * logit_off + 2.0 ** -20) * weight)[ok]).all()
+    assert_within(y[ok.cuda()], want[ok], (bound + mxref.half_step(want, x.dtype))[ok])
+    assert torch.equal(layer(x), y)  # same answer every time
+
+
+def test_experts_ties_go_to_the_lowest_index(mx):
+    router, gate_up, down, _ = layer_parts(64, 64, 40, "bf16", False, 3)
+    router[:] = router[0]
+    router[7] = router[0] * 2
+    x = torch.randn(9, 64, generator=gen(1), device="cuda").to(torch.bfloat16)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 4)
+    _, chosen, _ = layer(x, return_choice=True)
+    sign = (x.cpu().double() @ router[0].double()) > 0
+    for row, up in zip(chosen.tolist(), sign.tolist()):
+        assert row == ([7, 0, 1, 2] if up else [0, 1, 2, 3])
+
+
+def test_experts_every_token_to_one_expert(mx):
+    """The most uneven load: all tokens choose the same two experts of many."""
+    router, gate_up, down, _ = layer_parts(256, 200, 24, "bf16", False, 9)
+    bias = torch.full((24,), -50.0)
+    bias[[3, 20]] = 50.0
+    x = torch.randn(128, 256, generator=gen(6), device="cuda").to(torch.bfloat16)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2, bias=bias.cuda())
+    y, chosen, _ = layer(x, return_choice=True)
+    assert set(chosen.flatten().tolist()) == {3, 20}
+    ok = distinct(x, router, bias, 2)
+    want, _, _, bound = mxref.experts(x, router, gate_up, down, 2, True, bias)
+    assert_within(y[ok.cuda()], want[ok], (bound + mxref.half_step(want, x.dtype))[ok])
+
+
+def test_experts_nonfinite_token(mx):
+    router, gate_up, down, _ = layer_parts(96, 64, 8, "bf16", False, 5)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2)
+    x = torch.randn(6, 96, generator=gen(3), device="cuda").to(torch.bfloat16)
+    clean = layer(x)
+    for bad in (math.nan, math.inf):
+        x2 = x.clone()
+        x2[4, 50] = bad
+        y, chosen, _ = layer(x2, return_choice=True)
+        assert torch.isnan(y[4]).all() and torch.equal(y[:4], clean[:4]) and torch.equal(y[5], clean[5])
+        assert ((chosen >= 0) & (chosen < 8)).all()
+
+
+def test_experts_outputs_and_refusals(mx):
+    router, gate_up, down, _ = layer_parts(64, 64, 4, "f16", False, 5)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2)
+    x = torch.randn(2, 3, 64, generator=gen(3), device="cuda").to(torch.float16)
+    y = layer(x)
+    assert y.shape == (2, 3, 64) and layer(x[:0]).shape == (0, 3, 64)
+    wide = torch.full((7, 80), 3.0, device="cuda", dtype=torch.float16)
+    layer(x.view(6, 64), out=wide[:6, 1:65])
+    assert torch.equal(wide[:6, 1:65], y.view(6, 64)) and (wide[6] == 3).all() and (wide[:, 65:] == 3).all() and (wide[:, 0] == 3).all()
+    with pytest.raises(ValueError):
+        layer(x.to(torch.bfloat16))
+    with pytest.raises(ValueError):
+        layer(x[..., :32])
+    with pytest.raises(ValueError, match="at most 128"):
+        layer(torch.zeros(129, 64, device="cuda", dtype=torch.float16))
+    with pytest.raises(ValueError, match="top_k"):
+        mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 5)
+    with pytest.raises(ValueError, match="down"):
+        mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(gate_up), 2)
+    with pytest.raises(ValueError, match="bias"):
+        mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2, bias=torch.zeros(5, device="cuda"))
+
+
+# ---- streams, graphs, a run of them together -------------------------------------------------------
+
+def block(mx, x, w_in, w_mid, layer):
+    """A small network's step: a 16-bit product, a 4-bit product, the expert layer."""
+    h = mx.matmul(x, w_in)
+    h = mx.matmul(mx.quantize(h), w_mid, dtype=x.dtype)
+    return layer(h)
+
+
+def network(mx):
+    router, gate_up, down, _ = layer_parts(160, 96, 12, "bf16", False, 8)
+    return (mx.pack(*on_gpu(weights(192, 128, 1))), mx.pack(*on_gpu(weights(160, 192, 2))),
+            mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 3))
+
+
+def test_a_run_of_them_together(mx):
+    parts = network(mx)
+    x = torch.randn(10, 128, generator=gen(7), device="cuda").to(torch.bfloat16)
+    w1, w2 = weights(192, 128, 1), weights(160, 192, 2)
+    h1 = mx.matmul(x, parts[0])
+    a = mxref.values(*mxref.stored(h1), 192)
+    want = a @ mxref.values(*w2, 192).t()
+    h2 = mx.matmul(mx.quantize(h1), parts[1], dtype=x.dtype)
+    assert_within(h2, want, mxref.product_bound(a, mxref.values(*w2, 192), want, x.dtype))
+    assert_within(h1, x.cpu().double() @ mxref.values(*w1, 128).t(),
+                  mxref.product_bound(x.cpu().double(), mxref.values(*w1, 128), x.cpu().double() @ mxref.values(*w1, 128).t(), x.dtype) + 1e-5)
+    assert torch.equal(block(mx, x, *parts), parts[2](h2))
+    mx.check()
+
+
+def test_captured_graphs_replay_on_new_inputs(mx):
+    parts = network(mx)
+    x = torch.randn(10, 128, generator=gen(7), device="cuda").to(torch.bfloat16)
+    x2 = torch.randn(10, 128, generator=gen(8), device="cuda").to(torch.bfloat16)
+    want = [block(mx, v, *parts).clone() for v in (x, x2)]
+    graphs = []
+    for _ in range(2):  # two graphs, to be replayed at the same time
+        static = x.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block(mx, static, *parts)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = block(mx, static, *parts)
+        graphs.append((g, static, y))
+    graphs[1][1].copy_(x2)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for (g, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, _, y), w in zip(graphs, want):
+        assert torch.equal(y, w)
+    mx.check()
+
+
+def test_calls_on_two_streams_at_once(mx):
+    parts = network(mx)
+    xs = [torch.randn(12, 128, generator=gen(20 + i), device="cuda").to(torch.bfloat16) for i in range(4)]
+    want = [block(mx, x, *parts).clone() for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[] for _ in xs]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(block(mx, xs[i], *parts))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(v, w) for v in g)
+
+
+def test_calls_from_two_threads(mx):
+    import threading
+    parts = network(mx)
+    x = torch.randn(12, 128, generator=gen(30), device="cuda").to(torch.bfloat16)
+    want = block(mx, x, *parts)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                if not torch.equal(block(mx, x, *parts), want):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_experts_workspace_contents_do_not_matter(mx, native):
+    router, gate_up, down, _ = layer_parts(200, 136, 6, "bf16", False, 2)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 3)
+    x = torch.randn(5, 200, generator=gen(2), device="cuda").to(torch.bfloat16)
+    want = layer(x)
+    need = native.ug_mx4_experts_workspace(C.byref(layer._layer), 5)
+    for fill in (0, 255, 127):
+        ws = torch.full((need + 4096,), fill, dtype=torch.uint8, device="cuda")
+        y = torch.empty_like(x)
+        torch.cuda.synchronize()
+        rc = native.ug_mx4_experts(C.byref(layer._layer), x.data_ptr(), 200, 5, y.data_ptr(), 200, None, None, ws.data_ptr(),
+                                   need, None)
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and (ws[need:] == fill).all()
+
+
+def test_product_workspace_contents_do_not_matter(mx, native):
+    W = mx.pack(*on_gpu(weights(130, 200, 2)))
+    x = torch.randn(5, 200, generator=gen(2), device="cuda").to(torch.float16)
+    want = mx.matmul(x, W)
+    need = native.ug_mx4_matmul_x16_workspace(5, 200, 1)
+    for fill in (0, 255, 127):
+        ws = torch.full((need + 4096,), fill, dtype=torch.uint8, device="cuda")
+        y = torch.empty(5, 130, device="cuda", dtype=torch.float16)
+        torch.cuda.synchronize()
+        rc = native.ug_mx4_matmul_x16(x.data_ptr(), 1, 200, 5, W.codes.data_ptr(), W.scales.data_ptr(), 130, 200, y.data_ptr(), 1,
+                                      130, ws.data_ptr(), need, None)
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and (ws[need:] == fill).all()

@@ -1,0 +1,141 @@
+"""CPU: the MX4 operators' host side (include/unoq_mx.h, unoq_dsp.mx): sizes, refusals in their order
+before any device is touched, and the oracle's own format checks."""
+import ctypes as C
+
+import pytest
+import torch
+
+import mxref
+
+P = 1 << 20  # a well-aligned address that is never followed: every call here is refused first
+
+
+def test_sizes(native):
+    assert native.ug_mx4_codes_bytes(0, 5, 33) == 5 * 17 and native.ug_mx4_scales_bytes(0, 5, 33) == 10
+    assert native.ug_mx4_codes_bytes(1, 129, 129) == 4 * 8192 and native.ug_mx4_scales_bytes(1, 129, 129) == 4 * 512
+    assert native.ug_mx4_codes_bytes(2, 5, 33) == 0 and native.ug_mx4_scales_bytes(-1, 5, 33) == 0
+    assert native.ug_mx4_codes_bytes(1, 2 ** 32 - 1, 128) == 2 ** 25 * 8192  # past 32 bits
+    assert native.ug_mx4_pack_rows(3, 130, 0) == 3 * 256 and native.ug_mx4_pack_rows(3, 130, 1) == 3 * 256
+    assert native.ug_mx4_pack_rows(2, 260, 1) == 2 * 512
+    assert native.ug_mx4_pack_rows(2 ** 31, 130, 0) == 0  # does not fit
+    assert native.ug_mx4_matmul_x16_workspace(3, 100, 0) == 0
+    assert native.ug_mx4_matmul_x16_workspace(3, 100, 2) >= 6 * 128 + 512
+
+
+def test_quantize_refusals(native):
+    q = native.ug_mx4_quantize
+    assert q(P, 3, 1, 32, 32, 0, P, P, None) == 18       # type
+    assert q(P, 0, 1, 32, 32, 2, P, P, None) == 18       # layout
+    assert q(P, 0, 1, 0, 32, 0, P, P, None) == 18        # k
+    assert q(P, 0, 1, 32, 31, 0, P, P, None) == 18       # rows overlap
+    assert q(P, 0, 2 ** 31, 256, 256, 1, P, P, None) == 18
+    assert q(None, 0, 1, 32, 32, 0, P, P, None) == 22
+    assert q(P, 0, 1, 32, 32, 0, None, P, None) == 22
+    assert q(P + 2, 0, 1, 32, 32, 0, P, P, None) == 22   # x misaligned for its type
+    assert q(P, 0, 1, 32, 32, 1, P + 64, P, None) == 22  # operand codes misaligned
+    assert q(P, 0, 1, 32, 32, 1, P, P + 8, None) == 22
+    assert q(None, 0, 0, 32, 32, 0, None, None, None) == 0  # zero rows do nothing
+    assert native.ug_last_error()
+
+
+def test_dequantize_and_pack_refusals(native):
+    dq, pk = native.ug_mx4_dequantize, native.ug_mx4_pack
+    assert dq(P, P, 5, 1, 32, P, 0, 32, None) == 18
+    assert dq(P, P, 0, 1, 32, P, 9, 32, None) == 18
+    assert dq(P, P, 0, 1, 32, P, 0, 5, None) == 18
+    assert dq(P, None, 0, 1, 32, P, 0, 32, None) == 22
+    assert dq(P, P, 0, 1, 32, P + 1, 1, 32, None) == 22
+    assert dq(None, None, 0, 0, 32, None, 0, 32, None) == 0
+    assert pk(P, P, 1, 3, 32, 1, P, P, None) == 18   # odd rows do not pair
+    assert pk(P, P, 1, 4, 32, 2, P, P, None) == 18
+    assert pk(P, P, 1, 4, 0, 0, P, P, None) == 18
+    assert pk(P, P, 2 ** 31, 130, 32, 0, P, P, None) == 18
+    assert pk(P, None, 1, 4, 32, 0, P, P, None) == 22
+    assert pk(P, P, 1, 4, 32, 0, P + 16, P, None) == 22
+    assert pk(None, None, 0, 4, 32, 0, None, None, None) == 0
+
+
+def test_product_refusals(native):
+    mm, mx = native.ug_mx4_matmul, native.ug_mx4_matmul_x16
+    assert mm(P, P, 1, P, P, 8, 32, P, 4, 8, None) == 18
+    assert mm(P, P, 1, P, P, 8, 0, P, 0, 8, None) == 18
+    assert mm(P, P, 1, P, P, 8, 65537, P, 0, 8, None) == 18
+    assert mm(P, P, 1, P, P, 8, 32, P, 0, 7, None) == 18
+    assert mm(None, P, 1, P, P, 8, 32, P, 0, 8, None) == 22
+    assert mm(P, P, 1, None, P, 8, 32, P, 0, 8, None) == 22
+    assert mm(P, P, 1, P + 8, P, 8, 32, P, 0, 8, None) == 22
+    assert mm(P, P, 1, P, P, 8, 32, P + 2, 0, 8, None) == 22
+    assert mm(None, None, 0, None, None, 8, 32, None, 0, 8, None) == 0
+    need = native.ug_mx4_matmul_x16_workspace(1, 32, 2)
+    assert mx(P, 0, 32, 1, P, P, 8, 32, P, 0, 8, P, need, None) == 18   # 32-bit x
+    assert mx(P, 2, 31, 1, P, P, 8, 32, P, 0, 8, P, need, None) == 18
+    assert mx(P, 2, 32, 1, P, P, 8, 32, P, 0, 8, P, need - 1, None) == 22
+    assert mx(P, 2, 32, 1, P, P, 8, 32, P, 0, 8, P + 16, need, None) == 22
+    assert mx(P, 2, 32, 1, P, P, 8, 32, P, 0, 8, None, need, None) == 22
+    assert mx(P + 1, 2, 32, 1, P, P, 8, 32, P, 0, 8, P, need, None) == 22
+    assert mx(None, 2, 32, 0, None, None, 8, 32, None, 0, 8, None, 0, None) == 0
+
+
+def _layer(**other):
+    from unoq_dsp.mx import UgMx4Experts
+    fields = dict(experts=8, top_k=2, d=64, f=64, normalize=1, type=2, router=P, bias=None, gate_up_codes=P,
+                  gate_up_scales=P, down_codes=P, down_scales=P)
+    fields.update(other)
+    return UgMx4Experts(**fields)
+
+
+def test_experts_refusals(native):
+    size, run = native.ug_mx4_experts_workspace, native.ug_mx4_experts
+
+    def call(layer, x=P, xs=64, t=1, y=P, ys=64, ws=P, n=1 << 30):
+        return run(C.byref(layer), x, xs, t, y, ys, None, None, ws, n, None)
+
+    assert size(C.byref(_layer()), 4) > 0
+    for bad in (dict(experts=0), dict(experts=257), dict(top_k=0), dict(top_k=9), dict(experts=32, top_k=17), dict(d=0),
+                dict(d=16385), dict(f=0), dict(f=16385), dict(type=0)):
+        assert size(C.byref(_layer(**bad)), 4) == 0 and call(_layer(**bad)) == 18, bad
+    assert size(C.byref(_layer()), 129) == 0 and call(_layer(), t=129) == 18
+    assert call(_layer(), xs=63) == 18 and call(_layer(), ys=63) == 18
+    assert call(_layer(), x=None) == 22 and call(_layer(), y=None) == 22 and call(_layer(), ws=None) == 22
+    assert call(_layer(router=None)) == 22 and call(_layer(down_scales=None)) == 22
+    assert call(_layer(bias=P + 2)) == 22 and call(_layer(gate_up_codes=P + 64)) == 22 and call(_layer(), x=P + 1) == 22
+    assert call(_layer(), ws=P + 128) == 22
+    need = size(C.byref(_layer()), 1)
+    assert call(_layer(), n=need - 1) == 22
+    assert call(_layer(), t=0, x=None) == 0
+    assert run(None, P, 64, 1, P, 64, None, None, P, 1 << 30, None) == 22
+
+
+def test_no_device_is_an_error(native):
+    if torch.cuda.is_available():
+        pytest.skip("a device is here")
+    assert native.ug_mx4_quantize(P, 0, 1, 32, 32, 0, P, P, None) == 2002
+    assert native.ug_mx4_check(0) == 2002
+
+
+def test_python_refuses_host_tensors():
+    from unoq_dsp import mx
+    x = torch.zeros(2, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        mx.quantize(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        mx.pack(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="MX4"):
+        mx.matmul(x, x)
+    with pytest.raises(ValueError, match="CUDA"):
+        mx.Experts(torch.zeros(4, 64, dtype=torch.bfloat16), (x, x), (x, x), 2)
+
+
+@pytest.mark.parametrize("k", [1, 31, 32, 33, 77])
+def test_oracle_stored_form(k):
+    """The oracle's values are the nearest grid points: off by at most half the spacing of their binade."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(9, k, generator=g) * torch.exp(3 * torch.randn(9, 1, generator=g))
+    x[0] = 0
+    v = mxref.values(*mxref.stored(x), k)
+    for at in range(0, k, 32):
+        b, w = x[:, at:at + 32].double(), v[:, at:at + 32]
+        top = b.abs().amax(1, keepdim=True)
+        assert ((w - b).abs() <= top / 4 + 1e-300).all()       # top is in [4, 8) scales: off by 1, or by 2 past 6
+        small = b.abs() <= top / 4
+        assert ((w - b).abs()[small] <= (top / 16).expand_as(b)[small]).all()  # under 2 scales: off by a quarter

@@ -1,0 +1,165 @@
+// mx.cuh -- microscaled 4-bit (MX4) operators: layouts, number conversions and launchers shared by
+// k_mx.cu (quantisation, packing, activation pieces, router), mx_tc.cu (products) and mx_abi.cu.
+//
+// Types are UgMxType (0 f32, 1 f16, 2 bf16). Operand layout: tiles of 128 rows x 128 values, one
+// tile's codes 8192 contiguous bytes and its scales 512, in the order that the tensor cores' scale
+// copy takes (unoq_mx.h).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace uq {
+
+constexpr int kMxTile = 128;          // rows and values of an operand tile
+constexpr int kMxCodeTile = 8192;     // bytes of its codes
+constexpr int kMxScaleTile = 512;     // bytes of its scales
+constexpr int kMxHiddenPieces = 3;    // pieces of the hidden vector of ug_mx4_experts
+constexpr int kMxRouterCluster = 8;   // CTAs that share one token's router product
+
+__host__ __device__ inline uint32_t mx_tiles(uint32_t n) { return (n + kMxTile - 1) / kMxTile; }
+// Pieces of a 16-bit value: 4 significant bits each, so two hold a bf16 (8) and three an f16 (11).
+__host__ __device__ inline int mx_pieces(int type) { return type == 2 ? 2 : 3; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ size_t mx_code_at(uint32_t r, uint32_t j, uint32_t kt) {
+    return ((size_t)(r / kMxTile) * kt + j / kMxTile) * kMxCodeTile + (r % kMxTile) * 64 + (j % kMxTile) / 2;
+}
+__device__ __forceinline__ size_t mx_scale_at(uint32_t r, uint32_t b, uint32_t kt) {
+    return ((size_t)(r / kMxTile) * kt + b / 4) * kMxScaleTile + (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4;
+}
+
+// 2^(code - 127) of a scale byte; 255 is NaN and 0 the subnormal 2^-127.
+__device__ __forceinline__ float mx_scale_value(uint32_t code) {
+    return code == 255 ? __int_as_float(0x7FC00000) : __uint_as_float(code ? code << 23 : 0x00400000u);
+}
+
+// Eight floats (already divided by the scale) to eight e2m1 codes, the first in the low nibble:
+// round to nearest even, saturating at 6.
+__device__ __forceinline__ uint32_t mx_pack8(const float (&v)[8]) {
+    uint32_t d;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(d)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return d;
+}
+
+// Eight e2m1 codes to floats (exact: f16 holds every e2m1 value).
+__device__ __forceinline__ void mx_unpack8(uint32_t codes, float (&v)[8]) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(codes));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+// One float to e4m3 (nearest even, saturating) and the value that it stands for.
+__device__ __forceinline__ uint32_t mx_e4m3(float v, float *back) {
+    uint16_t p;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(0.0f), "f"(v));
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(p));
+    *back = __low2float(*reinterpret_cast<const __half2 *>(&h));
+    return p & 0xFFu;
+}
+
+// Scale byte of the first piece of a block whose largest magnitude is `top`: top / 2^(s - 127) lies
+// in [128, 256), under e4m3's 448, so no piece saturates. Piece p of the block has scale byte
+// s - 4p: a piece leaves at most half a step, 8 of these units, which the next, 16 times finer,
+// holds as 128. s is at least 12 so that s - 4p stays a scale. NaN and infinity give 255.
+__device__ __forceinline__ uint32_t mx_piece_scale(float top) {
+    const uint32_t e = __float_as_uint(top) >> 23;
+    return e == 255 ? 255u : max(e < 7 ? 0u : e - 7u, 12u);
+}
+__device__ __forceinline__ uint32_t mx_piece_scale_of(uint32_t s, int p) { return s == 255 ? 255u : s - 4 * p; }
+
+template <typename T>
+__device__ __forceinline__ float mx_float(T v);
+template <>
+__device__ __forceinline__ float mx_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float mx_float<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float mx_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T mx_to(float v);
+template <>
+__device__ __forceinline__ float mx_to<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half mx_to<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 mx_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+#endif
+
+cudaError_t launch_mx4_quantize(const void *x, int type, uint32_t rows, uint32_t k, uint64_t stride, int layout,
+                                uint8_t *codes, uint8_t *scales, cudaStream_t s);
+cudaError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int layout, uint32_t rows, uint32_t k,
+                                  void *y, int type, uint64_t stride, cudaStream_t s);
+cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_t count, uint32_t rows, uint32_t k,
+                            int paired, uint8_t *out_codes, uint8_t *out_scales, cudaStream_t s);
+
+// The router's results and the scratch of one ug_mx4_experts call, carved from its workspace.
+struct MxExpertsScratch {
+    int32_t *chosen;      // tokens x top_k
+    float *weight;        // tokens x top_k
+    uint32_t *arrived;    // tokens x mx_tiles(d): pairs whose down product of this tile is written
+    uint8_t *x_pieces;    // (tokens * pieces) x 128 mx_tiles(d), e4m3
+    uint8_t *x_scales;    // (tokens * pieces) x 4 mx_tiles(d)
+    uint8_t *h_pieces;    // (tokens * top_k * 3) x 128 mx_tiles(f), e4m3
+    uint8_t *h_scales;    // (tokens * top_k * 3) x 4 mx_tiles(f)
+    float *partial;       // (tokens * top_k) x d: weighted down products
+};
+
+struct MxExpertsArgs {
+    uint32_t experts, top_k, d, f, tokens;
+    int normalize, type;
+    const void *router;
+    const float *bias;
+    const uint8_t *gate_up_codes, *gate_up_scales, *down_codes, *down_scales;
+    const void *x;
+    uint64_t x_stride;
+    void *y;
+    uint64_t y_stride;
+    int32_t *chosen;      // the caller's copies, or null
+    float *weights;
+    MxExpertsScratch ws;
+};
+
+cudaError_t launch_mx4_router(const MxExpertsArgs &a, cudaStream_t s);
+
+struct MxProductArgs {
+    const void *x;            // 16-bit activations (x16), or null
+    int x_type;
+    uint64_t x_stride;
+    const uint8_t *a_codes, *a_scales;   // MX4 activations, or null
+    uint32_t m;
+    const uint8_t *w_codes, *w_scales;
+    uint32_t n, k;
+    void *y;
+    int type;
+    uint64_t stride;
+    void *workspace;          // x16: pieces and their scales
+};
+
+cudaError_t launch_mx4_product(const MxProductArgs &a, cudaStream_t s);
+cudaError_t launch_mx4_expert_products(const MxExpertsArgs &a, cudaStream_t s);
+
+}  // namespace uq

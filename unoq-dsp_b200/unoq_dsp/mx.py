@@ -1,0 +1,304 @@
+"""Microscaled 4-bit (MX4) operators on PyTorch tensors: quantise, product, expert layer.
+
+The functions check their tensors, allocate the results (and a workspace of the call's own) with
+PyTorch's allocator and launch the kernels of include/unoq_mx.h on the current stream of the
+tensors' device, without waiting for it; all of them may be captured into a CUDA graph. They are
+for inference: an input that needs a gradient is refused while gradients are recorded. PyTorch is imported here
+only; the rest of the package does not need it.
+
+    w = mx.quantize(weight)                      # (n, k) -> MX4, once
+    y = mx.matmul(x, w)                          # 16-bit x, 4-bit weights
+    y = mx.matmul(mx.quantize(x), w)             # both in 4 bits
+    layer = mx.Experts(router, gate_up, down, top_k=4)
+    y = layer(x)                                 # a few tokens through a mixture of experts
+"""
+import ctypes as C
+
+import torch
+
+from .errors import DSPError
+from .native import last_error, load_library
+
+STORED, OPERAND = 0, 1
+MAX_TOKENS = 128
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_HALF = (torch.float16, torch.bfloat16)
+
+
+class UgMx4Experts(C.Structure):
+    """include/unoq_mx.h UgMx4Experts."""
+    _fields_ = [("experts", C.c_uint32), ("top_k", C.c_uint32), ("d", C.c_uint32), ("f", C.c_uint32),
+                ("normalize", C.c_int), ("type", C.c_int), ("router", C.c_void_p), ("bias", C.c_void_p),
+                ("gate_up_codes", C.c_void_p), ("gate_up_scales", C.c_void_p), ("down_codes", C.c_void_p),
+                ("down_scales", C.c_void_p)]
+
+
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        _lib = load_library()
+    return _lib
+
+
+def _check(lib, rc, what):
+    if rc:
+        raise DSPError(f"{what} failed: {rc & 0xFFFFFFFF:#010x} {last_error(lib)}; no CPU fallback".rstrip())
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _input(x, what, types):
+    """Refuse what the kernels do not take: other types and devices, gradients."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    if x.dtype not in types:
+        raise ValueError(f"{what} must be one of {', '.join(str(t) for t in types)}, not {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} needs a gradient; the MX4 operators are for inference (use torch.no_grad())")
+    return x
+
+
+def _rows(x, what):
+    """x as rows of contiguous values: (rows, k) with any row stride; copied only where it has to be."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what} needs at least one value in its last axis")
+    x = x.reshape(-1, x.shape[-1])
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x
+
+
+def _row_stride(x):
+    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+
+
+def _output(out, shape, dtype, device, inputs):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.device != device:
+        raise ValueError(f"out must be a tensor of shape {tuple(shape)} on {device}")
+    if out.dtype != dtype:
+        raise ValueError(f"out must be {dtype}")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out needs a gradient; the MX4 operators are for inference")
+    if out.shape[-1] > 1 and out.stride(-1) != 1 or out.dim() != 2 and not out.is_contiguous() \
+            or out.dim() == 2 and out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("out needs contiguous rows that do not overlap")
+    lo = out.data_ptr()
+    hi = lo + _extent(out)
+    for x in inputs:
+        if lo < x.data_ptr() + _extent(x) and x.data_ptr() < hi:
+            raise ValueError("out must not overlap an input")
+    return out
+
+
+def _extent(x):
+    """Bytes from x's first to its last element."""
+    if x.numel() == 0:
+        return 0
+    return (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+
+class MX4:
+    """A matrix of ``rows`` x ``k`` 4-bit values with a scale per 32: ``codes`` and ``scales`` (uint8)
+    in the ``layout`` ``"operand"`` (what :func:`matmul` reads) or ``"stored"`` (row-major, the form of
+    files: (rows, ceil(k/2)) and (rows, ceil(k/32)))."""
+
+    __slots__ = ("codes", "scales", "rows", "k", "layout")
+
+    def __init__(self, codes, scales, rows, k, layout="operand"):
+        lib = _library()
+        code = _layout(layout)
+        for x, want, name in ((codes, lib.ug_mx4_codes_bytes(code, rows, k), "codes"),
+                              (scales, lib.ug_mx4_scales_bytes(code, rows, k), "scales")):
+            _input(x, name, (torch.uint8,))
+            if not x.is_contiguous() or x.numel() != want:
+                raise ValueError(f"{name} must be {want} contiguous bytes")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales are on two devices")
+        self.codes, self.scales, self.rows, self.k, self.layout = codes, scales, rows, k, layout
+
+    @property
+    def shape(self):
+        return (self.rows, self.k)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.bfloat16, out=None):
+        """The values, (rows, k), rounded to ``dtype`` once."""
+        if dtype not in _TYPES:
+            raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
+        lib = _library()
+        out = _output(out, (self.rows, self.k), dtype, self.device, (self.codes, self.scales))
+        _check(lib, lib.ug_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _layout(self.layout), self.rows,
+                                          self.k, out.data_ptr(), _TYPES[dtype], _row_stride(out), _stream(self.device)),
+               "MX4 dequantise")
+        return out
+
+
+def _layout(name):
+    if name not in ("stored", "operand"):
+        raise ValueError("layout must be stored or operand")
+    return OPERAND if name == "operand" else STORED
+
+
+def quantize(x, layout="operand"):
+    """(..., k) values in 32 or 16 bits -> :class:`MX4` of their rows. Each block of 32 gets the scale
+    2^(floor(log2 of its largest magnitude) - 2); values go to the nearest e2m1 (ties to even), at
+    most 6 scales; a block holding a NaN or an infinity becomes NaN."""
+    x = _rows(_input(x, "x", tuple(_TYPES)), "x")
+    lib, code = _library(), _layout(layout)
+    rows, k = x.shape
+    codes = torch.empty(lib.ug_mx4_codes_bytes(code, rows, k), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(lib.ug_mx4_scales_bytes(code, rows, k), dtype=torch.uint8, device=x.device)
+    _check(lib, lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, _row_stride(x), code, codes.data_ptr(),
+                                    scales.data_ptr(), _stream(x.device)), "MX4 quantise")
+    if layout == "stored":
+        codes, scales = codes.view(rows, (k + 1) // 2), scales.view(rows, (k + 31) // 32)
+    return MX4(codes, scales, rows, k, layout)
+
+
+def _stored_pair(codes, scales, k, what):
+    for x, name in ((codes, f"{what} codes"), (scales, f"{what} scales")):
+        _input(x, name, (torch.uint8,))
+    if codes.dim() < 2 or scales.shape[:-1] != codes.shape[:-1] or codes.device != scales.device:
+        raise ValueError(f"{what}: codes and scales need the same leading shape and device")
+    if k < 1 or codes.shape[-1] != (k + 1) // 2 or scales.shape[-1] != (k + 31) // 32:
+        raise ValueError(f"{what}: {k} values a row need {(k + 1) // 2} code and {(k + 31) // 32} scale bytes")
+    return codes.contiguous(), scales.contiguous()
+
+
+def _pack(codes, scales, count, rows, k, paired):
+    lib = _library()
+    padded = lib.ug_mx4_pack_rows(count, rows, paired)
+    out = [torch.empty(size(OPERAND, padded, k), dtype=torch.uint8, device=codes.device)
+           for size in (lib.ug_mx4_codes_bytes, lib.ug_mx4_scales_bytes)]
+    _check(lib, lib.ug_mx4_pack(codes.data_ptr(), scales.data_ptr(), count, rows, k, paired, out[0].data_ptr(),
+                                out[1].data_ptr(), _stream(codes.device)), "MX4 pack")
+    return out
+
+
+def pack(codes, scales, k=None):
+    """A stored matrix, (n, ceil(k/2)) and (n, ceil(k/32)) bytes, in the operand layout: once per weight.
+    ``k`` defaults to twice the code bytes of a row."""
+    k = 2 * codes.shape[-1] if k is None else k
+    codes, scales = _stored_pair(codes, scales, k, "pack")
+    if codes.dim() != 2:
+        raise ValueError("pack takes one matrix")
+    n = codes.shape[0]
+    return MX4(*_pack(codes, scales, 1, n, k, 0), n, k)
+
+
+def matmul(a, w, dtype=None, out=None):
+    """y = a w^T for 4-bit weights ``w`` (n x k): ``a`` is an :class:`MX4` (m x k), or 16-bit values (..., k)
+    which are not rounded to fewer bits. Sums are held in 32 bits and rounded once to ``dtype``
+    (default: a's, bfloat16 for an MX4). A NaN or an infinity in a block of ``a`` makes its row NaN."""
+    if not isinstance(w, MX4) or w.layout != "operand":
+        raise ValueError("w must be an MX4 in operand layout (quantize or pack)")
+    lib = _library()
+    four = isinstance(a, MX4)
+    if four:
+        if a.layout != "operand":
+            raise ValueError("a must be in operand layout")
+        lead, m, k, dtype = (a.rows,), a.rows, a.k, dtype or torch.bfloat16
+    else:
+        _input(a, "a", _HALF)
+        lead, dtype = a.shape[:-1], dtype or a.dtype
+        a = _rows(a, "a")
+        m, k = a.shape
+    if dtype not in _TYPES:
+        raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
+    if k != w.k or a.device != w.device:
+        raise ValueError(f"a has rows of {k} on {a.device}, w of {w.k} on {w.device}")
+    y = _output(out, (*lead, w.rows), dtype, w.device, (a.codes, a.scales) if four else (a,))
+    stride = y.stride(0) if y.dim() == 2 and m > 1 else w.rows
+    if four:
+        rc = lib.ug_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), m, w.codes.data_ptr(), w.scales.data_ptr(), w.rows,
+                               k, y.data_ptr(), _TYPES[dtype], stride, _stream(w.device))
+    else:
+        need = lib.ug_mx4_matmul_x16_workspace(m, k, _TYPES[a.dtype])
+        ws = torch.empty(need, dtype=torch.uint8, device=w.device)
+        rc = lib.ug_mx4_matmul_x16(a.data_ptr(), _TYPES[a.dtype], _row_stride(a), m, w.codes.data_ptr(),
+                                   w.scales.data_ptr(), w.rows, k, y.data_ptr(), _TYPES[dtype], stride, ws.data_ptr(), need,
+                                   _stream(w.device))
+    _check(lib, rc, "MX4 product")
+    return y
+
+
+class Experts:
+    """A mixture-of-experts layer for a few tokens (at most 128), its expert weights in 4 bits.
+
+    ``router``: (experts, d) in 16 bits; ``bias``: (experts,) float32 added to the logits, or None.
+    ``gate_up``: stored codes and scales of (experts, 2f, d), the gate's rows before the up rows;
+    ``down``: those of (experts, d, f). ``normalize``: softmax over the chosen logits, else over all.
+    The weights are packed once, here; the stored ones are not kept."""
+
+    def __init__(self, router, gate_up, down, top_k, normalize=True, bias=None):
+        _input(router, "router", _HALF)
+        if router.dim() != 2 or min(router.shape) < 1:
+            raise ValueError("router must be (experts, d)")
+        e, d = router.shape
+        if not 1 <= e <= 256 or not 1 <= top_k <= min(16, e):
+            raise ValueError("experts must be 1..256 and top_k 1..16, at most the experts")
+        (gc, gs), (dc, ds) = gate_up, down
+        if not isinstance(gc, torch.Tensor) or gc.dim() != 3 or gc.shape[0] != e or gc.shape[1] < 2 or gc.shape[1] % 2:
+            raise ValueError("gate_up must be codes and scales of (experts, 2f, d)")
+        f = gc.shape[1] // 2
+        if not isinstance(dc, torch.Tensor) or dc.dim() != 3 or dc.shape[:2] != (e, d):
+            raise ValueError("down must be codes and scales of (experts, d, f)")
+        if max(d, f) > 16384:
+            raise ValueError("widths must be at most 16384")
+        gc, gs = _stored_pair(gc, gs, d, "gate_up")
+        dc, ds = _stored_pair(dc, ds, f, "down")
+        if bias is not None:
+            _input(bias, "bias", (torch.float32,))
+            if bias.shape != (e,):
+                raise ValueError("bias must be (experts,)")
+            bias = bias.contiguous()
+        for x in (gc, dc) + (() if bias is None else (bias,)):
+            if x.device != router.device:
+                raise ValueError("the layer's tensors are on two devices")
+        self.router, self.bias, self.top_k, self.d, self.f, self.experts = router.contiguous(), bias, top_k, d, f, e
+        self.gate_up = _pack(gc, gs, e, 2 * f, d, 1)
+        self.down = _pack(dc, ds, e, d, f, 0)
+        self._layer = UgMx4Experts(e, top_k, d, f, int(bool(normalize)), _TYPES[router.dtype], self.router.data_ptr(),
+                                   None if bias is None else bias.data_ptr(), self.gate_up[0].data_ptr(),
+                                   self.gate_up[1].data_ptr(), self.down[0].data_ptr(), self.down[1].data_ptr())
+        self._lib = _library()
+
+    def __call__(self, x, out=None, return_choice=False):
+        """(..., d) of the router's type -> the same shape. ``return_choice``: also the chosen experts
+        (tokens, top_k) int32, in falling order of their logits, and their float32 weights."""
+        _input(x, "x", (self.router.dtype,))
+        if x.dim() < 1 or x.shape[-1] != self.d or x.device != self.router.device:
+            raise ValueError(f"x must be (..., {self.d}) on {self.router.device}")
+        shape = x.shape
+        x = _rows(x, "x")
+        t = x.shape[0]
+        if t > MAX_TOKENS:
+            raise ValueError(f"at most {MAX_TOKENS} tokens, not {t}")
+        y = _output(out, shape, x.dtype, x.device, (x,))
+        chosen = torch.empty((t, self.top_k), dtype=torch.int32, device=x.device) if return_choice else None
+        weights = torch.empty((t, self.top_k), dtype=torch.float32, device=x.device) if return_choice else None
+        need = self._lib.ug_mx4_experts_workspace(C.byref(self._layer), t)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        stride = y.stride(0) if y.dim() == 2 and t > 1 else self.d
+        _check(self._lib, self._lib.ug_mx4_experts(
+            C.byref(self._layer), x.data_ptr(), _row_stride(x), t, y.data_ptr(), stride,
+            chosen.data_ptr() if return_choice else None, weights.data_ptr() if return_choice else None, ws.data_ptr(),
+            need, _stream(x.device)), "MX4 experts")
+        return (y, chosen, weights) if return_choice else y
+
+
+def check(device=None):
+    """Wait for the device; raise DSPError if a kernel failed or ran out of its bounded waits."""
+    device = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    lib = _library()
+    _check(lib, lib.ug_mx4_check(device), "MX4 check")

@@ -75,6 +75,24 @@ _SIGNATURES = {
     "ug_detect_buffer": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.POINTER(C.c_void_p)]),
     "ug_measure_int8_peak": (C.c_int, [C.c_uint32, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "ug_last_error": (C.c_char_p, []),
+    "ug_mx4_codes_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32]),
+    "ug_mx4_scales_bytes": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32]),
+    "ug_mx4_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_uint64, C.c_int, C.c_void_p,
+                                  C.c_void_p, C.c_void_p]),
+    "ug_mx4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_void_p, C.c_int,
+                                    C.c_uint64, C.c_void_p]),
+    "ug_mx4_pack_rows": (C.c_uint32, [C.c_uint32, C.c_uint32, C.c_int]),
+    "ug_mx4_pack": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p,
+                              C.c_void_p, C.c_void_p]),
+    "ug_mx4_matmul": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
+                                C.c_void_p, C.c_int, C.c_uint64, C.c_void_p]),
+    "ug_mx4_matmul_x16": (C.c_int, [C.c_void_p, C.c_int, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32,
+                                    C.c_uint32, C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ug_mx4_matmul_x16_workspace": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_int]),
+    "ug_mx4_experts": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ug_mx4_experts_workspace": (C.c_size_t, [C.c_void_p, C.c_uint32]),
+    "ug_mx4_check": (C.c_int, [C.c_int]),
 }
 
 _cache = {}
