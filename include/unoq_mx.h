@@ -39,6 +39,7 @@ enum UgMxType { UG_F32 = 0, UG_F16 = 1, UG_BF16 = 2 };
 enum UgMx4Layout { UG_MX4_STORED = 0, UG_MX4_OPERAND = 1 };
 
 #define UG_MX4_MAX_K 65536        /* longest row of a product */
+#define UG_MX4_MAX_M 2097152      /* rows of a product's activations */
 #define UG_MX4_MAX_TOKENS 128     /* ug_mx4_experts: rows of x */
 #define UG_MX4_MAX_EXPERTS 256
 #define UG_MX4_MAX_TOP_K 16

@@ -191,6 +191,7 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
     T *row = reinterpret_cast<T *>(raw);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = blockIdx.x, t = blockIdx.y;
+    grid_dep_launch();  // the products' set-up may begin; they wait for this kernel's results
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const T *x = static_cast<const T *>(a.x) + t * a.x_stride;
     for (uint32_t i = threadIdx.x; i < a.d; i += blockDim.x) row[i] = x[i];
@@ -224,7 +225,7 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
         const float v = i < a.d ? mx_float(row[i]) : 0.0f;
         // infinity and NaN order above every number here
         const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(v) & 0x7FFFFFFFu);
-        const uint32_t s = mx_piece_scale(__uint_as_float(top));
+        const uint32_t s = mx_piece_scale(__uint_as_float(top), pieces);
         float left = v * __uint_as_float((254u - min(s, 253u)) << 23);
         for (int p = 0; p < pieces; p++) {
             float back;
@@ -236,7 +237,7 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
         }
     }
     if (rank == 0)
-        for (uint32_t i = threadIdx.x; i < mx_tiles(a.d); i += blockDim.x) a.ws.arrived[(size_t)t * mx_tiles(a.d) + i] = 0;
+        for (uint32_t i = threadIdx.x; i < kt * 4; i += blockDim.x) a.ws.arrived[(size_t)t * kt * 4 + i] = 0;
 
     cluster.sync();
     if (rank != 0 || warp != 0) return;

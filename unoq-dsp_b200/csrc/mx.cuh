@@ -84,10 +84,10 @@ __device__ __forceinline__ uint32_t mx_e4m3(float v, float *back) {
 // Scale byte of the first piece of a block whose largest magnitude is `top`: top / 2^(s - 127) lies
 // in [128, 256), under e4m3's 448, so no piece saturates. Piece p of the block has scale byte
 // s - 4p: a piece leaves at most half a step, 8 of these units, which the next, 16 times finer,
-// holds as 128. s is at least 12 so that s - 4p stays a scale. NaN and infinity give 255.
-__device__ __forceinline__ uint32_t mx_piece_scale(float top) {
-    const uint32_t e = __float_as_uint(top) >> 23;
-    return e == 255 ? 255u : max(e < 7 ? 0u : e - 7u, 12u);
+// holds as 128. s is at least 4 (pieces - 1) so that every s - 4p is a scale. NaN and infinity: 255.
+__device__ __forceinline__ uint32_t mx_piece_scale(float top, int pieces) {
+    const uint32_t e = __float_as_uint(top) >> 23, least = 4 * (pieces - 1);
+    return e == 255 ? 255u : max(e < 7 ? 0u : e - 7u, least);
 }
 __device__ __forceinline__ uint32_t mx_piece_scale_of(uint32_t s, int p) { return s == 255 ? 255u : s - 4 * p; }
 
@@ -120,7 +120,7 @@ cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_
 struct MxExpertsScratch {
     int32_t *chosen;      // tokens x top_k
     float *weight;        // tokens x top_k
-    uint32_t *arrived;    // tokens x mx_tiles(d): pairs whose down product of this tile is written
+    uint32_t *arrived;    // tokens x 4 mx_tiles(d): pairs whose 32 values are written
     uint8_t *x_pieces;    // (tokens * pieces) x 128 mx_tiles(d), e4m3
     uint8_t *x_scales;    // (tokens * pieces) x 4 mx_tiles(d)
     uint8_t *h_pieces;    // (tokens * top_k * 3) x 128 mx_tiles(f), e4m3
@@ -159,6 +159,10 @@ struct MxProductArgs {
     void *workspace;          // x16: pieces and their scales
 };
 
+// Rows of e4m3 pieces of m 16-bit tokens (x16).
+size_t mx_piece_rows(uint32_t m, int x_type);
+// Site code of a product kernel's wait that ran out of time on the current device since the last reset.
+int mx_tc_error(bool reset);
 cudaError_t launch_mx4_product(const MxProductArgs &a, cudaStream_t s);
 cudaError_t launch_mx4_expert_products(const MxExpertsArgs &a, cudaStream_t s);
 

@@ -85,10 +85,10 @@ size_t experts_scratch(const UgMx4Experts &l, uint32_t tokens, uint8_t *base, uq
     uq::MxExpertsScratch w;
     w.chosen = reinterpret_cast<int32_t *>(take(pairs * 4));
     w.weight = reinterpret_cast<float *>(take(pairs * 4));
-    w.arrived = reinterpret_cast<uint32_t *>(take(tokens * dt * 4));
+    w.arrived = reinterpret_cast<uint32_t *>(take(tokens * dt * 16));
     w.x_pieces = take(xr * dt * 128);
     w.x_scales = take(xr * dt * 4);
-    w.h_pieces = take(hr * ft * 128 * 2);
+    w.h_pieces = take(hr * ft * 128);
     w.h_scales = take(hr * ft * 4);
     w.partial = reinterpret_cast<float *>(take(pairs * l.d * 4));
     if (ws) *ws = w;
@@ -177,7 +177,9 @@ int ug_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_t count, uin
 
 static int product(uq::MxProductArgs &p, void *stream, const char *name) {
     if (!is_type(p.type)) return fail(18, name);
-    if (p.k < 1 || p.k > UG_MX4_MAX_K || !sizes_ok((uint64_t)p.m * 3, p.k) || !sizes_ok(p.n, p.k) || p.stride < p.n)
+    // rows counted with their padding: whole tiles of n, up to four rows of pieces to a token of m
+    if (p.k < 1 || p.k > UG_MX4_MAX_K || p.m > UG_MX4_MAX_M || !sizes_ok((uint64_t)p.m * 4 + 256, p.k) ||
+        !sizes_ok((uint64_t)p.n + 127, p.k) || p.stride < p.n)
         return fail(18, name);
     if (!p.m || !p.n) return 0;
     const void *x = p.x ? p.x : p.a_codes;
@@ -209,7 +211,7 @@ int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32_t m, c
 
 size_t ug_mx4_matmul_x16_workspace(uint32_t m, uint32_t k, int x_type) {
     if (!is_half(x_type) || !k) return 0;
-    const size_t rows = (size_t)m * uq::mx_pieces(x_type), kt = (k + 127ull) / 128;
+    const size_t rows = uq::mx_piece_rows(m, x_type), kt = (k + 127ull) / 128;
     return up(rows * kt * 128) + up((rows + 127) / 128 * kt * uq::kMxScaleTile);
 }
 
@@ -295,8 +297,10 @@ int ug_mx4_check(int device) {
     }
     if (device < 0 || device >= count) return fail(2002, "device index out of range");
     if (cudaGetDevice(&current) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return fail(2001, "cudaSetDevice");
-    cudaError_t e = cudaDeviceSynchronize();
+    const cudaError_t e = cudaDeviceSynchronize();
+    const int late = e == cudaSuccess ? uq::mx_tc_error(true) : 0;
     cudaSetDevice(current);
+    if (late) return fail(2003, "MX4: a device-side wait timed out");
     return launched(e);
 }
 
