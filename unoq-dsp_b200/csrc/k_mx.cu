@@ -2,6 +2,8 @@
 // expert layer (include/unoq_mx.h). The products are in mx_tc.cu.
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "common.cuh"
 #include "mx.cuh"
 
@@ -12,125 +14,97 @@ namespace cg = cooperative_groups;
 
 // ---- quantise / dequantise -------------------------------------------------------------------
 //
-// 16 lanes take one row's 128 values (one operand tile's width), 8 each: four lanes to a block of
-// 32, whose largest magnitude is found by two shuffles. Bound by memory: in bf16 a value is 2 bytes
-// read and 17/32 written.
+// A warp takes 256 columns (two operand tiles' width, 8 values to a lane, four lanes to a block of
+// 32) of ROWS consecutive rows: the loads of all of them go out first, and a row's addresses are the
+// one before's plus a constant. What bounds it is memory, once the instructions are few: with one
+// row to a thread and its indices by division, 168 instructions a thread held a matrix of 8192 x 8192
+// bf16 to 50 us of issue time.
 
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, uint32_t left, bool vec, float (&v)[8]) {
-    if (vec && left >= 8) {
-        if (sizeof(T) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+template <typename T, bool OPERAND, int ROWS>
+__global__ void __launch_bounds__(256) quantize_kernel(const T *x, uint32_t rows, uint32_t k, uint64_t stride, uint32_t kt,
+                                                       uint32_t chunks, uint8_t *codes, uint8_t *scales, bool vec_in,
+                                                       bool vec_out) {
+    const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
+    const uint32_t group = w / chunks, chunk = w - group * chunks, r0 = group * ROWS;
+    if (r0 >= rows) return;
+    const uint32_t n = min((uint32_t)ROWS, rows - r0), j = chunk * 256 + lane * 8;
+    MxRaw<T> raw[ROWS];
+    mx_load_rows<T, ROWS>(raw, x + r0 * stride + j, stride, n, j < k ? k - j : 0, vec_in && chunk * 256 + 256 <= k);
+    const uint32_t row_bytes = (k + 1) / 2, blocks = (k + 31) / 32;
+    uint8_t *to = codes + (OPERAND ? mx_code_at(r0, j, kt) : (size_t)r0 * row_bytes + j / 2);
+    uint8_t *st = scales + (OPERAND ? mx_scale_at(r0, j / 32, kt) : (size_t)r0 * blocks + j / 32);
+    const bool mine = OPERAND ? j / kMxTile < kt : j < k;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint16_t h = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-                v[i] = mx_float(*reinterpret_cast<const T *>(&h));
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (uint32_t)i < left ? mx_float(p[i]) : 0.0f;
-    }
-}
-
-template <typename T, bool OPERAND>
-__global__ void __launch_bounds__(256) quantize_kernel(const T *x, uint32_t rows, uint32_t k, uint64_t stride,
-                                                       uint32_t kt, uint32_t units, uint8_t *codes, uint8_t *scales,
-                                                       bool vec_in, bool vec_out) {
-    const uint32_t lane = threadIdx.x % 16;
-    const uint32_t step = gridDim.x * (blockDim.x / 16);
-    const uint32_t first = (blockIdx.x * blockDim.x + threadIdx.x) / 16;
-    // every lane of a warp runs the same number of rounds: the two halves differ by one unit
-    for (uint32_t base = first & ~1u; base < units; base += step) {
-        const uint32_t u = base + (first & 1u);
-        const bool live = u < units;
-        const uint32_t r = live ? u / kt : 0, tile = live ? u - r * kt : 0;
-        const uint32_t j = tile * kMxTile + lane * 8;
-        float v[8];
-        load8(x + r * stride + j, live && j < k ? k - j : 0, vec_in, v);
-        float top = 0.0f;
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            top = fmaxf(top, fabsf(v[i]));   // fmaxf drops NaN: kept apart
-            nan |= v[i] != v[i];
-        }
-        uint32_t bits = nan ? 0x7FC00000u : __float_as_uint(top);  // orders as the magnitudes do
-        bits = max(bits, __shfl_xor_sync(~0u, bits, 1));
-        bits = max(bits, __shfl_xor_sync(~0u, bits, 2));
-        const uint32_t e = bits >> 23;                  // biased exponent; subnormal and zero: 0
+    for (int i = 0; i < ROWS; i++) {
+        if ((uint32_t)i >= n) break;
+        uint32_t top = raw[i].top();
+        top = max(top, __shfl_xor_sync(~0u, top, 1));
+        top = max(top, __shfl_xor_sync(~0u, top, 2));
+        const uint32_t e = raw[i].top_bits(top) >> 23;  // biased exponent; subnormal and zero: 0
         const uint32_t s = e == 255 ? 255u : (e < 2 ? 0u : e - 2);
-        const float inverse = __uint_as_float((254u - min(s, 253u)) << 23);   // 2^(127 - s), exact
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= inverse;
+        float v[8];
+        raw[i].values(v, __uint_as_float((254u - min(s, 253u)) << 23));   // times 2^(127 - s), exact
         const uint32_t c = s == 255 ? 0u : mx_pack8(v);
-        if (OPERAND) {
-            uint32_t all = s | __shfl_down_sync(~0u, s, 4) << 8;
-            all |= __shfl_down_sync(~0u, all, 8) << 16;
-            if (live) {
-                *reinterpret_cast<uint32_t *>(codes + mx_code_at(r, j, kt)) = c;
-                if (lane == 0) *reinterpret_cast<uint32_t *>(scales + mx_scale_at(r, tile * 4, kt)) = all;
+        if (mine) {
+            if (OPERAND || (vec_out && j + 8 <= k)) {
+                *reinterpret_cast<uint32_t *>(to) = c;
+            } else {
+                for (uint32_t b = 0; b < 4 && j / 2 + b < row_bytes; b++) to[b] = (uint8_t)(c >> (8 * b));
             }
-        } else if (live && j < k) {
-            const uint32_t row_bytes = (k + 1) / 2;
-            uint8_t *dst = codes + (size_t)r * row_bytes + j / 2;
-            if (vec_out && j + 8 <= k)
-                *reinterpret_cast<uint32_t *>(dst) = c;
-            else
-                for (uint32_t i = 0; i < 4 && j / 2 + i < row_bytes; i++) dst[i] = (uint8_t)(c >> (8 * i));
-            if (lane % 4 == 0) scales[(size_t)r * ((k + 31) / 32) + j / 32] = (uint8_t)s;
+            if (lane % 4 == 0) *st = (uint8_t)s;
         }
+        to += OPERAND ? 64 : row_bytes;
+        st += OPERAND ? 16 : blocks;
     }
 }
 
-template <typename T, bool OPERAND>
-__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t rows,
-                                                         uint32_t k, uint32_t kt, uint32_t units, T *y, uint64_t stride,
-                                                         bool vec_in, bool vec_out) {
-    const uint32_t lane = threadIdx.x % 16;
-    const uint32_t step = gridDim.x * (blockDim.x / 16);
-    for (uint32_t u = (blockIdx.x * blockDim.x + threadIdx.x) / 16; u < units; u += step) {
-        const uint32_t r = u / kt, tile = u - r * kt;
-        const uint32_t j = tile * kMxTile + lane * 8;
-        if (j >= k) continue;
-        uint32_t c = 0, s;
-        if (OPERAND) {
-            c = __ldg(reinterpret_cast<const uint32_t *>(codes + mx_code_at(r, j, kt)));
-            s = __ldg(scales + mx_scale_at(r, j / 32, kt));
-        } else {
-            const uint32_t row_bytes = (k + 1) / 2;
-            const uint8_t *src = codes + (size_t)r * row_bytes + j / 2;
-            if (vec_in && j + 8 <= k)
-                c = __ldg(reinterpret_cast<const uint32_t *>(src));
-            else
-                for (uint32_t i = 0; i < 4 && j / 2 + i < row_bytes; i++) c |= (uint32_t)src[i] << (8 * i);
-            s = __ldg(scales + (size_t)r * ((k + 31) / 32) + j / 32);
-        }
-        float v[8];
-        mx_unpack8(c, v);
-        const float scale = mx_scale_value(s);
+template <typename T, bool OPERAND, int ROWS>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t rows, uint32_t k,
+                                                         uint32_t kt, uint32_t chunks, T *y, uint64_t stride, bool vec_in,
+                                                         bool vec_out) {
+    const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
+    const uint32_t group = w / chunks, chunk = w - group * chunks, r0 = group * ROWS;
+    const uint32_t j = chunk * 256 + lane * 8;
+    if (r0 >= rows || j >= k) return;
+    const uint32_t n = min((uint32_t)ROWS, rows - r0), row_bytes = (k + 1) / 2, blocks = (k + 31) / 32;
+    const uint8_t *from = codes + (OPERAND ? mx_code_at(r0, j, kt) : (size_t)r0 * row_bytes + j / 2);
+    const uint8_t *sf = scales + (OPERAND ? mx_scale_at(r0, j / 32, kt) : (size_t)r0 * blocks + j / 32);
+    uint32_t c[ROWS], s[ROWS];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= scale;
-        T *dst = y + r * stride + j;
+    for (int i = 0; i < ROWS; i++) {
+        c[i] = s[i] = 0;
+        if ((uint32_t)i < n) {
+            if (OPERAND || (vec_in && j + 8 <= k)) {
+                c[i] = __ldg(reinterpret_cast<const uint32_t *>(from));
+            } else {
+                for (uint32_t b = 0; b < 4 && j / 2 + b < row_bytes; b++) c[i] |= (uint32_t)from[b] << (8 * b);
+            }
+            s[i] = __ldg(sf);
+        }
+        from += OPERAND ? 64 : row_bytes;
+        sf += OPERAND ? 16 : blocks;
+    }
+    T *to = y + r0 * stride + j;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++, to += stride) {
+        if ((uint32_t)i >= n) break;
+        float v[8];
+        mx_unpack8(c[i], v);
+        const float scale = mx_scale_value(s[i]);
+#pragma unroll
+        for (int b = 0; b < 8; b++) v[b] *= scale;
         if (vec_out && j + 8 <= k) {
             if (sizeof(T) == 4) {
-                reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
             } else {
-                uint32_t w[4];
+                uint32_t p[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    T p[2] = {mx_to<T>(v[2 * i]), mx_to<T>(v[2 * i + 1])};
-                    w[i] = *reinterpret_cast<const uint32_t *>(p);
-                }
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int b = 0; b < 4; b++) p[b] = mx_pair<T>(v[2 * b], v[2 * b + 1]);
+                *reinterpret_cast<uint4 *>(to) = make_uint4(p[0], p[1], p[2], p[3]);
             }
         } else {
-            for (uint32_t i = 0; i < 8 && j + i < k; i++) dst[i] = mx_to<T>(v[i]);
+            for (uint32_t b = 0; b < 8 && j + b < k; b++) to[b] = mx_to<T>(v[b]);
         }
     }
 }
@@ -179,43 +153,46 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t *codes, const u
 
 // ---- router ------------------------------------------------------------------------------------
 //
-// A cluster of 8 CTAs per token: each holds the token's row in shared memory and takes every eighth
-// expert, one warp to an expert's product (32 lanes across d, fixed order, so logits do not depend
+// A cluster of 8 CTAs per token: each takes every eighth expert, one warp to an expert's product (32 lanes across d, fixed order, so logits do not depend
 // on timing). The logits meet in the first CTA's shared memory, whose first warp selects. The same
 // CTAs split the row into the pieces that the gate / up product reads.
 
 template <typename T>
 __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) router_kernel(MxExpertsArgs a, bool vec) {
-    extern __shared__ __align__(16) uint8_t raw[];
     __shared__ float logits[256];
-    T *row = reinterpret_cast<T *>(raw);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = blockIdx.x, t = blockIdx.y;
     grid_dep_launch();  // the products' set-up may begin; they wait for this kernel's results
+    auto started = cluster.barrier_arrive();  // the first CTA's shared memory exists for the others after the wait
+    bool waited = false;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const T *x = static_cast<const T *>(a.x) + t * a.x_stride;
-    for (uint32_t i = threadIdx.x; i < a.d; i += blockDim.x) row[i] = x[i];
-    cluster.sync();  // the row is staged, and the first CTA's shared memory exists for the others
+    const T *row = static_cast<const T *>(a.x) + t * a.x_stride;
 
     float *remote = cluster.map_shared_rank(logits, 0);
     for (uint32_t e = rank + kMxRouterCluster * warp; e < a.experts; e += kMxRouterCluster * 8) {
         const T *w = static_cast<const T *>(a.router) + (size_t)e * a.d;
         float sum = 0.0f;
         if (vec) {
-#pragma unroll 4
+#pragma unroll 8
             for (uint32_t i = lane * 8; i < a.d; i += 256) {
-                const uint4 p = __ldg(reinterpret_cast<const uint4 *>(w + i)), q = *reinterpret_cast<const uint4 *>(row + i);
+                const uint4 p = __ldg(reinterpret_cast<const uint4 *>(w + i)), q = __ldg(reinterpret_cast<const uint4 *>(row + i));
                 const T *ph = reinterpret_cast<const T *>(&p), *qh = reinterpret_cast<const T *>(&q);
 #pragma unroll
                 for (int j = 0; j < 8; j++) sum = fmaf(mx_float(ph[j]), mx_float(qh[j]), sum);
             }
         } else {
+#pragma unroll 8
             for (uint32_t i = lane; i < a.d; i += 32) sum = fmaf(mx_float(w[i]), mx_float(row[i]), sum);
         }
 #pragma unroll
         for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
+        if (!waited) {
+            cluster.barrier_wait(std::move(started));
+            waited = true;
+        }
         if (lane == 0) remote[e] = sum + (a.bias ? a.bias[e] : 0.0f);
     }
+    if (!waited) cluster.barrier_wait(std::move(started));
 
     // the row's pieces: one warp to a block of 32 values
     const uint32_t kt = mx_tiles(a.d);
@@ -300,33 +277,46 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
 
 bool aligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-// Blocks of 256 threads (16 units) to fill the GPU a few times over, no more than the units need.
+// Blocks of 256 threads (16 units each) to fill the GPU a few times over, no more than the units need.
 unsigned unit_grid(uint64_t units) {
     const uint64_t need = (units + 15) / 16;
     return (unsigned)(need < 148 * 16 ? need : 148 * 16);
 }
 
+// Rows to a warp: 8 (4 in 32 bits) once that still leaves every SM a full set of 64 warps, else one,
+// so that small matrices spread over the GPU.
+bool many_rows(uint32_t rows, uint32_t chunks, int each) { return (uint64_t)(rows / each) * chunks >= 148 * 64; }
+unsigned row_grid(uint32_t rows, uint32_t chunks, int each) {
+    return (unsigned)((((uint64_t)rows + each - 1) / each * chunks + 7) / 8);
+}
+
 template <typename T>
 cudaError_t quantize(const void *x, uint32_t rows, uint32_t k, uint64_t stride, int layout, uint8_t *codes,
                      uint8_t *scales, cudaStream_t s) {
-    const uint32_t kt = mx_tiles(k), units = rows * kt;
+    constexpr int kRows = sizeof(T) == 4 ? 4 : 8;
+    const uint32_t kt = mx_tiles(k), chunks = (k + 255) / 256;
     const bool vec_in = aligned(x, 16) && stride * sizeof(T) % 16 == 0;
     const bool vec_out = aligned(codes, 4) && (k + 1) / 2 % 4 == 0;
-    auto kernel = layout ? quantize_kernel<T, true> : quantize_kernel<T, false>;
-    kernel<<<unit_grid(units), 256, 0, s>>>(static_cast<const T *>(x), rows, k, stride, kt, units, codes, scales, vec_in,
-                                           vec_out);
+    const bool many = many_rows(rows, chunks, kRows);
+    auto kernel = layout ? (many ? quantize_kernel<T, true, kRows> : quantize_kernel<T, true, 1>)
+                         : (many ? quantize_kernel<T, false, kRows> : quantize_kernel<T, false, 1>);
+    kernel<<<row_grid(rows, chunks, many ? kRows : 1), 256, 0, s>>>(static_cast<const T *>(x), rows, k, stride, kt, chunks, codes,
+                                                                    scales, vec_in, vec_out);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t dequantize(const uint8_t *codes, const uint8_t *scales, int layout, uint32_t rows, uint32_t k, void *y,
                        uint64_t stride, cudaStream_t s) {
-    const uint32_t kt = mx_tiles(k), units = rows * kt;
+    constexpr int kRows = 8;
+    const uint32_t kt = mx_tiles(k), chunks = (k + 255) / 256;
     const bool vec_in = aligned(codes, 4) && (k + 1) / 2 % 4 == 0;
     const bool vec_out = aligned(y, 16) && stride * sizeof(T) % 16 == 0;
-    auto kernel = layout ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
-    kernel<<<unit_grid(units), 256, 0, s>>>(codes, scales, rows, k, kt, units, static_cast<T *>(y), stride, vec_in,
-                                           vec_out);
+    const bool many = many_rows(rows, chunks, kRows);
+    auto kernel = layout ? (many ? dequantize_kernel<T, true, kRows> : dequantize_kernel<T, true, 1>)
+                         : (many ? dequantize_kernel<T, false, kRows> : dequantize_kernel<T, false, 1>);
+    kernel<<<row_grid(rows, chunks, many ? kRows : 1), 256, 0, s>>>(codes, scales, rows, k, kt, chunks, static_cast<T *>(y), stride,
+                                                                    vec_in, vec_out);
     return cudaGetLastError();
 }
 
@@ -355,13 +345,12 @@ cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_
 }
 
 cudaError_t launch_mx4_router(const MxExpertsArgs &a, cudaStream_t s) {
-    const bool vec = aligned(a.router, 16) && a.d % 8 == 0;
+    const bool vec = aligned(a.router, 16) && a.d % 8 == 0 && aligned(a.x, 16) && a.x_stride % 8 == 0;
     const dim3 grid(kMxRouterCluster, a.tokens);
-    const size_t smem = (a.d * 2 + 15) / 16 * 16;
     if (a.type == 1)
-        router_kernel<__half><<<grid, 256, smem, s>>>(a, vec);
+        router_kernel<__half><<<grid, 256, 0, s>>>(a, vec);
     else
-        router_kernel<__nv_bfloat16><<<grid, 256, smem, s>>>(a, vec);
+        router_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, vec);
     return cudaGetLastError();
 }
 

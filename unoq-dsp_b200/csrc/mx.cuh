@@ -71,6 +71,111 @@ __device__ __forceinline__ void mx_unpack8(uint32_t codes, float (&v)[8]) {
     }
 }
 
+// Two floats rounded to a pair of 16-bit values, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t mx_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t mx_pair<float>(float, float) { return 0; }  // 32-bit rows take another path
+template <>
+__device__ __forceinline__ uint32_t mx_pair<__half>(float a, float b) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+template <>
+__device__ __forceinline__ uint32_t mx_pair<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+
+// Eight values of a row as they are in memory.
+template <typename T>
+struct MxRaw {   // 16-bit types, two to a word
+    uint32_t w[4];
+    // largest magnitude as its 16 bits (NaN above infinity above every number), and that in 32 bits
+    __device__ __forceinline__ uint32_t top() const {
+        const uint32_t m = __vimax3_u16x2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu,
+                                          __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+        return max(m >> 16, m & 0xFFFFu);
+    }
+    __device__ __forceinline__ static uint32_t top_bits(uint32_t t) {
+        return sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? t << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)t)));
+    }
+    __device__ __forceinline__ void values(float (&v)[8], float scale) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float2 f;
+            if (__is_same(T, __nv_bfloat16)) {
+                f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+            } else {
+                f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            }
+            v[2 * i] = f.x * scale;
+            v[2 * i + 1] = f.y * scale;
+        }
+    }
+    __device__ __forceinline__ void load(const T *p) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    }
+    __device__ __forceinline__ void load_some(const T *p, uint32_t left) {
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            w[i] = (2 * i < left ? h[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+    }
+};
+template <>
+struct MxRaw<float> {
+    uint32_t w[8];
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
+    }
+    __device__ __forceinline__ static uint32_t top_bits(uint32_t t) { return t; }
+    __device__ __forceinline__ void values(float (&v)[8], float scale) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(w[i]) * scale;
+    }
+    __device__ __forceinline__ void load(const float *p) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p)), b = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    }
+    __device__ __forceinline__ void load_some(const float *p, uint32_t left) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) w[i] = i < left ? __float_as_uint(p[i]) : 0u;
+    }
+};
+
+// The same eight columns of n <= ROWS rows, zeros past `left` columns and n rows; `whole`: 16-byte
+// aligned and all inside.
+template <typename T, int ROWS>
+__device__ __forceinline__ void mx_load_rows(MxRaw<T> (&raw)[ROWS], const T *p, uint64_t stride, uint32_t n, uint32_t left,
+                                             bool whole) {
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < ROWS; i++, p += stride) {
+            if ((uint32_t)i < n) raw[i].load(p);
+            else raw[i].load_some(p, 0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; i++, p += stride) raw[i].load_some(p, (uint32_t)i < n ? left : 0);
+    }
+}
+
+// Two floats to two e4m3 bytes (nearest even, saturating), the first in the low byte; their values
+// come back too.
+__device__ __forceinline__ uint32_t mx_e4m3x2(float a, float b, float2 *back) {
+    uint16_t p;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(b), "f"(a));
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(p));
+    *back = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    return p;
+}
+
 // One float to e4m3 (nearest even, saturating) and the value that it stands for.
 __device__ __forceinline__ uint32_t mx_e4m3(float v, float *back) {
     uint16_t p;

@@ -27,8 +27,10 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxStages = 12;
 constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
-constexpr int kCtrlBytes = 2048;   // barriers, TMEM slot and, for the experts, the token list
+constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
 constexpr int kChunk = 32;         // tokens of one expert that one CTA takes
+
+__host__ __device__ constexpr uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
@@ -37,13 +39,13 @@ struct TcArgs {
     uint32_t nt;              // tokens of a full CTA tile
     uint32_t group;           // tokens per 256 rows of pieces (KIND 8, kDense)
     uint32_t stages, split;   // ring depth; CTAs of a cluster that share a tile's K
-    uint32_t stage_bytes, b_bytes, b_box_bytes, tmem_cols, d_cols;
+    uint32_t stage_bytes, b_bytes, b_box_bytes, tmem_cols, d_cols, ring_bytes;
     const uint8_t *w_scales, *x_scales;
     void *y;
     int type;
     uint64_t stride;
     // experts
-    uint32_t experts, top_k, chunks, row_tiles, sfb_bytes;
+    uint32_t top_k, row_tiles, head_bytes;   // head: the choices and the columns' scales
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
@@ -55,9 +57,8 @@ struct Ctrl {
     unsigned long long full[kMaxStages], empty[kMaxStages], done;
     uint32_t tmem;
     int abort;
-    uint32_t chosen_bits[8];
+    unsigned long long rows_ready, scales_ready;
     uint32_t pairs[kChunk];
-    uint32_t count;
     alignas(16) int32_t rows[kChunk * 4];
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
@@ -132,16 +133,16 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
     for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));  // no use moves above the wait
 }
 
-// Eight tokens' values of this thread's weight row: the P columns of each, added in 32 bits, the
+// N tokens' values of this thread's weight row: the P columns of each, added in 32 bits, the
 // smallest piece first.
-template <int P>
-__device__ __forceinline__ void load_tokens(uint32_t addr, float (&v)[8]) {
-    uint32_t r[8 * P];
+template <int P, int N>
+__device__ __forceinline__ void load_tokens(uint32_t addr, float (&v)[N]) {
+    uint32_t r[N * P];
 #pragma unroll
-    for (int p = 0; p < P; p++) tmem_ld8(addr + 8 * p, r + 8 * p);
+    for (int p = 0; p < N * P / 8; p++) tmem_ld8(addr + 8 * p, r + 8 * p);
     tmem_wait(r);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < N; i++) {
         v[i] = __uint_as_float(r[i * P + P - 1]);
 #pragma unroll
         for (int p = P - 2; p >= 0; p--) v[i] += __uint_as_float(r[i * P + p]);
@@ -154,26 +155,51 @@ __device__ __forceinline__ void put_as(void *y, int type, size_t at, float v) {
     else static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
 }
 
+// `count` tokens' values of one weight row (this thread's), rows of y `stride` apart: the 32 lanes of a
+// warp write 32 neighbouring values of a token.
+template <typename T, int N>
+__device__ __forceinline__ void put_tokens(T *p, uint64_t stride, const float (&v)[N], uint32_t count) {
+    if (count >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i++, p += stride) *p = mx_to<T>(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++, p += stride)
+            if ((uint32_t)i < count) *p = mx_to<T>(v[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void put_tokens_as(void *y, int type, size_t at, uint64_t stride, const float (&v)[N], uint32_t count) {
+    if (type == 0) put_tokens(static_cast<float *>(y) + at, stride, v, count);
+    else if (type == 1) put_tokens(static_cast<__half *>(y) + at, stride, v, count);
+    else put_tokens(static_cast<__nv_bfloat16 *>(y) + at, stride, v, count);
+}
+
 template <int KIND, int P, int MODE>
 __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__ CUtensorMap wmap,
                                                          const __grid_constant__ CUtensorMap xmap, const TcArgs a) {
     constexpr uint32_t kA = KIND == 8 ? 16384 : 8192;   // one weight tile in shared memory
-    constexpr uint32_t kMats = MODE == kGateUp ? 2 : 1;  // weight tiles per stage: gate and up
+    constexpr uint32_t kMats = MODE == kGateUp ? 2 : 1;  // weight tiles per step of K: gate and up
     extern __shared__ uint8_t raw[];
     uint8_t *base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     Ctrl &c = *reinterpret_cast<Ctrl *>(base);
-    uint8_t *sfb_all = base + kCtrlBytes;
-    uint8_t *ring = sfb_all + (MODE == kDense ? 0 : a.sfb_bytes);
+    // experts: tokens of each, the chosen expert of every pair, the columns' scales
+    uint32_t *counts = reinterpret_cast<uint32_t *>(base + kCtrlBytes);
+    uint8_t *ids = base + kCtrlBytes + 1024;
+    uint8_t *sfb_all = ids + (MODE == kDense ? 0 : up_to(a.m * a.top_k, kMxScaleTile));
+    uint8_t *ring = base + kCtrlBytes + (MODE == kDense ? 0 : a.head_bytes);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = blockIdx.z;
     volatile int *abort = &c.abort;
 
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < a.stages; i++) {
+        for (uint32_t i = 0; i < kMaxStages; i++) {
             mbar_init(smem_u32(&c.full[i]), 1);
             mbar_init(smem_u32(&c.empty[i]), 1);
         }
         mbar_init(smem_u32(&c.done), 1);
+        mbar_init(smem_u32(&c.rows_ready), 128);
+        mbar_init(smem_u32(&c.scales_ready), 128);
         c.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
@@ -182,96 +208,93 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 
     // ---- what this CTA computes ----
     uint32_t w_tile = blockIdx.x;           // first weight tile along the rows
-    uint32_t tokens, tok0 = 0, expert = 0;  // columns: tokens, or pairs of one expert
+    uint32_t tokens, tok0 = 0, expert = 0, chunk = 0;  // columns: tokens, or a chunk of one expert's pairs
     const uint32_t kt0 = a.kt * rank / a.split, kt1 = a.kt * (rank + 1) / a.split;
     if (MODE == kDense) {
         tok0 = blockIdx.y * a.nt;
         tokens = min(a.nt, a.m - tok0);
     } else {
-        const uint32_t slot = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, pairs = a.m * a.top_k;
-        if (threadIdx.x < 8) c.chosen_bits[threadIdx.x] = 0;
+        // Work items: every chosen expert's tokens in chunks of 32, experts in order. This CTA's item is
+        // found from the choices themselves, in shared memory.
+        const uint32_t pairs = a.m * a.top_k;
+        for (uint32_t i = threadIdx.x; i < 256; i += kThreads) counts[i] = 0;
         __syncthreads();
         grid_dep_wait();  // the router's choice, or the hidden vectors, of the kernel before
+#pragma unroll 4
         for (uint32_t i = threadIdx.x; i < pairs; i += kThreads) {
             const uint32_t e = (uint32_t)__ldcg(a.chosen + i);
-            atomicOr(&c.chosen_bits[e / 32 % 8], 1u << (e % 32));
+            ids[i] = (uint8_t)e;
+            atomicAdd(&counts[e % 256], 1u);
         }
         __syncthreads();
-        // the slot-th chosen expert
-        uint32_t left = slot;
-        expert = 0xFFFFFFFFu;
-        for (int w = 0; w < 8 && expert == 0xFFFFFFFFu; w++) {
-            const uint32_t bits = c.chosen_bits[w], here = __popc(bits);
-            if (left < here) expert = w * 32 + __fns(bits, 0, left + 1);
-            else left -= here;
+        uint32_t n[8], items = 0;   // every warp on its own: a lane has eight experts
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            n[i] = counts[lane * 8 + i];
+            items += (n[i] + kChunk - 1) / kChunk;
         }
-        if (expert == 0xFFFFFFFFu) return;  // the same in the whole cluster
-        if (warp == 0) {  // its pairs, in order
-            uint32_t found = 0;
-            for (uint32_t i = 0; i < pairs; i += 32) {
-                const bool hit = i + lane < pairs && (uint32_t)__ldcg(a.chosen + i + lane) == expert;
-                const uint32_t mask = __ballot_sync(~0u, hit);
-                const uint32_t at = found + __popc(mask & ((1u << lane) - 1));
-                if (hit && at / kChunk == chunk) c.pairs[at % kChunk] = i + lane;
-                found += __popc(mask);
+        uint32_t upto = items;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const uint32_t below = __shfl_up_sync(~0u, upto, o);
+            if (lane >= o) upto += below;
+        }
+        const uint32_t item = blockIdx.y, holders = __ballot_sync(~0u, item < upto);
+        if (!holders) return;  // the same in the whole cluster
+        uint32_t left = item - (upto - items), found = 0, here = 0;
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t chunks = (n[i] + kChunk - 1) / kChunk;
+            if (open && left < chunks) {
+                found = lane * 8 + i;
+                here = n[i];
+                open = false;
             }
-            if (lane == 0) c.count = found > chunk * kChunk ? min(found - chunk * kChunk, (uint32_t)kChunk) : 0;
+            if (open) left -= chunks;
         }
-        __syncthreads();
-        tokens = c.count;
-        if (!tokens) return;
+        const int holder = __ffs(holders) - 1;
+        expert = __shfl_sync(~0u, found, holder);
+        chunk = __shfl_sync(~0u, left, holder);
+        tokens = min(__shfl_sync(~0u, here, holder) - chunk * kChunk, (uint32_t)kChunk);
         w_tile = (expert * a.row_tiles + blockIdx.x) * kMats;
     }
     const uint32_t n_cols = (tokens * P + 7) / 8 * 8;
     const uint32_t sfb_tiles = MODE == kDense ? (n_cols + 127) / 128 : 1;
-    const uint32_t sf_cols = 4 * kMats + (a.nt * P > 128 ? 8 : 4);
+    const uint32_t sf_cols = 4 + (a.nt * P > 128 ? 8 : 4);
+    // the experts' ring is as deep as this expert's few tokens allow
+    const uint32_t b_bytes = MODE == kDense ? a.b_bytes : n_cols * 128;
+    const uint32_t stage_bytes = MODE == kDense ? a.stage_bytes : kA + 1024 + b_bytes;
+    const uint32_t stages = MODE == kDense ? a.stages : min(a.stages, a.ring_bytes / stage_bytes);
 
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
                      "r"(a.tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (MODE != kDense) {
-        // the columns' rows of pieces, and all their scales of this CTA's share of K
-        for (uint32_t i = threadIdx.x; i < n_cols; i += kThreads) {
-            const uint32_t t = min(i / P, tokens - 1);  // columns past the last token repeat it
-            const uint32_t src = MODE == kGateUp ? c.pairs[t] / a.top_k : c.pairs[t];
-            const uint32_t row = src * P + (i / P < tokens ? i % P : 0);
-            c.rows[i] = (int32_t)row;
-            const uint32_t *s = reinterpret_cast<const uint32_t *>(a.x_scales) + (size_t)row * a.kt;
-            for (uint32_t t2 = kt0; t2 < kt1; t2++)
-                *reinterpret_cast<uint32_t *>(sfb_all + (t2 - kt0) * kMxScaleTile + i % 32 * 16 + i / 32 * 4) = __ldcg(s + t2);
-        }
-        fence_proxy_async();  // read by the tensor core's scale copy
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (MODE == kGateUp) grid_dep_launch();  // every CTA holds its TMEM: the next kernel's may come
     const uint32_t tmem = c.tmem;
-    const uint32_t iters = kt1 - kt0;
+    const uint32_t steps = kt1 - kt0, iters = steps * kMats;   // gate and up tiles of a step follow each other
 
     if (warp == 0 && lane == 0) {
         // ---- TMA ----
         // a copy that unpacks counts the bytes that it read, 64 a row, for either kind
-        const uint32_t stage_tx = kMats * (kMxCodeTile + kMxScaleTile) +
+        const uint32_t stage_tx = kMxCodeTile + kMxScaleTile +
                                   (MODE == kDense ? (KIND == 8 ? a.b_box_bytes : sfb_tiles * a.b_box_bytes) + sfb_tiles * kMxScaleTile
                                                   : n_cols * 128);
-        auto load_w = [&](uint32_t it) {
-            const uint32_t s = it % a.stages, bar = smem_u32(&c.full[s]);
-            const uint32_t st = smem_u32(ring + s * a.stage_bytes), sf = st + kMats * kA + a.b_bytes;
+        auto load_w = [&](uint32_t it, uint32_t s) {
+            const uint32_t bar = smem_u32(&c.full[s]), st = smem_u32(ring + s * stage_bytes);
             mbar_expect(bar, stage_tx);
-#pragma unroll
-            for (uint32_t i = 0; i < kMats; i++) {
-                const size_t t = (size_t)(w_tile + i) * a.kt + kt0 + it;
-                tma_2d(st + i * kA, &wmap, 0, (int)(t * 128), bar);
-                bulk_copy(sf + i * kMxScaleTile, a.w_scales + t * kMxScaleTile, kMxScaleTile, bar);
-            }
+            const size_t t = (size_t)(w_tile + it % kMats) * a.kt + kt0 + it / kMats;
+            tma_2d(st, &wmap, 0, (int)(t * 128), bar);
+            bulk_copy(st + kA + b_bytes, a.w_scales + t * kMxScaleTile, kMxScaleTile, bar);
         };
-        auto load_x = [&](uint32_t it) {
-            const uint32_t s = it % a.stages, bar = smem_u32(&c.full[s]);
-            const uint32_t st = smem_u32(ring + s * a.stage_bytes), b = st + kMats * kA, sf = b + a.b_bytes + kMats * kMxScaleTile;
-            const uint32_t k = kt0 + it;
+        auto load_x = [&](uint32_t it, uint32_t s) {
+            const uint32_t bar = smem_u32(&c.full[s]), b = smem_u32(ring + s * stage_bytes) + kA;
+            const uint32_t sf = b + b_bytes + kMxScaleTile, k = kt0 + it / kMats;
             if (MODE != kDense) {
                 for (uint32_t i = 0; i < n_cols; i += 4)
                     tma_gather4(b + i * 128, &xmap, (int)(k * 128), *reinterpret_cast<const int4 *>(&c.rows[i]), bar);
@@ -289,59 +312,84 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
         };
         // weights do not depend on the kernel before: the ring's first round of them goes out at once
-        const uint32_t ahead = min(a.stages, iters);
-        uint32_t issued = ahead;
-        for (uint32_t it = 0; it < ahead; it++) load_w(it);
+        const uint32_t ahead = min(stages, iters);
+        for (uint32_t it = 0; it < ahead; it++) load_w(it, it);
         if (MODE == kDense && KIND == 8) grid_dep_wait();  // the pieces
-        for (uint32_t it = 0; it < ahead; it++) load_x(it);
-        for (uint32_t it = ahead; it < iters; it++) {
-            if (!mbar_wait(smem_u32(&c.empty[it % a.stages]), (it / a.stages & 1) ^ 1, abort, 601)) break;
-            load_w(it);
-            load_x(it);
-            issued = it + 1;
+        const bool listed = MODE == kDense || mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605);
+        if (listed)
+            for (uint32_t it = 0; it < ahead; it++) load_x(it, it);
+        uint32_t s = 0, phase = 0, issued = ahead;   // stage and round of the next copy's wait
+        for (; listed && issued < iters; issued++) {
+            if (!mbar_wait(smem_u32(&c.empty[s]), phase, abort, 601)) break;
+            load_w(issued, s);
+            load_x(issued, s);
+            if (++s == stages) s = 0, phase ^= 1;
         }
         if (*abort)  // no copy may land after this CTA has left
-            for (uint32_t it = issued > a.stages ? issued - a.stages : 0; it < issued; it++)
-                for (int i = 0; i < 1000 && !mbar_try_wait(smem_u32(&c.full[it % a.stages]), it / a.stages & 1, 1000000); i++) {
+            for (uint32_t it = issued > stages ? issued - stages : 0; it < issued; it++)
+                for (int i = 0; i < 1000 && !mbar_try_wait(smem_u32(&c.full[it % stages]), it / stages & 1, 1000000); i++) {
                 }
     } else if (warp == 1 && lane == 0) {
         // ---- MMA ----
-        const uint32_t sf_tmem = tmem + a.d_cols * kMats;
-        bool ok = true;
-        for (uint32_t it = 0; it < iters; it++) {
-            const uint32_t s = it % a.stages;
-            if (!mbar_wait(smem_u32(&c.full[s]), it / a.stages & 1, abort, 602)) {
+        const uint32_t sf_tmem = tmem + a.d_cols * kMats, idesc = scaled_instr_desc<KIND>(n_cols);
+        bool ok = MODE == kDense || mbar_wait(smem_u32(&c.scales_ready), 0, abort, 606);
+        uint32_t s = 0, phase = 0;
+        for (uint32_t it = 0; ok && it < iters; it++) {
+            if (!mbar_wait(smem_u32(&c.full[s]), phase, abort, 602)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t st = smem_u32(ring + s * a.stage_bytes), b = st + kMats * kA, sf = b + a.b_bytes;
+            const uint32_t st = smem_u32(ring + s * stage_bytes), b = st + kA, sf = b + b_bytes;
             // each stage has scale columns of its own: they are rewritten only after its MMAs are done
-            const uint32_t sfa = sf_tmem + s * sf_cols, sfb = sfa + 4 * kMats;
-#pragma unroll
-            for (uint32_t i = 0; i < kMats; i++) scales_to_tmem(sfa + 4 * i, sf + i * kMxScaleTile);
+            const uint32_t sfa = sf_tmem + s * sf_cols, sfb = sfa + 4;
+            scales_to_tmem(sfa, sf);
             if (MODE == kDense)
-                for (uint32_t i = 0; i < sfb_tiles; i++) scales_to_tmem(sfb + 4 * i, sf + (kMats + i) * kMxScaleTile);
+                for (uint32_t i = 0; i < sfb_tiles; i++) scales_to_tmem(sfb + 4 * i, sf + (1 + i) * kMxScaleTile);
             else
-                scales_to_tmem(sfb, smem_u32(sfb_all + it * kMxScaleTile));
-            const uint64_t bd = operand_desc<KIND>(b);
-            const uint32_t idesc = scaled_instr_desc<KIND>(n_cols);
+                scales_to_tmem(sfb, smem_u32(sfb_all + it / kMats * kMxScaleTile));
+            const uint64_t ad = operand_desc<KIND>(st), bd = operand_desc<KIND>(b);
+            const uint32_t d = tmem + it % kMats * a.d_cols;
 #pragma unroll
-            for (uint32_t i = 0; i < kMats; i++) {
-                const uint64_t ad = operand_desc<KIND>(st + i * kA);
-#pragma unroll
-                for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
-                    const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
-                    mma_scaled<KIND>(tmem + i * a.d_cols, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa + 4 * i, sfb,
-                                     it | j);
-                }
+            for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
+                const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
+                mma_scaled<KIND>(d, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa, sfb, it >= kMats || j);
             }
             mma_commit(smem_u32(&c.empty[s]));
+            if (++s == stages) s = 0, phase ^= 1;
         }
         mma_commit(smem_u32(&c.done));
         if (!ok) mbar_wait(smem_u32(&c.done), 0, &c.abort, 603);
     }
     __syncwarp();
+    if (MODE != kDense && warp >= 2) {
+        // ---- the columns: which rows of pieces, and all their scales of this CTA's share of K ----
+        const uint32_t at = threadIdx.x - 64, pairs = a.m * a.top_k;
+        if (warp == 2) {   // the expert's pairs of this chunk, in order
+            uint32_t seen = 0;
+            for (uint32_t i = 0; i < pairs; i += 32) {
+                const bool hit = i + lane < pairs && ids[i + lane] == expert;
+                const uint32_t mask = __ballot_sync(~0u, hit), to = seen + __popc(mask & ((1u << lane) - 1));
+                if (hit && to / kChunk == chunk) c.pairs[to % kChunk] = i + lane;
+                seen += __popc(mask);
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        auto row_of = [&](uint32_t i) {   // columns past the last token repeat it
+            const uint32_t pair = c.pairs[min(i / P, tokens - 1)];
+            return (MODE == kGateUp ? pair / a.top_k : pair) * P + (i / P < tokens ? i % P : 0);
+        };
+        if (at < n_cols) c.rows[at] = (int32_t)row_of(at);
+        mbar_arrive(smem_u32(&c.rows_ready));
+#pragma unroll 4
+        for (uint32_t j = at; j < n_cols * steps; j += 128) {
+            const uint32_t i = j / steps, t = j - i * steps;
+            *reinterpret_cast<uint32_t *>(sfb_all + t * kMxScaleTile + i % 32 * 16 + i / 32 * 4) =
+                __ldcg(reinterpret_cast<const uint32_t *>(a.x_scales) + (size_t)row_of(i) * a.kt + kt0 + t);
+        }
+        fence_proxy_async();  // read by the tensor core's scale copy
+        mbar_arrive(smem_u32(&c.scales_ready));
+    }
 
     // ---- epilogue: thread = weight row ----
     const uint32_t q = warp % 4, row = blockIdx.x * 128 + q * 32 + lane;
@@ -368,21 +416,29 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 if (lane == 0) a.h_scales[(r + p) * kt * 4 + row / 32] = (uint8_t)mx_piece_scale_of(s, p);
             }
         } else {
-            // Weighted, to the pair's own place; the warp whose pair comes last for a token adds the
-            // token's top_k parts in their order, so the sum does not depend on who that is.
-            const uint32_t pair = c.pairs[i], t = pair / a.top_k;
-            if (row < a.n) a.partial[(size_t)pair * a.n + row] = g * __ldcg(a.weight + pair);
-            __threadfence();
-            __syncwarp();
-            uint32_t before = 0;
-            if (lane == 0) before = atomicAdd(a.arrived + ((size_t)t * a.row_tiles + blockIdx.x) * 4 + q, 1u);
-            if (__shfl_sync(~0u, before, 0) == a.top_k - 1) {
-                __threadfence();
-                if (row < a.n) {
-                    float sum = 0.0f;
-                    for (uint32_t j = 0; j < a.top_k; j++) sum += __ldcg(a.partial + (size_t)(t * a.top_k + j) * a.n + row);
-                    put_as(a.y, a.type, t * a.stride + row, sum);
-                }
+            if (row < a.n) a.partial[(size_t)c.pairs[i] * a.n + row] = g * __ldcg(a.weight + c.pairs[i]);
+        }
+    };
+    // Down products lie weighted in their pairs' places. The warp that brings a token's last pair of
+    // these 32 rows adds the token's top_k parts in their order, so the sum does not depend on
+    // who that is. Lane i counts token i in: one fence and one round of atomics for all of them.
+    auto combine = [&](uint32_t first, uint32_t step) {
+        __threadfence();
+        __syncwarp();
+        const uint32_t i = first + lane * step;
+        const uint32_t t = i < tokens ? c.pairs[i] / a.top_k : 0;
+        const bool last = i < tokens && atomicAdd(a.arrived + ((size_t)t * a.row_tiles + blockIdx.x) * 4 + q, 1u) == a.top_k - 1;
+        uint32_t mask = __ballot_sync(~0u, last);
+        __threadfence();
+        while (mask) {
+            const uint32_t to = __shfl_sync(~0u, t, __ffs(mask) - 1);
+            mask &= mask - 1;
+            if (row < a.n) {
+                const float *part = a.partial + (size_t)to * a.top_k * a.n + row;
+                float sum = 0.0f;
+#pragma unroll 8
+                for (uint32_t j = 0; j < a.top_k; j++) sum += __ldcg(part + (size_t)j * a.n);
+                put_as(a.y, a.type, to * a.stride + row, sum);
             }
         }
     };
@@ -391,21 +447,37 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         mbar_wait(smem_u32(&c.done), 0, abort, 604);
         tc_fence_after();
         const uint32_t taddr = tmem + (q * 32 << 16);
-        for (uint32_t i0 = 0; i0 < tokens; i0 += 8) {
-            float g[8], u[8];
-            load_tokens<P>(taddr + i0 * P, g);
-            if (MODE == kGateUp) load_tokens<P>(taddr + a.d_cols + i0 * P, u);
+        if (MODE == kDense && a.split == 1) {
+            constexpr uint32_t kAt = P == 1 ? 32 : P == 2 ? 16 : 8;   // tokens at a time: up to 32 columns
+            uint32_t i0 = 0;
+            for (; i0 + kAt <= up_to(tokens, 8); i0 += kAt) {
+                float v[kAt];
+                load_tokens<P>(taddr + i0 * P, v);
+                if (row < a.n) put_tokens_as(a.y, a.type, (tok0 + i0) * a.stride + row, a.stride, v, tokens - i0);
+            }
+            for (; i0 < tokens; i0 += 8) {
+                float v[8];
+                load_tokens<P>(taddr + i0 * P, v);
+                if (row < a.n) put_tokens_as(a.y, a.type, (tok0 + i0) * a.stride + row, a.stride, v, tokens - i0);
+            }
+        } else {
+            for (uint32_t i0 = 0; i0 < tokens; i0 += 8) {
+                float g[8], u[8];
+                load_tokens<P>(taddr + i0 * P, g);
+                if (MODE == kGateUp) load_tokens<P>(taddr + a.d_cols + i0 * P, u);
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                if (i0 + i >= tokens) break;
-                if (a.split == 1) {
-                    finish(i0 + i, g[i], MODE == kGateUp ? u[i] : 0.0f);
-                } else {
-                    red[(i0 + i) * 128 + q * 32 + lane] = g[i];
-                    if (MODE == kGateUp) red[(a.nt + i0 + i) * 128 + q * 32 + lane] = u[i];
+                for (uint32_t i = 0; i < 8; i++) {
+                    if (i0 + i >= tokens) break;
+                    if (MODE != kDense && a.split == 1) {
+                        finish(i0 + i, g[i], MODE == kGateUp ? u[i] : 0.0f);
+                    } else {
+                        red[(i0 + i) * 128 + q * 32 + lane] = g[i];
+                        if (MODE == kGateUp) red[(a.nt + i0 + i) * 128 + q * 32 + lane] = u[i];
+                    }
                 }
             }
         }
+        if (MODE == kDown && a.split == 1) combine(0, 1);
         tc_fence_before();
     }
     if (a.split > 1) {
@@ -423,7 +495,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 finish(i, g, u);
             }
         __syncwarp();
-        cluster.sync();
+        cluster.barrier_arrive();   // this CTA reads the others' shared memory no more
+        if (MODE == kDown && epi) combine(rank, a.split);
+        __syncwarp();
+        cluster.barrier_wait();
     }
     __syncthreads();
     if (warp == 1) {
@@ -434,59 +509,45 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 
 // ---- activation pieces of a dense product ---------------------------------------------------------
 //
-// 16 lanes take one row's 128 values, 8 each (as the quantiser does), and write P rows of e4m3.
-// Token t's pieces are rows t / group * 256 + t % group * P + p, so that a full tile of tokens
-// starts on a scale tile.
+// The quantiser's division of work (k_mx.cu): a warp takes 256 columns of ROWS tokens and writes P
+// rows of e4m3 for each. Token t's pieces are rows t / group * 256 + t % group * P + p, so that a
+// full tile of tokens starts on a scale tile.
 
-template <typename T, int P>
+template <typename T, int P, int ROWS>
 __global__ void __launch_bounds__(256) pieces_kernel(const T *x, uint32_t m, uint32_t k, uint64_t stride, uint32_t kt,
-                                                     uint32_t group, uint8_t *pieces, uint8_t *scales, bool vec) {
+                                                     uint32_t chunks, uint32_t group, uint8_t *pieces, uint8_t *scales, bool vec) {
     grid_dep_launch();  // the product may start on its weights
-    const uint32_t lane = threadIdx.x % 16, units = m * kt;
-    const uint32_t step = gridDim.x * (blockDim.x / 16), first = (blockIdx.x * blockDim.x + threadIdx.x) / 16;
-    for (uint32_t base = first & ~1u; base < units; base += step) {
-        const uint32_t un = base + (first & 1u);
-        const bool live = un < units;
-        const uint32_t t = live ? un / kt : 0, tile = live ? un - t * kt : 0, j = tile * kMxTile + lane * 8;
-        const uint32_t left = live && j < k ? k - j : 0;
-        const T *src = x + t * stride + j;
-        float v[8];
-        if (vec && left >= 8) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src));
-            const T *h = reinterpret_cast<const T *>(&w);
+    const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
+    const uint32_t tokens = w / chunks, chunk = w - tokens * chunks, t0 = tokens * ROWS;
+    if (t0 >= m) return;
+    const uint32_t n = min((uint32_t)ROWS, m - t0), j = chunk * 256 + lane * 8;
+    MxRaw<T> raw[ROWS];
+    mx_load_rows<T, ROWS>(raw, x + t0 * stride + j, stride, n, j < k ? k - j : 0, vec && chunk * 256 + 256 <= k);
+    uint32_t r = t0 / group * 256 + t0 % group * P;   // ROWS divides the group: the rows follow each other
+    uint8_t *to = pieces + (size_t)r * kt * 128 + j;
+    const bool mine = j / kMxTile < kt;
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = mx_float(h[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = (uint32_t)i < left ? mx_float(src[i]) : 0.0f;
-        }
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);  // NaN above infinity above all
+    for (int i = 0; i < ROWS; i++) {
+        if ((uint32_t)i >= n) break;
+        uint32_t top = raw[i].top();
         top = max(top, __shfl_xor_sync(~0u, top, 1));
         top = max(top, __shfl_xor_sync(~0u, top, 2));
-        const uint32_t s = mx_piece_scale(__uint_as_float(top), P);
-        const float inverse = __uint_as_float((254u - min(s, 253u)) << 23);
+        const uint32_t s = mx_piece_scale(__uint_as_float(raw[i].top_bits(top)), P);
+        float v[8];
+        raw[i].values(v, __uint_as_float((254u - min(s, 253u)) << 23));
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= inverse;
-        const uint32_t row = t / group * 256 + t % group * P;
+        for (int p = 0; p < P; p++, r++, to += (size_t)kt * 128) {
+            uint32_t h[4];
 #pragma unroll
-        for (int p = 0; p < P; p++) {
-            uint32_t w[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float back;
-                w[i / 4] |= mx_e4m3(v[i], &back) << (i % 4 * 8);
-                v[i] = (v[i] - back) * 16.0f;
+            for (int b = 0; b < 4; b++) {
+                float2 back;
+                h[b] = mx_e4m3x2(v[2 * b], v[2 * b + 1], &back);
+                v[2 * b] = (v[2 * b] - back.x) * 16.0f;
+                v[2 * b + 1] = (v[2 * b + 1] - back.y) * 16.0f;
             }
-            const uint32_t sp = mx_piece_scale_of(s, p);
-            uint32_t all = sp | __shfl_down_sync(~0u, sp, 4) << 8;
-            all |= __shfl_down_sync(~0u, all, 8) << 16;
-            if (live) {
-                const uint32_t r = row + p;
-                *reinterpret_cast<uint2 *>(pieces + ((size_t)r * kt + tile) * 128 + lane * 8) =
-                    s == 255 ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
-                if (lane == 0) *reinterpret_cast<uint32_t *>(scales + mx_scale_at(r, tile * 4, kt)) = all;
+            if (mine) {
+                *reinterpret_cast<uint2 *>(to) = s == 255 ? make_uint2(0, 0) : make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+                if (lane % 4 == 0) scales[mx_scale_at(r, j / 32, kt)] = (uint8_t)mx_piece_scale_of(s, p);
             }
         }
     }
@@ -513,7 +574,6 @@ cudaError_t encode_weights(CUtensorMap *map, const uint8_t *codes, uint64_t tile
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 64, tiles * 128, 64, 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 uint32_t pow2_cols(uint32_t v) {
     uint32_t c = 32;
     while (c < v) c *= 2;
@@ -551,18 +611,26 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t mats = MODE == kGateUp ? 2 : 1, n = up_to(a.nt * P, 8);
     // KIND 4 copies whole boxes of 128 rows past the first 128 columns
     a.b_bytes = KIND == 8 ? n * 128 : n <= 128 ? up_to(n * 64, 1024) : up_to(n, 128) * 64;
-    const uint32_t sf = kMxScaleTile * (mats + (MODE == kDense ? (n + 127) / 128 : 0));
-    a.stage_bytes = up_to(mats * (KIND == 8 ? 16384 : 8192) + a.b_bytes + sf, 1024);
+    const uint32_t sf = kMxScaleTile * (1 + (MODE == kDense ? (n + 127) / 128 : 0));
+    a.stage_bytes = (KIND == 8 ? 16384 : 8192) + a.b_bytes + up_to(sf, 1024);
     a.d_cols = up_to(a.nt, 8) * P;
-    const uint32_t sf_cols = 4 * mats + (a.nt * P > 128 ? 8 : 4);
-    const uint32_t extra = 1024 + kCtrlBytes + a.sfb_bytes;
-    const uint32_t budget = (per_sm == 1 ? 226 : per_sm == 2 ? 112 : 74) * 1024 - extra;
-    const uint32_t cols = per_sm == 1 ? 512 : per_sm == 2 ? 256 : 128;
-    a.stages = std::min<uint32_t>({budget / a.stage_bytes, (cols - a.d_cols * mats) / sf_cols, (uint32_t)kMaxStages,
-                                   std::max(1u, (a.kt + a.split - 1) / a.split)});
+    const uint32_t sf_cols = 4 + (a.nt * P > 128 ? 8 : 4);
+    const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
+    const uint32_t budget = (per_sm == 1 ? 226 : 112) * 1024 - extra;
+    const uint32_t cols = per_sm == 1 ? 512 : 256;
+    const uint32_t iters = (a.kt + a.split - 1) / a.split * mats;
+    a.stages = std::min({(cols - a.d_cols * mats) / sf_cols, (uint32_t)kMaxStages, iters});
+    if (MODE == kDense) {
+        a.stages = std::min(a.stages, budget / a.stage_bytes);
+        a.ring_bytes = a.stages * a.stage_bytes;
+    } else {   // the kernel fits its stages into this by its expert's number of tokens
+        const uint32_t least = (KIND == 8 ? 16384 : 8192) + 2048;
+        a.ring_bytes = std::max(std::min(budget, a.stages * a.stage_bytes), a.stage_bytes);
+        a.stages = std::min(a.stages, a.ring_bytes / least);
+    }
     a.tmem_cols = pow2_cols(a.d_cols * mats + a.stages * sf_cols);
     const uint32_t red = a.split > 1 ? mats * a.nt * 128 * 4 : 0;
-    return extra + std::max(a.stages * a.stage_bytes, red);
+    return extra + std::max(a.ring_bytes, red);
 }
 
 template <int KIND, int P>
@@ -606,14 +674,17 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
 
 template <typename T, int P>
 cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
-    const uint32_t kt = mx_tiles(p.k), units = p.m * kt;
+    const uint32_t kt = mx_tiles(p.k), chunks = (p.k + 255) / 256;
     constexpr uint32_t kGroup = P == 2 ? 128 : 64;
     uint8_t *pieces = static_cast<uint8_t *>(p.workspace);
     const size_t rows = mx_piece_rows(p.m, p.x_type);
     uint8_t *scales = pieces + (rows * kt * 128 + 255) / 256 * 256;
     const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.x_stride % 8 == 0;
-    const unsigned grid = std::min<unsigned>((units + 15) / 16, 148 * 8);
-    pieces_kernel<T, P><<<grid, 256, 0, s>>>(static_cast<const T *>(p.x), p.m, p.k, p.x_stride, kt, kGroup, pieces, scales, vec);
+    const bool many = (uint64_t)(p.m / 4) * chunks >= 148 * 64;   // as the quantiser's rule
+    const uint64_t warps = many ? (uint64_t)((p.m + 3) / 4) * chunks : (uint64_t)p.m * chunks;
+    auto kernel = many ? pieces_kernel<T, P, 4> : pieces_kernel<T, P, 1>;
+    kernel<<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(static_cast<const T *>(p.x), p.m, p.k, p.x_stride, kt, chunks, kGroup,
+                                                       pieces, scales, vec);
     const cudaError_t e = cudaGetLastError();
     return e != cudaSuccess ? e : dense<8, P>(p, pieces, scales, s);
 }
@@ -627,8 +698,6 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.kt = mx_tiles(width);
     a.row_tiles = mx_tiles(rows);
     a.nt = std::min<uint32_t>(e.tokens, kChunk);
-    a.chunks = (e.tokens + kChunk - 1) / kChunk;
-    a.experts = e.experts;
     a.top_k = e.top_k;
     a.chosen = e.ws.chosen;
     a.weight = e.ws.weight;
@@ -641,12 +710,13 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.y = e.y;
     a.type = e.type;
     a.stride = e.y_stride;
-    const uint32_t slots = std::min(e.experts, e.tokens * e.top_k);
+    // as many items as there can be: one to each chosen expert, one more for every further 32 pairs
+    const uint32_t pairs = e.tokens * e.top_k, slots = std::min(e.experts, pairs), items = slots + (pairs - slots) / kChunk;
     a.split = 1;
     while (a.split < 8 && a.kt / (a.split * 2) >= 2 &&
            (a.row_tiles * slots * a.split * 2 <= 148 * 2 || a.kt / a.split > 32))
         a.split *= 2;
-    a.sfb_bytes = up_to((a.kt + a.split - 1) / a.split * kMxScaleTile, 1024);
+    a.head_bytes = up_to(1024 + up_to(pairs, kMxScaleTile) + (a.kt + a.split - 1) / a.split * kMxScaleTile, 1024);
     const uint32_t smem = plan_ring<8, P, MODE>(a, 2);
     const uint32_t mats = MODE == kGateUp ? 2 : 1;
     CUtensorMap wmap, xmap;
@@ -657,7 +727,7 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.kt * 128,
                piece_rows, (uint64_t)a.kt * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
-    return launch<8, P, MODE>(wmap, xmap, a, dim3(a.row_tiles, slots * a.chunks, a.split), smem, true, s);
+    return launch<8, P, MODE>(wmap, xmap, a, dim3(a.row_tiles, items, a.split), smem, true, s);
 }
 
 }  // namespace

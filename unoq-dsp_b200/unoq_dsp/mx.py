@@ -49,7 +49,8 @@ def _check(lib, rc, what):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    # the current stream's handle without building a Stream object (which costs as much as a launch)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _input(x, what, types):
@@ -64,22 +65,28 @@ def _input(x, what, types):
 
 
 def _rows(x, what):
-    """x as rows of contiguous values: (rows, k) with any row stride; copied only where it has to be."""
-    if x.dim() < 1 or x.shape[-1] < 1:
+    """(x as rows of contiguous values, rows, k, row stride); copied only where it has to be."""
+    if x.dim() != 2:
+        if x.dim() < 1 or x.shape[-1] < 1:
+            raise ValueError(f"{what} needs at least one value in its last axis")
+        x = x.reshape(-1, x.shape[-1])
+    rows, k = x.shape
+    if k < 1:
         raise ValueError(f"{what} needs at least one value in its last axis")
-    x = x.reshape(-1, x.shape[-1])
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()
-    return x
+    row, step = x.stride()
+    if rows < 2:
+        row = k
+    if (step != 1 and k > 1) or row < k:
+        x, row = x.contiguous(), k
+    return x, rows, k, row
 
 
-def _row_stride(x):
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+def _row_stride(x, rows, k):
+    return x.stride(0) if rows > 1 else max(k, 1)
 
 
 def _output(out, shape, dtype, device, inputs):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+    """Refuse an `out` that the kernels cannot write."""
     if not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.device != device:
         raise ValueError(f"out must be a tensor of shape {tuple(shape)} on {device}")
     if out.dtype != dtype:
@@ -94,7 +101,6 @@ def _output(out, shape, dtype, device, inputs):
     for x in inputs:
         if lo < x.data_ptr() + _extent(x) and x.data_ptr() < hi:
             raise ValueError("out must not overlap an input")
-    return out
 
 
 def _extent(x):
@@ -104,42 +110,55 @@ def _extent(x):
     return (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
 
 
+def _sizes(operand, rows, k):
+    """Bytes of the codes and of the scales (ug_mx4_codes_bytes, ug_mx4_scales_bytes)."""
+    if operand:
+        tiles = -(-rows // 128) * -(-k // 128)
+        return tiles * 8192, tiles * 512
+    return rows * ((k + 1) // 2), rows * ((k + 31) // 32)
+
+
 class MX4:
     """A matrix of ``rows`` x ``k`` 4-bit values with a scale per 32: ``codes`` and ``scales`` (uint8)
     in the ``layout`` ``"operand"`` (what :func:`matmul` reads) or ``"stored"`` (row-major, the form of
     files: (rows, ceil(k/2)) and (rows, ceil(k/32)))."""
 
-    __slots__ = ("codes", "scales", "rows", "k", "layout")
+    __slots__ = ("codes", "scales", "rows", "k", "layout", "device")
 
     def __init__(self, codes, scales, rows, k, layout="operand"):
-        lib = _library()
-        code = _layout(layout)
-        for x, want, name in ((codes, lib.ug_mx4_codes_bytes(code, rows, k), "codes"),
-                              (scales, lib.ug_mx4_scales_bytes(code, rows, k), "scales")):
+        if rows < 0 or k < 1:
+            raise ValueError("rows must be 0 or more and k 1 or more")
+        for x, want, name in zip((codes, scales), _sizes(_layout(layout), rows, k), ("codes", "scales")):
             _input(x, name, (torch.uint8,))
             if not x.is_contiguous() or x.numel() != want:
                 raise ValueError(f"{name} must be {want} contiguous bytes")
         if codes.device != scales.device:
             raise ValueError("codes and scales are on two devices")
-        self.codes, self.scales, self.rows, self.k, self.layout = codes, scales, rows, k, layout
+        self._set(codes, scales, rows, k, layout, codes.device)
+
+    def _set(self, *fields):
+        self.codes, self.scales, self.rows, self.k, self.layout, self.device = fields
+        return self
 
     @property
     def shape(self):
         return (self.rows, self.k)
 
-    @property
-    def device(self):
-        return self.codes.device
-
     def dequantize(self, dtype=torch.bfloat16, out=None):
         """The values, (rows, k), rounded to ``dtype`` once."""
         if dtype not in _TYPES:
             raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
-        lib = _library()
-        out = _output(out, (self.rows, self.k), dtype, self.device, (self.codes, self.scales))
-        _check(lib, lib.ug_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _layout(self.layout), self.rows,
-                                          self.k, out.data_ptr(), _TYPES[dtype], _row_stride(out), _stream(self.device)),
-               "MX4 dequantise")
+        lib, rows, k, device = _library(), self.rows, self.k, self.device
+        stride = k
+        if out is None:
+            out = torch.empty((rows, k), dtype=dtype, device=device)
+        else:
+            _output(out, (rows, k), dtype, device, (self.codes, self.scales))
+            stride = _row_stride(out, rows, k)
+        rc = lib.ug_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _layout(self.layout), rows, k,
+                                   out.data_ptr(), _TYPES[dtype], stride, _stream(device))
+        if rc:
+            _check(lib, rc, "MX4 dequantise")
         return out
 
 
@@ -153,16 +172,19 @@ def quantize(x, layout="operand"):
     """(..., k) values in 32 or 16 bits -> :class:`MX4` of their rows. Each block of 32 gets the scale
     2^(floor(log2 of its largest magnitude) - 2); values go to the nearest e2m1 (ties to even), at
     most 6 scales; a block holding a NaN or an infinity becomes NaN."""
-    x = _rows(_input(x, "x", tuple(_TYPES)), "x")
-    lib, code = _library(), _layout(layout)
-    rows, k = x.shape
-    codes = torch.empty(lib.ug_mx4_codes_bytes(code, rows, k), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(lib.ug_mx4_scales_bytes(code, rows, k), dtype=torch.uint8, device=x.device)
-    _check(lib, lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, _row_stride(x), code, codes.data_ptr(),
-                                    scales.data_ptr(), _stream(x.device)), "MX4 quantise")
-    if layout == "stored":
-        codes, scales = codes.view(rows, (k + 1) // 2), scales.view(rows, (k + 31) // 32)
-    return MX4(codes, scales, rows, k, layout)
+    x, rows, k, stride = _rows(_input(x, "x", _TYPES), "x")
+    lib, code, device = _library(), _layout(layout), x.device
+    if code:
+        shapes = _sizes(code, rows, k)
+    else:
+        shapes = (rows, (k + 1) // 2), (rows, (k + 31) // 32)
+    codes = torch.empty(shapes[0], dtype=torch.uint8, device=device)
+    scales = torch.empty(shapes[1], dtype=torch.uint8, device=device)
+    rc = lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, stride, code, codes.data_ptr(), scales.data_ptr(),
+                             _stream(device))
+    if rc:
+        _check(lib, rc, "MX4 quantise")
+    return MX4.__new__(MX4)._set(codes, scales, rows, k, layout, device)
 
 
 def _stored_pair(codes, scales, k, what):
@@ -178,8 +200,7 @@ def _stored_pair(codes, scales, k, what):
 def _pack(codes, scales, count, rows, k, paired):
     lib = _library()
     padded = lib.ug_mx4_pack_rows(count, rows, paired)
-    out = [torch.empty(size(OPERAND, padded, k), dtype=torch.uint8, device=codes.device)
-           for size in (lib.ug_mx4_codes_bytes, lib.ug_mx4_scales_bytes)]
+    out = [torch.empty(size, dtype=torch.uint8, device=codes.device) for size in _sizes(OPERAND, padded, k)]
     _check(lib, lib.ug_mx4_pack(codes.data_ptr(), scales.data_ptr(), count, rows, k, paired, out[0].data_ptr(),
                                 out[1].data_ptr(), _stream(codes.device)), "MX4 pack")
     return out
@@ -202,34 +223,41 @@ def matmul(a, w, dtype=None, out=None):
     (default: a's, bfloat16 for an MX4). A NaN or an infinity in a block of ``a`` makes its row NaN."""
     if not isinstance(w, MX4) or w.layout != "operand":
         raise ValueError("w must be an MX4 in operand layout (quantize or pack)")
-    lib = _library()
+    lib, n, device = _library(), w.rows, w.device
     four = isinstance(a, MX4)
     if four:
         if a.layout != "operand":
             raise ValueError("a must be in operand layout")
-        lead, m, k, dtype = (a.rows,), a.rows, a.k, dtype or torch.bfloat16
+        m, k, dtype = a.rows, a.k, dtype or torch.bfloat16
+        shape = (m, n)
     else:
         _input(a, "a", _HALF)
-        lead, dtype = a.shape[:-1], dtype or a.dtype
-        a = _rows(a, "a")
-        m, k = a.shape
+        dtype = dtype or a.dtype
+        shape = (*a.shape[:-1], n)
+        a, m, k, a_stride = _rows(a, "a")
     if dtype not in _TYPES:
         raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
-    if k != w.k or a.device != w.device:
-        raise ValueError(f"a has rows of {k} on {a.device}, w of {w.k} on {w.device}")
-    y = _output(out, (*lead, w.rows), dtype, w.device, (a.codes, a.scales) if four else (a,))
-    stride = y.stride(0) if y.dim() == 2 and m > 1 else w.rows
-    if four:
-        rc = lib.ug_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), m, w.codes.data_ptr(), w.scales.data_ptr(), w.rows,
-                               k, y.data_ptr(), _TYPES[dtype], stride, _stream(w.device))
+    if k != w.k or a.device != device:
+        raise ValueError(f"a has rows of {k} on {a.device}, w of {w.k} on {device}")
+    stride = n
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
     else:
-        need = lib.ug_mx4_matmul_x16_workspace(m, k, _TYPES[a.dtype])
-        ws = torch.empty(need, dtype=torch.uint8, device=w.device)
-        rc = lib.ug_mx4_matmul_x16(a.data_ptr(), _TYPES[a.dtype], _row_stride(a), m, w.codes.data_ptr(),
-                                   w.scales.data_ptr(), w.rows, k, y.data_ptr(), _TYPES[dtype], stride, ws.data_ptr(), need,
-                                   _stream(w.device))
-    _check(lib, rc, "MX4 product")
-    return y
+        _output(out, shape, dtype, device, (a.codes, a.scales, w.codes, w.scales) if four else (a, w.codes, w.scales))
+        if out.dim() == 2:
+            stride = _row_stride(out, m, n)
+    if four:
+        rc = lib.ug_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), m, w.codes.data_ptr(), w.scales.data_ptr(), n, k,
+                               out.data_ptr(), _TYPES[dtype], stride, _stream(device))
+    else:
+        x_type = _TYPES[a.dtype]
+        need = lib.ug_mx4_matmul_x16_workspace(m, k, x_type)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = lib.ug_mx4_matmul_x16(a.data_ptr(), x_type, a_stride, m, w.codes.data_ptr(), w.scales.data_ptr(), n, k,
+                                   out.data_ptr(), _TYPES[dtype], stride, ws.data_ptr(), need, _stream(device))
+    if rc:
+        _check(lib, rc, "MX4 product")
+    return out
 
 
 class Experts:
@@ -271,30 +299,40 @@ class Experts:
         self._layer = UgMx4Experts(e, top_k, d, f, int(bool(normalize)), _TYPES[router.dtype], self.router.data_ptr(),
                                    None if bias is None else bias.data_ptr(), self.gate_up[0].data_ptr(),
                                    self.gate_up[1].data_ptr(), self.down[0].data_ptr(), self.down[1].data_ptr())
-        self._lib = _library()
+        self._lib, self._ref, self._need = _library(), C.byref(self._layer), {}
+        self.device = router.device
 
     def __call__(self, x, out=None, return_choice=False):
         """(..., d) of the router's type -> the same shape. ``return_choice``: also the chosen experts
         (tokens, top_k) int32, in falling order of their logits, and their float32 weights."""
         _input(x, "x", (self.router.dtype,))
-        if x.dim() < 1 or x.shape[-1] != self.d or x.device != self.router.device:
-            raise ValueError(f"x must be (..., {self.d}) on {self.router.device}")
-        shape = x.shape
-        x = _rows(x, "x")
-        t = x.shape[0]
+        d, device, shape = self.d, self.device, x.shape
+        if not shape or shape[-1] != d or x.device != device:
+            raise ValueError(f"x must be (..., {d}) on {device}")
+        x, t, _, x_stride = _rows(x, "x")
         if t > MAX_TOKENS:
             raise ValueError(f"at most {MAX_TOKENS} tokens, not {t}")
-        y = _output(out, shape, x.dtype, x.device, (x,))
-        chosen = torch.empty((t, self.top_k), dtype=torch.int32, device=x.device) if return_choice else None
-        weights = torch.empty((t, self.top_k), dtype=torch.float32, device=x.device) if return_choice else None
-        need = self._lib.ug_mx4_experts_workspace(C.byref(self._layer), t)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        stride = y.stride(0) if y.dim() == 2 and t > 1 else self.d
-        _check(self._lib, self._lib.ug_mx4_experts(
-            C.byref(self._layer), x.data_ptr(), _row_stride(x), t, y.data_ptr(), stride,
-            chosen.data_ptr() if return_choice else None, weights.data_ptr() if return_choice else None, ws.data_ptr(),
-            need, _stream(x.device)), "MX4 experts")
-        return (y, chosen, weights) if return_choice else y
+        stride = d
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=device)
+        else:
+            _output(out, shape, x.dtype, device, (x, self.router, *self.gate_up, *self.down))
+            if out.dim() == 2:
+                stride = _row_stride(out, t, d)
+        chosen = weights = None
+        if return_choice:
+            chosen = torch.empty((t, self.top_k), dtype=torch.int32, device=device)
+            weights = torch.empty((t, self.top_k), dtype=torch.float32, device=device)
+        need = self._need.get(t)
+        if need is None:
+            need = self._need[t] = self._lib.ug_mx4_experts_workspace(self._ref, t)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = self._lib.ug_mx4_experts(self._ref, x.data_ptr(), x_stride, t, out.data_ptr(), stride,
+                                      chosen.data_ptr() if return_choice else None,
+                                      weights.data_ptr() if return_choice else None, ws.data_ptr(), need, _stream(device))
+        if rc:
+            _check(self._lib, rc, "MX4 experts")
+        return (out, chosen, weights) if return_choice else out
 
 
 def check(device=None):
