@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, c
     const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
     const uint32_t group = w / chunks, chunk = w - group * chunks, r0 = group * ROWS;
     const uint32_t j = chunk * 256 + lane * 8;
-    if (r0 >= rows || j >= k) return;
-    const uint32_t n = min((uint32_t)ROWS, rows - r0), row_bytes = (k + 1) / 2, blocks = (k + 31) / 32;
+    if (r0 >= rows) return;
+    const uint32_t n = j < k ? min((uint32_t)ROWS, rows - r0) : 0, row_bytes = (k + 1) / 2, blocks = (k + 31) / 32;
     const uint8_t *from = codes + (OPERAND ? mx_code_at(r0, j, kt) : (size_t)r0 * row_bytes + j / 2);
     const uint8_t *sf = scales + (OPERAND ? mx_scale_at(r0, j / 32, kt) : (size_t)r0 * blocks + j / 32);
     uint32_t c[ROWS], s[ROWS];
@@ -84,6 +84,26 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, c
         from += OPERAND ? 64 : row_bytes;
         sf += OPERAND ? 16 : blocks;
     }
+    if (!vec_out) {
+        // rows that start anywhere: lane l writes values l, l + 32, ..., neighbours side by side
+        T *to = y + r0 * stride + chunk * 256;
+        const uint32_t inside = k - chunk * 256;
+        for (uint32_t i = 0; i < min((uint32_t)ROWS, rows - r0); i++, to += stride) {
+            uint32_t word = 0, code = 0;
+#pragma unroll
+            for (int b = 0; b < ROWS; b++)
+                if ((uint32_t)b == i) word = c[b], code = s[b];
+            const float scale = mx_scale_value(code);
+#pragma unroll
+            for (uint32_t b = 0; b < 8; b++) {
+                const uint32_t at = b * 32 + lane;
+                const uint32_t w8 = __shfl_sync(~0u, word, at / 8);
+                const float sc = __shfl_sync(~0u, scale, at / 8);
+                if (at < inside) to[at] = mx_to<T>(mx_unpack1(w8 >> (at % 8 * 4)) * sc);
+            }
+        }
+        return;
+    }
     T *to = y + r0 * stride + j;
 #pragma unroll
     for (int i = 0; i < ROWS; i++, to += stride) {
@@ -93,7 +113,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, c
         const float scale = mx_scale_value(s[i]);
 #pragma unroll
         for (int b = 0; b < 8; b++) v[b] *= scale;
-        if (vec_out && j + 8 <= k) {
+        if (j + 8 <= k) {
             if (sizeof(T) == 4) {
                 reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
                 reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);

@@ -71,6 +71,13 @@ __device__ __forceinline__ void mx_unpack8(uint32_t codes, float (&v)[8]) {
     }
 }
 
+// The e2m1 value of the low four bits.
+__device__ __forceinline__ float mx_unpack1(uint32_t code) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(code));
+    return __low2float(*reinterpret_cast<const __half2 *>(&h));
+}
+
 // Two floats rounded to a pair of 16-bit values, the first in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t mx_pair(float a, float b);

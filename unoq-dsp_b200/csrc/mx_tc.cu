@@ -28,7 +28,7 @@ namespace cg = cooperative_groups;
 constexpr int kMaxStages = 12;
 constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
 constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
-constexpr int kChunk = 32;         // tokens of one expert that one CTA takes
+constexpr int kChunk = 32;         // most tokens of one expert that one CTA takes
 
 __host__ __device__ constexpr uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
@@ -45,7 +45,7 @@ struct TcArgs {
     int type;
     uint64_t stride;
     // experts
-    uint32_t top_k, row_tiles, head_bytes;   // head: the choices and the columns' scales
+    uint32_t top_k, row_tiles, per_cta, chunk, head_bytes;   // head: the choices and the columns' scales
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
@@ -54,7 +54,7 @@ struct TcArgs {
 };
 
 struct Ctrl {
-    unsigned long long full[kMaxStages], empty[kMaxStages], done;
+    unsigned long long full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     uint32_t tmem;
     int abort;
     unsigned long long rows_ready, scales_ready;
@@ -197,7 +197,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             mbar_init(smem_u32(&c.full[i]), 1);
             mbar_init(smem_u32(&c.empty[i]), 1);
         }
-        mbar_init(smem_u32(&c.done), 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&c.acc_full[i]), 1);
+            mbar_init(smem_u32(&c.acc_empty[i]), 4);
+        }
         mbar_init(smem_u32(&c.rows_ready), 128);
         mbar_init(smem_u32(&c.scales_ready), 128);
         c.abort = 0;
@@ -207,14 +210,15 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     }
 
     // ---- what this CTA computes ----
-    uint32_t w_tile = blockIdx.x;           // first weight tile along the rows
+    const uint32_t tile0 = blockIdx.x * a.per_cta, tiles = min(a.per_cta, a.row_tiles - tile0);  // 128 rows each
+    uint32_t w_tile = tile0;
     uint32_t tokens, tok0 = 0, expert = 0, chunk = 0;  // columns: tokens, or a chunk of one expert's pairs
     const uint32_t kt0 = a.kt * rank / a.split, kt1 = a.kt * (rank + 1) / a.split;
     if (MODE == kDense) {
         tok0 = blockIdx.y * a.nt;
         tokens = min(a.nt, a.m - tok0);
     } else {
-        // Work items: every chosen expert's tokens in chunks of 32, experts in order. This CTA's item is
+        // Work items: every chosen expert's tokens in chunks, experts in order. This CTA's item is
         // found from the choices themselves, in shared memory.
         const uint32_t pairs = a.m * a.top_k;
         for (uint32_t i = threadIdx.x; i < 256; i += kThreads) counts[i] = 0;
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             n[i] = counts[lane * 8 + i];
-            items += (n[i] + kChunk - 1) / kChunk;
+            items += (n[i] + a.chunk - 1) / a.chunk;
         }
         uint32_t upto = items;
 #pragma unroll
@@ -245,7 +249,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         bool open = true;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint32_t chunks = (n[i] + kChunk - 1) / kChunk;
+            const uint32_t chunks = (n[i] + a.chunk - 1) / a.chunk;
             if (open && left < chunks) {
                 found = lane * 8 + i;
                 here = n[i];
@@ -256,8 +260,8 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         const int holder = __ffs(holders) - 1;
         expert = __shfl_sync(~0u, found, holder);
         chunk = __shfl_sync(~0u, left, holder);
-        tokens = min(__shfl_sync(~0u, here, holder) - chunk * kChunk, (uint32_t)kChunk);
-        w_tile = (expert * a.row_tiles + blockIdx.x) * kMats;
+        tokens = min(__shfl_sync(~0u, here, holder) - chunk * a.chunk, a.chunk);
+        w_tile = (expert * a.row_tiles + tile0) * kMats;
     }
     const uint32_t n_cols = (tokens * P + 7) / 8 * 8;
     const uint32_t sfb_tiles = MODE == kDense ? (n_cols + 127) / 128 : 1;
@@ -277,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     tc_fence_after();
     if (MODE == kGateUp) grid_dep_launch();  // every CTA holds its TMEM: the next kernel's may come
     const uint32_t tmem = c.tmem;
-    const uint32_t steps = kt1 - kt0, iters = steps * kMats;   // gate and up tiles of a step follow each other
+    const uint32_t steps = kt1 - kt0, iters = steps * kMats * tiles;   // gate and up tiles of a step follow each other
 
     if (warp == 0 && lane == 0) {
         // ---- TMA ----
@@ -288,13 +292,14 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         auto load_w = [&](uint32_t it, uint32_t s) {
             const uint32_t bar = smem_u32(&c.full[s]), st = smem_u32(ring + s * stage_bytes);
             mbar_expect(bar, stage_tx);
-            const size_t t = (size_t)(w_tile + it % kMats) * a.kt + kt0 + it / kMats;
+            const uint32_t step = it / kMats, tile = step / steps;
+            const size_t t = (size_t)(w_tile + tile * kMats + it % kMats) * a.kt + kt0 + (step - tile * steps);
             tma_2d(st, &wmap, 0, (int)(t * 128), bar);
             bulk_copy(st + kA + b_bytes, a.w_scales + t * kMxScaleTile, kMxScaleTile, bar);
         };
         auto load_x = [&](uint32_t it, uint32_t s) {
             const uint32_t bar = smem_u32(&c.full[s]), b = smem_u32(ring + s * stage_bytes) + kA;
-            const uint32_t sf = b + b_bytes + kMxScaleTile, k = kt0 + it / kMats;
+            const uint32_t sf = b + b_bytes + kMxScaleTile, k = kt0 + it / kMats % steps;
             if (MODE != kDense) {
                 for (uint32_t i = 0; i < n_cols; i += 4)
                     tma_gather4(b + i * 128, &xmap, (int)(k * 128), *reinterpret_cast<const int4 *>(&c.rows[i]), bar);
@@ -331,35 +336,46 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 }
     } else if (warp == 1 && lane == 0) {
         // ---- MMA ----
-        const uint32_t sf_tmem = tmem + a.d_cols * kMats, idesc = scaled_instr_desc<KIND>(n_cols);
+        const uint32_t accs = tiles > 1 ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
+        const uint32_t sf_tmem = tmem + a.d_cols * kMats * accs, idesc = scaled_instr_desc<KIND>(n_cols);
         bool ok = MODE == kDense || mbar_wait(smem_u32(&c.scales_ready), 0, abort, 606);
         uint32_t s = 0, phase = 0;
-        for (uint32_t it = 0; ok && it < iters; it++) {
-            if (!mbar_wait(smem_u32(&c.full[s]), phase, abort, 602)) {
+        for (uint32_t tile = 0; ok && tile < tiles; tile++) {
+            if (tile >= 2 && !mbar_wait(smem_u32(&c.acc_empty[tile & 1]), (tile / 2 & 1) ^ 1, abort, 607)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t st = smem_u32(ring + s * stage_bytes), b = st + kA, sf = b + b_bytes;
-            // each stage has scale columns of its own: they are rewritten only after its MMAs are done
-            const uint32_t sfa = sf_tmem + s * sf_cols, sfb = sfa + 4;
-            scales_to_tmem(sfa, sf);
-            if (MODE == kDense)
-                for (uint32_t i = 0; i < sfb_tiles; i++) scales_to_tmem(sfb + 4 * i, sf + (1 + i) * kMxScaleTile);
-            else
-                scales_to_tmem(sfb, smem_u32(sfb_all + it / kMats * kMxScaleTile));
-            const uint64_t ad = operand_desc<KIND>(st), bd = operand_desc<KIND>(b);
-            const uint32_t d = tmem + it % kMats * a.d_cols;
+            for (uint32_t it = 0; it < steps * kMats; it++) {
+                if (!mbar_wait(smem_u32(&c.full[s]), phase, abort, 602)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t st = smem_u32(ring + s * stage_bytes), b = st + kA, sf = b + b_bytes;
+                // each stage has scale columns of its own: they are rewritten only after its MMAs are done
+                const uint32_t sfa = sf_tmem + s * sf_cols, sfb = sfa + 4;
+                scales_to_tmem(sfa, sf);
+                if (MODE == kDense)
+                    for (uint32_t i = 0; i < sfb_tiles; i++) scales_to_tmem(sfb + 4 * i, sf + (1 + i) * kMxScaleTile);
+                else
+                    scales_to_tmem(sfb, smem_u32(sfb_all + it / kMats * kMxScaleTile));
+                const uint64_t ad = operand_desc<KIND>(st), bd = operand_desc<KIND>(b);
+                const uint32_t d = tmem + ((tile & 1) * kMats + it % kMats) * a.d_cols;
 #pragma unroll
-            for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
-                const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
-                mma_scaled<KIND>(d, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa, sfb, it >= kMats || j);
+                for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
+                    const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
+                    mma_scaled<KIND>(d, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa, sfb, it >= kMats || j);
+                }
+                mma_commit(smem_u32(&c.empty[s]));
+                if (++s == stages) s = 0, phase ^= 1;
             }
-            mma_commit(smem_u32(&c.empty[s]));
-            if (++s == stages) s = 0, phase ^= 1;
+            mma_commit(smem_u32(&c.acc_full[tile & 1]));
         }
-        mma_commit(smem_u32(&c.done));
-        if (!ok) mbar_wait(smem_u32(&c.done), 0, &c.abort, 603);
+        if (!ok) {   // the MMAs that were issued end before TMEM is freed
+            mma_commit(smem_u32(&c.rows_ready));
+            for (int i = 0; i < 100; i++) mbar_try_wait(smem_u32(&c.rows_ready), 0, 1000000);
+        }
     }
     __syncwarp();
     if (MODE != kDense && warp >= 2) {
@@ -367,10 +383,11 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         const uint32_t at = threadIdx.x - 64, pairs = a.m * a.top_k;
         if (warp == 2) {   // the expert's pairs of this chunk, in order
             uint32_t seen = 0;
+#pragma unroll 4
             for (uint32_t i = 0; i < pairs; i += 32) {
                 const bool hit = i + lane < pairs && ids[i + lane] == expert;
                 const uint32_t mask = __ballot_sync(~0u, hit), to = seen + __popc(mask & ((1u << lane) - 1));
-                if (hit && to / kChunk == chunk) c.pairs[to % kChunk] = i + lane;
+                if (hit && to - chunk * a.chunk < a.chunk) c.pairs[to - chunk * a.chunk] = i + lane;
                 seen += __popc(mask);
             }
         }
@@ -392,7 +409,8 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     }
 
     // ---- epilogue: thread = weight row ----
-    const uint32_t q = warp % 4, row = blockIdx.x * 128 + q * 32 + lane;
+    const uint32_t q = warp % 4;
+    uint32_t tile = tile0, row = tile0 * 128 + q * 32 + lane;   // of the tile being read
     const bool epi = warp >= 2;
     float *red = reinterpret_cast<float *>(ring);   // [token][128] per matrix, once the ring is idle
 
@@ -427,7 +445,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         __syncwarp();
         const uint32_t i = first + lane * step;
         const uint32_t t = i < tokens ? c.pairs[i] / a.top_k : 0;
-        const bool last = i < tokens && atomicAdd(a.arrived + ((size_t)t * a.row_tiles + blockIdx.x) * 4 + q, 1u) == a.top_k - 1;
+        const bool last = i < tokens && atomicAdd(a.arrived + ((size_t)t * a.row_tiles + tile) * 4 + q, 1u) == a.top_k - 1;
         uint32_t mask = __ballot_sync(~0u, last);
         __threadfence();
         while (mask) {
@@ -443,10 +461,12 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
     };
 
-    if (epi) {
-        mbar_wait(smem_u32(&c.done), 0, abort, 604);
+    for (uint32_t nth = 0; epi && nth < tiles; nth++) {
+        tile = tile0 + nth;
+        row = tile * 128 + q * 32 + lane;
+        mbar_wait(smem_u32(&c.acc_full[nth & 1]), nth / 2 & 1, abort, 604);
         tc_fence_after();
-        const uint32_t taddr = tmem + (q * 32 << 16);
+        const uint32_t taddr = tmem + (q * 32 << 16) + (nth & 1) * kMats * a.d_cols;
         if (MODE == kDense && a.split == 1) {
             constexpr uint32_t kAt = P == 1 ? 32 : P == 2 ? 16 : 8;   // tokens at a time: up to 32 columns
             uint32_t i0 = 0;
@@ -477,8 +497,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 }
             }
         }
-        if (MODE == kDown && a.split == 1) combine(0, 1);
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c.acc_empty[nth & 1]));
+        if (MODE == kDown && a.split == 1) combine(0, 1);
     }
     if (a.split > 1) {
         // the cluster's partial tiles, added in rank order through distributed shared memory
@@ -618,8 +640,9 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
     const uint32_t budget = (per_sm == 1 ? 226 : 112) * 1024 - extra;
     const uint32_t cols = per_sm == 1 ? 512 : 256;
-    const uint32_t iters = (a.kt + a.split - 1) / a.split * mats;
-    a.stages = std::min({(cols - a.d_cols * mats) / sf_cols, (uint32_t)kMaxStages, iters});
+    const uint32_t iters = (a.kt + a.split - 1) / a.split * mats * a.per_cta;
+    const uint32_t acc_cols = a.d_cols * mats * (a.per_cta > 1 ? 2 : 1);
+    a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, iters});
     if (MODE == kDense) {
         a.stages = std::min(a.stages, budget / a.stage_bytes);
         a.ring_bytes = a.stages * a.stage_bytes;
@@ -628,7 +651,7 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
         a.ring_bytes = std::max(std::min(budget, a.stages * a.stage_bytes), a.stage_bytes);
         a.stages = std::min(a.stages, a.ring_bytes / least);
     }
-    a.tmem_cols = pow2_cols(a.d_cols * mats + a.stages * sf_cols);
+    a.tmem_cols = pow2_cols(acc_cols + a.stages * sf_cols);
     const uint32_t red = a.split > 1 ? mats * a.nt * 128 * 4 : 0;
     return extra + std::max(a.ring_bytes, red);
 }
@@ -642,6 +665,8 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.n = p.n;
     a.kt = kt;
     a.group = kGroup;
+    a.row_tiles = rt;
+    a.per_cta = 1;
     a.nt = p.m < kGroup ? p.m : kGroup;
     const uint32_t tt = (p.m + a.nt - 1) / a.nt;
     const uint32_t per_sm = up_to(a.nt, 8) * P <= 128 ? 2 : 1;
@@ -697,7 +722,6 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.n = rows;
     a.kt = mx_tiles(width);
     a.row_tiles = mx_tiles(rows);
-    a.nt = std::min<uint32_t>(e.tokens, kChunk);
     a.top_k = e.top_k;
     a.chosen = e.ws.chosen;
     a.weight = e.ws.weight;
@@ -710,12 +734,23 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.y = e.y;
     a.type = e.type;
     a.stride = e.y_stride;
-    // as many items as there can be: one to each chosen expert, one more for every further 32 pairs
-    const uint32_t pairs = e.tokens * e.top_k, slots = std::min(e.experts, pairs), items = slots + (pairs - slots) / kChunk;
+    // Tokens to a CTA: 16 where the experts get few, which leaves TMEM for a second accumulator.
+    const uint32_t pairs = e.tokens * e.top_k, slots = std::min(e.experts, pairs);
+    a.chunk = pairs <= e.experts * 8 ? 16 : kChunk;
+    a.nt = std::min(e.tokens, a.chunk);
+    // as many items as there can be: one to each chosen expert, one more for every further chunk of pairs
+    const uint32_t items = slots + (pairs - slots) / a.chunk;
     a.split = 1;
     while (a.split < 8 && a.kt / (a.split * 2) >= 2 &&
            (a.row_tiles * slots * a.split * 2 <= 148 * 2 || a.kt / a.split > 32))
         a.split *= 2;
+    // Row tiles to a CTA: its set-up (finding its tokens, their scales) costs as much as some 100 KB of
+    // weights, so it takes more tiles once there are enough to go round.
+    const uint32_t mats0 = MODE == kGateUp ? 2 : 1, cols = up_to(a.nt, 8) * P * mats0;
+    a.per_cta = 1;
+    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < 4 && a.per_cta * a.kt * mats0 < 32 &&
+           a.row_tiles * slots >= 148 * 2 * 2 * a.per_cta)
+        a.per_cta *= 2;
     a.head_bytes = up_to(1024 + up_to(pairs, kMxScaleTile) + (a.kt + a.split - 1) / a.split * kMxScaleTile, 1024);
     const uint32_t smem = plan_ring<8, P, MODE>(a, 2);
     const uint32_t mats = MODE == kGateUp ? 2 : 1;
@@ -727,7 +762,7 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.kt * 128,
                piece_rows, (uint64_t)a.kt * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
-    return launch<8, P, MODE>(wmap, xmap, a, dim3(a.row_tiles, items, a.split), smem, true, s);
+    return launch<8, P, MODE>(wmap, xmap, a, dim3((a.row_tiles + a.per_cta - 1) / a.per_cta, items, a.split), smem, true, s);
 }
 
 }  // namespace
