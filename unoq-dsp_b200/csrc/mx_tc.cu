@@ -26,7 +26,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxStages = 12;
-constexpr int kThreads = 192;      // warp 0: TMA, warp 1: MMA, warps 2-5: epilogue
+constexpr int kThreads = 224;      // warp 0: weight copies, warp 1: MMA, warps 2-5: epilogue, warp 6: activation copies
 constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
 constexpr int kChunk = 32;         // most tokens of one expert that one CTA takes
 
@@ -57,12 +57,34 @@ struct Ctrl {
     unsigned long long full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     uint32_t tmem;
     int abort;
-    unsigned long long rows_ready, scales_ready;
+    unsigned long long rows_ready, scales_ready, spare;
     uint32_t pairs[kChunk];
     alignas(16) int32_t rows[kChunk * 4];
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 
+// One thread of a converged warp. The copy and MMA threads are chosen so, and not by their lane number: the
+// compiler then knows that one thread runs, and issues a copy in about 15 cycles, not 55.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// Bounded wait that polls instead of suspending: what the copy and MMA threads wait for is mostly there, or
+// comes within some hundred cycles, and a wait with a suspension limit costs 63 cycles even then, a
+// plain one 27.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int *abort, int code) {
+    for (int i = 0; i < 64; i++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(bar), "r"(parity)
+                     : "memory");
+        if (ok) return true;
+    }
+    return mbar_wait(bar, parity, abort, code);
+}
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
                  : "memory");
@@ -194,13 +216,14 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kMaxStages; i++) {
-            mbar_init(smem_u32(&c.full[i]), 1);
+            mbar_init(smem_u32(&c.full[i]), 2);
             mbar_init(smem_u32(&c.empty[i]), 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_u32(&c.acc_full[i]), 1);
             mbar_init(smem_u32(&c.acc_empty[i]), 4);
         }
+        mbar_init(smem_u32(&c.spare), 1);
         mbar_init(smem_u32(&c.rows_ready), 128);
         mbar_init(smem_u32(&c.scales_ready), 128);
         c.abort = 0;
@@ -281,104 +304,146 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     tc_fence_after();
     if (MODE == kGateUp) grid_dep_launch();  // every CTA holds its TMEM: the next kernel's may come
     const uint32_t tmem = c.tmem;
-    const uint32_t steps = kt1 - kt0, iters = steps * kMats * tiles;   // gate and up tiles of a step follow each other
+    const uint32_t steps = kt1 - kt0;   // of K; gate and up tiles of a step follow each other
 
-    if (warp == 0 && lane == 0) {
-        // ---- TMA ----
-        // a copy that unpacks counts the bytes that it read, 64 a row, for either kind
-        const uint32_t stage_tx = kMxCodeTile + kMxScaleTile +
-                                  (MODE == kDense ? (KIND == 8 ? a.b_box_bytes : sfb_tiles * a.b_box_bytes) + sfb_tiles * kMxScaleTile
-                                                  : n_cols * 128);
-        auto load_w = [&](uint32_t it, uint32_t s) {
-            const uint32_t bar = smem_u32(&c.full[s]), st = smem_u32(ring + s * stage_bytes);
-            mbar_expect(bar, stage_tx);
-            const uint32_t step = it / kMats, tile = step / steps;
-            const size_t t = (size_t)(w_tile + tile * kMats + it % kMats) * a.kt + kt0 + (step - tile * steps);
-            tma_2d(st, &wmap, 0, (int)(t * 128), bar);
-            bulk_copy(st + kA + b_bytes, a.w_scales + t * kMxScaleTile, kMxScaleTile, bar);
-        };
-        auto load_x = [&](uint32_t it, uint32_t s) {
-            const uint32_t bar = smem_u32(&c.full[s]), b = smem_u32(ring + s * stage_bytes) + kA;
-            const uint32_t sf = b + b_bytes + kMxScaleTile, k = kt0 + it / kMats % steps;
-            if (MODE != kDense) {
-                for (uint32_t i = 0; i < n_cols; i += 4)
-                    tma_gather4(b + i * 128, &xmap, (int)(k * 128), *reinterpret_cast<const int4 *>(&c.rows[i]), bar);
-            } else if (KIND == 8) {
-                const uint32_t row = tok0 / a.group * 256 + tok0 % a.group * P;
-                tma_2d(b, &xmap, (int)(k * 128), (int)row, bar);
-                for (uint32_t i = 0; i < sfb_tiles; i++)
-                    bulk_copy(sf + i * kMxScaleTile, a.x_scales + ((size_t)(row / 128 + i) * a.kt + k) * kMxScaleTile, kMxScaleTile, bar);
-            } else {
-                for (uint32_t i = 0; i < sfb_tiles; i++) {
-                    const size_t t = (size_t)(tok0 / 128 + i) * a.kt + k;
-                    tma_2d(b + i * a.b_box_bytes, &xmap, 0, (int)(t * 128), bar);
-                    bulk_copy(sf + i * kMxScaleTile, a.x_scales + t * kMxScaleTile, kMxScaleTile, bar);
+    // no copy may land after this CTA has left: the last round's barriers, on the way out of an abort
+    auto drain = [&](uint32_t issued) {
+        for (uint32_t it = issued > stages ? issued - stages : 0; it < issued; it++)
+            for (int i = 0; i < 100 && !mbar_try_wait(smem_u32(&c.full[it % stages]), it / stages & 1, 1000000); i++) {
+            }
+    };
+
+    if (warp == 0 && elect_one()) {
+        // ---- weight tiles and their scales: the order of the tiles in memory, but gate and up in turn ----
+        // (a copy that unpacks counts the bytes that it read, 64 a row, for either kind)
+        const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
+        uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;   // phase 1: not yet used
+        for (uint32_t tile = 0; tile < tiles; tile++) {
+            const size_t first = (size_t)(w_tile + tile * kMats) * a.kt + kt0;
+            int y = (int)(first * 128);
+            const uint8_t *sf = a.w_scales + first * kMxScaleTile;
+            for (uint32_t step = 0; step < steps; step++, y += 128, sf += kMxScaleTile) {
+#pragma unroll
+                for (uint32_t i = 0; i < kMats; i++) {
+                    if (!mbar_poll(empty, phase, abort, 601)) goto weights_out;
+                    mbar_expect(full, kMxCodeTile + kMxScaleTile);
+                    tma_2d(st, &wmap, 0, y + (int)(i * a.kt * 128), full);
+                    bulk_copy(st + kA + b_bytes, sf + i * a.kt * kMxScaleTile, kMxScaleTile, full);
+                    issued++;
+                    st += stage_bytes, full += 8, empty += 8;
+                    if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
                 }
             }
-        };
-        // weights do not depend on the kernel before: the ring's first round of them goes out at once
-        const uint32_t ahead = min(stages, iters);
-        for (uint32_t it = 0; it < ahead; it++) load_w(it, it);
-        if (MODE == kDense && KIND == 8) grid_dep_wait();  // the pieces
-        const bool listed = MODE == kDense || mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605);
-        if (listed)
-            for (uint32_t it = 0; it < ahead; it++) load_x(it, it);
-        uint32_t s = 0, phase = 0, issued = ahead;   // stage and round of the next copy's wait
-        for (; listed && issued < iters; issued++) {
-            if (!mbar_wait(smem_u32(&c.empty[s]), phase, abort, 601)) break;
-            load_w(issued, s);
-            load_x(issued, s);
-            if (++s == stages) s = 0, phase ^= 1;
         }
-        if (*abort)  // no copy may land after this CTA has left
-            for (uint32_t it = issued > stages ? issued - stages : 0; it < issued; it++)
-                for (int i = 0; i < 1000 && !mbar_try_wait(smem_u32(&c.full[it % stages]), it / stages & 1, 1000000); i++) {
+    weights_out:
+        if (*abort) drain(issued);
+    } else if (warp == 6 && elect_one()) {
+        // ---- activation columns and, for dense products, their scales ----
+        if (MODE == kDense && KIND == 8) grid_dep_wait();  // the pieces
+        const uint32_t st0 = smem_u32(ring) + kA, full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
+        uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;
+        const uint32_t tx = MODE == kDense ? (KIND == 8 ? a.b_box_bytes : sfb_tiles * a.b_box_bytes) + sfb_tiles * kMxScaleTile
+                                           : n_cols * 128;
+        const uint32_t row = MODE == kDense && KIND == 8 ? tok0 / a.group * 256 + tok0 % a.group * P : tok0;
+        if (MODE != kDense && !mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605)) goto columns_out;
+        if (MODE == kDense) {
+            const bool two = sfb_tiles > 1;
+            const uint32_t next_x = a.kt * 128, next_sf = a.kt * kMxScaleTile;   // the second tile of 128 columns
+            const uint8_t *sf = a.x_scales + ((size_t)(row / 128) * a.kt + kt0) * kMxScaleTile;
+            int x = KIND == 8 ? (int)(kt0 * 128) : (int)((row / 128 * a.kt + kt0) * 128);
+            for (uint32_t step = 0; step < steps; step++, x += 128, sf += kMxScaleTile) {
+                if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
+                mbar_expect(full, tx);
+                if (KIND == 8) {
+                    tma_2d(st, &xmap, x, (int)row, full);
+                } else {
+                    tma_2d(st, &xmap, 0, x, full);
+                    if (two) tma_2d(st + a.b_box_bytes, &xmap, 0, x + (int)next_x, full);
                 }
-    } else if (warp == 1 && lane == 0) {
+                bulk_copy(st + b_bytes + kMxScaleTile, sf, kMxScaleTile, full);
+                if (two) bulk_copy(st + b_bytes + 2 * kMxScaleTile, sf + next_sf, kMxScaleTile, full);
+                issued++;
+                st += stage_bytes, full += 8, empty += 8;
+                if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
+            }
+        } else {
+            const int4 *rows = reinterpret_cast<const int4 *>(c.rows);
+            const int4 r0 = rows[0], r1 = rows[1], r2 = rows[2], r3 = rows[3];   // most experts' columns
+            for (uint32_t tile = 0; tile < tiles; tile++) {
+                int x = (int)(kt0 * 128);
+                for (uint32_t step = 0; step < steps; step++, x += 128) {
+#pragma unroll
+                    for (uint32_t mat = 0; mat < kMats; mat++) {
+                        if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
+                        mbar_expect(full, tx);
+                        tma_gather4(st, &xmap, x, r0, full);
+                        tma_gather4(st + 512, &xmap, x, r1, full);
+                        if (n_cols > 8) {
+                            tma_gather4(st + 1024, &xmap, x, r2, full);
+                            tma_gather4(st + 1536, &xmap, x, r3, full);
+                        }
+                        for (uint32_t i = 16; i < n_cols; i += 4) tma_gather4(st + i * 128, &xmap, x, rows[i / 4], full);
+                        issued++;
+                        st += stage_bytes, full += 8, empty += 8;
+                        if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
+                    }
+                }
+            }
+        }
+    columns_out:
+        if (*abort) drain(issued);
+    } else if (warp == 1 && elect_one()) {
         // ---- MMA ----
         const uint32_t accs = tiles > 1 ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
         const uint32_t sf_tmem = tmem + a.d_cols * kMats * accs, idesc = scaled_instr_desc<KIND>(n_cols);
+        const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
+        // each stage has scale columns of its own: they are rewritten only after its MMAs are done
+        uint32_t st = st0, full = full0, empty = empty0, sfa = sf_tmem, s = 0, phase = 0;
         bool ok = MODE == kDense || mbar_wait(smem_u32(&c.scales_ready), 0, abort, 606);
-        uint32_t s = 0, phase = 0;
         for (uint32_t tile = 0; ok && tile < tiles; tile++) {
-            if (tile >= 2 && !mbar_wait(smem_u32(&c.acc_empty[tile & 1]), (tile / 2 & 1) ^ 1, abort, 607)) {
+            if (tile >= 2 && !mbar_poll(smem_u32(&c.acc_empty[tile & 1]), (tile / 2 & 1) ^ 1, abort, 607)) {
                 ok = false;
                 break;
             }
-            tc_fence_after();
+            const uint32_t d0 = tmem + (tile & 1) * kMats * a.d_cols;
+            uint32_t sfb_smem = smem_u32(sfb_all);
             for (uint32_t it = 0; it < steps * kMats; it++) {
-                if (!mbar_wait(smem_u32(&c.full[s]), phase, abort, 602)) {
+                if (!mbar_poll(full, phase, abort, 602)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t st = smem_u32(ring + s * stage_bytes), b = st + kA, sf = b + b_bytes;
-                // each stage has scale columns of its own: they are rewritten only after its MMAs are done
-                const uint32_t sfa = sf_tmem + s * sf_cols, sfb = sfa + 4;
+                const uint32_t b = st + kA, sf = b + b_bytes, sfb = sfa + 4;
                 scales_to_tmem(sfa, sf);
-                if (MODE == kDense)
-                    for (uint32_t i = 0; i < sfb_tiles; i++) scales_to_tmem(sfb + 4 * i, sf + (1 + i) * kMxScaleTile);
-                else
-                    scales_to_tmem(sfb, smem_u32(sfb_all + it / kMats * kMxScaleTile));
+                if (MODE == kDense) {
+                    scales_to_tmem(sfb, sf + kMxScaleTile);
+                    if (sfb_tiles > 1) scales_to_tmem(sfb + 4, sf + 2 * kMxScaleTile);
+                } else {
+                    scales_to_tmem(sfb, sfb_smem);
+                    if (kMats == 1 || it % 2) sfb_smem += kMxScaleTile;
+                }
                 const uint64_t ad = operand_desc<KIND>(st), bd = operand_desc<KIND>(b);
-                const uint32_t d = tmem + ((tile & 1) * kMats + it % kMats) * a.d_cols;
+                const uint32_t d = d0 + (kMats == 2 ? it % 2 * a.d_cols : 0);
 #pragma unroll
                 for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
                     const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
                     mma_scaled<KIND>(d, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa, sfb, it >= kMats || j);
                 }
-                mma_commit(smem_u32(&c.empty[s]));
-                if (++s == stages) s = 0, phase ^= 1;
+                mma_commit(empty);
+                st += stage_bytes, full += 8, empty += 8, sfa += sf_cols;
+                if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0, sfa = sf_tmem;
             }
             mma_commit(smem_u32(&c.acc_full[tile & 1]));
         }
         if (!ok) {   // the MMAs that were issued end before TMEM is freed
-            mma_commit(smem_u32(&c.rows_ready));
-            for (int i = 0; i < 100; i++) mbar_try_wait(smem_u32(&c.rows_ready), 0, 1000000);
+            mma_commit(smem_u32(&c.spare));
+            for (int i = 0; i < 100 && !mbar_try_wait(smem_u32(&c.spare), 0, 1000000); i++) {
+            }
         }
     }
     __syncwarp();
-    if (MODE != kDense && warp >= 2) {
+    const bool epi = warp >= 2 && warp < 6;
+    if (MODE != kDense && epi) {
         // ---- the columns: which rows of pieces, and all their scales of this CTA's share of K ----
         const uint32_t at = threadIdx.x - 64, pairs = a.m * a.top_k;
         if (warp == 2) {   // the expert's pairs of this chunk, in order
@@ -411,7 +476,6 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     // ---- epilogue: thread = weight row ----
     const uint32_t q = warp % 4;
     uint32_t tile = tile0, row = tile0 * 128 + q * 32 + lane;   // of the tile being read
-    const bool epi = warp >= 2;
     float *red = reinterpret_cast<float *>(ring);   // [token][128] per matrix, once the ring is idle
 
     auto finish = [&](uint32_t i, float g, float u) {
@@ -508,13 +572,19 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         cluster.sync();
         if (epi)
             for (uint32_t i = rank; i < tokens; i += a.split) {
-                float g = 0.0f, u = 0.0f;
-                for (uint32_t r = 0; r < a.split; r++) {
-                    const float *other = cluster.map_shared_rank(red, r);
-                    g += other[i * 128 + q * 32 + lane];
-                    if (MODE == kGateUp) u += other[(a.nt + i) * 128 + q * 32 + lane];
+                float g[8], u[8];   // all loads go out before the first sum
+#pragma unroll
+                for (uint32_t r = 0; r < 8; r++) {
+                    g[r] = u[r] = 0.0f;
+                    if (r < a.split) {
+                        const float *other = cluster.map_shared_rank(red, r);
+                        g[r] = other[i * 128 + q * 32 + lane];
+                        if (MODE == kGateUp) u[r] = other[(a.nt + i) * 128 + q * 32 + lane];
+                    }
                 }
-                finish(i, g, u);
+#pragma unroll
+                for (uint32_t r = 1; r < 8; r++) g[0] += g[r], u[0] += u[r];
+                finish(i, g[0], u[0]);
             }
         __syncwarp();
         cluster.barrier_arrive();   // this CTA reads the others' shared memory no more
