@@ -21,12 +21,13 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 // steps at 512 images per GPU, 1% at 4,096). The depthwise kernel is launched in full stream order
 // (early depthwise blocks measured 1-3% slower), but it still lets the next convolution start once
 // all its blocks are running. UNOQ_PDL=<bits> overrides the set (a tuning and diagnosis switch;
-// results are the same either way).
-enum PdlKind { kPdlConvTc = 1, kPdlConvRows = 2, kPdlConvTaps = 4, kPdlDw = 8, kPdlDwTc = 16 };
+// results are the same either way). The MX4 kernels (mx.cuh) all take them: a call is one to three
+// short kernels, and 1-2 us of each is launch and set-up.
+enum PdlKind { kPdlConvTc = 1, kPdlConvRows = 2, kPdlConvTaps = 4, kPdlDw = 8, kPdlDwTc = 16, kPdlMx = 32 };
 inline bool pdl_enabled(int kind) {
     static const int mask = [] {
         const char *e = std::getenv("UNOQ_PDL");
-        return e ? std::atoi(e) : (kPdlConvTc | kPdlConvRows | kPdlConvTaps | kPdlDwTc);
+        return e ? std::atoi(e) : (kPdlConvTc | kPdlConvRows | kPdlConvTaps | kPdlDwTc | kPdlMx);
     }();
     return (mask & kind) != 0;
 }

@@ -24,6 +24,8 @@ template <typename T, bool OPERAND, int ROWS>
 __global__ void __launch_bounds__(256) quantize_kernel(const T *x, uint32_t rows, uint32_t k, uint64_t stride, uint32_t kt,
                                                        uint32_t chunks, uint8_t *codes, uint8_t *scales, bool vec_in,
                                                        bool vec_out) {
+    grid_dep_wait();
+    grid_dep_launch();
     const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
     const uint32_t group = w / chunks, chunk = w - group * chunks, r0 = group * ROWS;
     if (r0 >= rows) return;
@@ -62,6 +64,8 @@ template <typename T, bool OPERAND, int ROWS>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t rows, uint32_t k,
                                                          uint32_t kt, uint32_t chunks, T *y, uint64_t stride, bool vec_in,
                                                          bool vec_out) {
+    grid_dep_wait();
+    grid_dep_launch();
     const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
     const uint32_t group = w / chunks, chunk = w - group * chunks, r0 = group * ROWS;
     const uint32_t j = chunk * 256 + lane * 8;
@@ -173,71 +177,96 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t *codes, const u
 
 // ---- router ------------------------------------------------------------------------------------
 //
-// A cluster of 8 CTAs per token: each takes every eighth expert, one warp to an expert's product (32 lanes across d, fixed order, so logits do not depend
-// on timing). The logits meet in the first CTA's shared memory, whose first warp selects. The same
-// CTAs split the row into the pieces that the gate / up product reads.
+// A cluster of 8 CTAs takes TOKENS tokens: each CTA has every eighth expert, one warp to an expert's
+// products (32 lanes across d, fixed order, so logits do not depend on timing). A token's logits meet
+// in the shared memory of one of the CTAs, whose first warp selects. The same CTAs split the rows
+// into the pieces that the gate / up product reads. One token is a chain of latencies (4.5 us for 32
+// experts of 2048: 2 for the products, 0.7 for the cluster's barrier, 0.6 for the selection); with
+// many, four tokens share each router row read, which is all the L2 traffic (64 tokens, 128
+// experts: 6.4 us of products with one).
 
-template <typename T>
+template <typename T, int TOKENS>
 __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) router_kernel(MxExpertsArgs a, bool vec) {
     __shared__ float logits[256];
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t rank = blockIdx.x, t = blockIdx.y;
+    const uint32_t rank = blockIdx.x, t0 = blockIdx.y * TOKENS, tokens = min((uint32_t)TOKENS, a.tokens - t0);
+    auto started = cluster.barrier_arrive();  // the CTAs' shared memory exists for the others after the wait
+    grid_dep_wait();
     grid_dep_launch();  // the products' set-up may begin; they wait for this kernel's results
-    auto started = cluster.barrier_arrive();  // the first CTA's shared memory exists for the others after the wait
     bool waited = false;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const T *row = static_cast<const T *>(a.x) + t * a.x_stride;
+    const T *x = static_cast<const T *>(a.x) + t0 * a.x_stride;
 
-    float *remote = cluster.map_shared_rank(logits, 0);
     for (uint32_t e = rank + kMxRouterCluster * warp; e < a.experts; e += kMxRouterCluster * 8) {
         const T *w = static_cast<const T *>(a.router) + (size_t)e * a.d;
-        float sum = 0.0f;
-        if (vec) {
-#pragma unroll 8
-            for (uint32_t i = lane * 8; i < a.d; i += 256) {
-                const uint4 p = __ldg(reinterpret_cast<const uint4 *>(w + i)), q = __ldg(reinterpret_cast<const uint4 *>(row + i));
-                const T *ph = reinterpret_cast<const T *>(&p), *qh = reinterpret_cast<const T *>(&q);
+        float sum[TOKENS];
 #pragma unroll
-                for (int j = 0; j < 8; j++) sum = fmaf(mx_float(ph[j]), mx_float(qh[j]), sum);
+        for (int n = 0; n < TOKENS; n++) sum[n] = 0.0f;
+        if (vec) {
+#pragma unroll(TOKENS == 1 ? 8 : 2)
+            for (uint32_t i = lane * 8; i < a.d; i += 256) {
+                const uint4 p = __ldg(reinterpret_cast<const uint4 *>(w + i));
+                const T *ph = reinterpret_cast<const T *>(&p);
+#pragma unroll
+                for (int n = 0; n < TOKENS; n++) {
+                    // a token past the last repeats it
+                    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(x + min((uint32_t)n, tokens - 1) * a.x_stride + i));
+                    const T *qh = reinterpret_cast<const T *>(&q);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) sum[n] = fmaf(mx_float(ph[j]), mx_float(qh[j]), sum[n]);
+                }
             }
         } else {
-#pragma unroll 8
-            for (uint32_t i = lane; i < a.d; i += 32) sum = fmaf(mx_float(w[i]), mx_float(row[i]), sum);
+#pragma unroll 4
+            for (uint32_t i = lane; i < a.d; i += 32) {
+                const float p = mx_float(w[i]);
+#pragma unroll
+                for (int n = 0; n < TOKENS; n++)
+                    sum[n] = fmaf(p, mx_float(x[min((uint32_t)n, tokens - 1) * a.x_stride + i]), sum[n]);
+            }
         }
 #pragma unroll
-        for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
+        for (int n = 0; n < TOKENS; n++)
+#pragma unroll
+            for (int o = 16; o; o /= 2) sum[n] += __shfl_xor_sync(~0u, sum[n], o);
         if (!waited) {
             cluster.barrier_wait(std::move(started));
             waited = true;
         }
-        if (lane == 0) remote[e] = sum + (a.bias ? a.bias[e] : 0.0f);
+#pragma unroll
+        for (int n = 0; n < TOKENS; n++)
+            if (lane == n) cluster.map_shared_rank(logits, n)[e] = sum[n] + (a.bias ? a.bias[e] : 0.0f);
     }
     if (!waited) cluster.barrier_wait(std::move(started));
 
-    // the row's pieces: one warp to a block of 32 values
+    // the rows' pieces: one warp to a block of 32 values
     const uint32_t kt = mx_tiles(a.d);
     const int pieces = mx_pieces(a.type);
-    for (uint32_t b = rank * 8 + warp; b < kt * 4; b += kMxRouterCluster * 8) {
-        const uint32_t i = b * 32 + lane;
-        const float v = i < a.d ? mx_float(row[i]) : 0.0f;
-        // infinity and NaN order above every number here
-        const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(v) & 0x7FFFFFFFu);
-        const uint32_t s = mx_piece_scale(__uint_as_float(top), pieces);
-        float left = v * __uint_as_float((254u - min(s, 253u)) << 23);
-        for (int p = 0; p < pieces; p++) {
-            float back;
-            const uint32_t code = mx_e4m3(left, &back);
-            left = (left - back) * 16.0f;
-            const size_t r = (size_t)t * pieces + p;
-            a.ws.x_pieces[r * kt * 128 + i] = s == 255 ? 0 : (uint8_t)code;
-            if (lane == 0) a.ws.x_scales[r * kt * 4 + b] = (uint8_t)mx_piece_scale_of(s, p);
+    for (uint32_t n = 0; n < tokens; n++) {
+        const T *row = x + n * a.x_stride;
+        for (uint32_t b = rank * 8 + warp; b < kt * 4; b += kMxRouterCluster * 8) {
+            const uint32_t i = b * 32 + lane;
+            const float v = i < a.d ? mx_float(row[i]) : 0.0f;
+            // infinity and NaN order above every number here
+            const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(v) & 0x7FFFFFFFu);
+            const uint32_t s = mx_piece_scale(__uint_as_float(top), pieces);
+            float left = v * __uint_as_float((254u - min(s, 253u)) << 23);
+            for (int p = 0; p < pieces; p++) {
+                float back;
+                const uint32_t code = mx_e4m3(left, &back);
+                left = (left - back) * 16.0f;
+                const size_t r = (size_t)(t0 + n) * pieces + p;
+                a.ws.x_pieces[r * kt * 128 + i] = s == 255 ? 0 : (uint8_t)code;
+                if (lane == 0) a.ws.x_scales[r * kt * 4 + b] = (uint8_t)mx_piece_scale_of(s, p);
+            }
         }
     }
-    if (rank == 0)
+    const uint32_t t = t0 + rank;   // the token whose logits are here
+    if (rank < tokens)
         for (uint32_t i = threadIdx.x; i < kt * 4; i += blockDim.x) a.ws.arrived[(size_t)t * kt * 4 + i] = 0;
 
     cluster.sync();
-    if (rank != 0 || warp != 0) return;
+    if (rank >= tokens || warp != 0) return;
     // selection: keys order as the logits do; a NaN is below every number, a taken expert is 0
     uint32_t key[8];
 #pragma unroll
@@ -320,9 +349,8 @@ cudaError_t quantize(const void *x, uint32_t rows, uint32_t k, uint64_t stride, 
     const bool many = many_rows(rows, chunks, kRows);
     auto kernel = layout ? (many ? quantize_kernel<T, true, kRows> : quantize_kernel<T, true, 1>)
                          : (many ? quantize_kernel<T, false, kRows> : quantize_kernel<T, false, 1>);
-    kernel<<<row_grid(rows, chunks, many ? kRows : 1), 256, 0, s>>>(static_cast<const T *>(x), rows, k, stride, kt, chunks, codes,
-                                                                    scales, vec_in, vec_out);
-    return cudaGetLastError();
+    return launch_pdl(kPdlMx, kernel, row_grid(rows, chunks, many ? kRows : 1), 256, 0, s, static_cast<const T *>(x), rows, k,
+                      stride, kt, chunks, codes, scales, vec_in, vec_out);
 }
 
 template <typename T>
@@ -335,9 +363,8 @@ cudaError_t dequantize(const uint8_t *codes, const uint8_t *scales, int layout, 
     const bool many = many_rows(rows, chunks, kRows);
     auto kernel = layout ? (many ? dequantize_kernel<T, true, kRows> : dequantize_kernel<T, true, 1>)
                          : (many ? dequantize_kernel<T, false, kRows> : dequantize_kernel<T, false, 1>);
-    kernel<<<row_grid(rows, chunks, many ? kRows : 1), 256, 0, s>>>(codes, scales, rows, k, kt, chunks, static_cast<T *>(y), stride,
-                                                                    vec_in, vec_out);
-    return cudaGetLastError();
+    return launch_pdl(kPdlMx, kernel, row_grid(rows, chunks, many ? kRows : 1), 256, 0, s, codes, scales, rows, k, kt, chunks,
+                      static_cast<T *>(y), stride, vec_in, vec_out);
 }
 
 }  // namespace
@@ -366,12 +393,11 @@ cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_
 
 cudaError_t launch_mx4_router(const MxExpertsArgs &a, cudaStream_t s) {
     const bool vec = aligned(a.router, 16) && a.d % 8 == 0 && aligned(a.x, 16) && a.x_stride % 8 == 0;
-    const dim3 grid(kMxRouterCluster, a.tokens);
-    if (a.type == 1)
-        router_kernel<__half><<<grid, 256, 0, s>>>(a, vec);
-    else
-        router_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, vec);
-    return cudaGetLastError();
+    const bool many = a.tokens > 16;   // 16 clusters of one token each have an SM to every CTA
+    const dim3 grid(kMxRouterCluster, many ? (a.tokens + 3) / 4 : a.tokens);
+    auto kernel = a.type == 1 ? (many ? router_kernel<__half, 4> : router_kernel<__half, 1>)
+                              : (many ? router_kernel<__nv_bfloat16, 4> : router_kernel<__nv_bfloat16, 1>);
+    return launch_pdl(kPdlMx, kernel, grid, 256, 0, s, a, vec);
 }
 
 }  // namespace uq

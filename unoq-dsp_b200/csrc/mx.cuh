@@ -221,6 +221,9 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 mx_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 #endif
 
+// Every kernel below is launched programmatically (common.cuh): its first access to memory follows
+// grid_dep_wait(), and it lets the next one start only after that, so a kernel that has started
+// early never meets memory of one before the last.
 cudaError_t launch_mx4_quantize(const void *x, int type, uint32_t rows, uint32_t k, uint64_t stride, int layout,
                                 uint8_t *codes, uint8_t *scales, cudaStream_t s);
 cudaError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int layout, uint32_t rows, uint32_t k,
@@ -232,6 +235,7 @@ cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_
 struct MxExpertsScratch {
     int32_t *chosen;      // tokens x top_k
     float *weight;        // tokens x top_k
+    uint32_t *items;      // the work items of the products: mx_experts_items of 34 words, after one for their number
     uint32_t *arrived;    // tokens x 4 mx_tiles(d): pairs whose 32 values are written
     uint8_t *x_pieces;    // (tokens * pieces) x 128 mx_tiles(d), e4m3
     uint8_t *x_scales;    // (tokens * pieces) x 4 mx_tiles(d)
@@ -239,6 +243,12 @@ struct MxExpertsScratch {
     uint8_t *h_scales;    // (tokens * top_k * 3) x 4 mx_tiles(f)
     float *partial;       // (tokens * top_k) x d: weighted down products
 };
+
+// The most work items that `pairs` (token, choice) pairs over `experts` can make, in the smallest chunks of 16.
+inline size_t mx_experts_items(size_t pairs, size_t experts) {
+    const size_t slots = pairs < experts ? pairs : experts;
+    return slots + (pairs - slots) / 16;
+}
 
 struct MxExpertsArgs {
     uint32_t experts, top_k, d, f, tokens;

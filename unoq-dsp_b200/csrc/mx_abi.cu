@@ -85,6 +85,7 @@ size_t experts_scratch(const UgMx4Experts &l, uint32_t tokens, uint8_t *base, uq
     uq::MxExpertsScratch w;
     w.chosen = reinterpret_cast<int32_t *>(take(pairs * 4));
     w.weight = reinterpret_cast<float *>(take(pairs * 4));
+    w.items = reinterpret_cast<uint32_t *>(take((1 + uq::mx_experts_items(pairs, l.experts)) * 34 * 4));
     w.arrived = reinterpret_cast<uint32_t *>(take(tokens * dt * 16));
     w.x_pieces = take(xr * dt * 128);
     w.x_scales = take(xr * dt * 4);

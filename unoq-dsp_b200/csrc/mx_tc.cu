@@ -25,9 +25,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 16;
 constexpr int kThreads = 224;      // warp 0: weight copies, warp 1: MMA, warps 2-5: epilogue, warp 6: activation copies
 constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
+constexpr int kItemWords = 2 + 32; // an item: expert, tokens, the pairs
 constexpr int kChunk = 32;         // most tokens of one expert that one CTA takes
 
 __host__ __device__ constexpr uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
@@ -49,6 +50,7 @@ struct TcArgs {
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
+    uint32_t *items;          // the gate / up product's work items, for the down product
     uint8_t *h_pieces, *h_scales;
     float *partial;
 };
@@ -58,7 +60,7 @@ struct Ctrl {
     uint32_t tmem;
     int abort;
     unsigned long long rows_ready, scales_ready, spare;
-    uint32_t pairs[kChunk];
+    uint32_t pairs[kChunk], found[4];
     alignas(16) int32_t rows[kChunk * 4];
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
@@ -241,49 +243,62 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         tok0 = blockIdx.y * a.nt;
         tokens = min(a.nt, a.m - tok0);
     } else {
-        // Work items: every chosen expert's tokens in chunks, experts in order. This CTA's item is
-        // found from the choices themselves, in shared memory.
-        const uint32_t pairs = a.m * a.top_k;
-        for (uint32_t i = threadIdx.x; i < 256; i += kThreads) counts[i] = 0;
-        __syncthreads();
-        grid_dep_wait();  // the router's choice, or the hidden vectors, of the kernel before
+        // Work items: every chosen expert's tokens in chunks, experts in order. The gate / up product
+        // finds its item from the choices themselves, in shared memory, and leaves the list to the
+        // down product.
+        const uint32_t item = blockIdx.y;
+        if (MODE == kGateUp) {
+            const uint32_t pairs = a.m * a.top_k;
+            for (uint32_t i = threadIdx.x; i < 256; i += kThreads) counts[i] = 0;
+            __syncthreads();
+            grid_dep_wait();  // the router's choice
 #pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < pairs; i += kThreads) {
-            const uint32_t e = (uint32_t)__ldcg(a.chosen + i);
-            ids[i] = (uint8_t)e;
-            atomicAdd(&counts[e % 256], 1u);
-        }
-        __syncthreads();
-        uint32_t n[8], items = 0;   // every warp on its own: a lane has eight experts
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            n[i] = counts[lane * 8 + i];
-            items += (n[i] + a.chunk - 1) / a.chunk;
-        }
-        uint32_t upto = items;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const uint32_t below = __shfl_up_sync(~0u, upto, o);
-            if (lane >= o) upto += below;
-        }
-        const uint32_t item = blockIdx.y, holders = __ballot_sync(~0u, item < upto);
-        if (!holders) return;  // the same in the whole cluster
-        uint32_t left = item - (upto - items), found = 0, here = 0;
-        bool open = true;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t chunks = (n[i] + a.chunk - 1) / a.chunk;
-            if (open && left < chunks) {
-                found = lane * 8 + i;
-                here = n[i];
-                open = false;
+            for (uint32_t i = threadIdx.x; i < pairs; i += kThreads) {
+                const uint32_t e = (uint32_t)__ldcg(a.chosen + i);
+                ids[i] = (uint8_t)e;
+                atomicAdd(&counts[e % 256], 1u);
             }
-            if (open) left -= chunks;
+            __syncthreads();
+            uint32_t n[8], items = 0;   // every warp on its own: a lane has eight experts
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                n[i] = counts[lane * 8 + i];
+                items += (n[i] + a.chunk - 1) / a.chunk;
+            }
+            uint32_t upto = items;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint32_t below = __shfl_up_sync(~0u, upto, o);
+                if (lane >= o) upto += below;
+            }
+            if (item == 0 && blockIdx.x == 0 && rank == 0 && threadIdx.x == 31) a.items[0] = upto;
+            const uint32_t holders = __ballot_sync(~0u, item < upto);
+            if (!holders) return;  // the same in the whole cluster
+            uint32_t left = item - (upto - items), found = 0, here = 0;
+            bool open = true;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t chunks = (n[i] + a.chunk - 1) / a.chunk;
+                if (open && left < chunks) {
+                    found = lane * 8 + i;
+                    here = n[i];
+                    open = false;
+                }
+                if (open) left -= chunks;
+            }
+            const int holder = __ffs(holders) - 1;
+            expert = __shfl_sync(~0u, found, holder);
+            chunk = __shfl_sync(~0u, left, holder);
+            tokens = min(__shfl_sync(~0u, here, holder) - chunk * a.chunk, a.chunk);
+        } else {
+            grid_dep_wait();  // the items and the hidden vectors
+            const uint32_t *it = a.items + kItemWords * (1 + item);
+            const uint32_t total = __ldcg(a.items), of = __ldcg(it), pair = __ldcg(it + 2 + lane);
+            tokens = __ldcg(it + 1);
+            if (item >= total) return;
+            expert = of;
+            if (warp == 2) c.pairs[lane] = pair;
         }
-        const int holder = __ffs(holders) - 1;
-        expert = __shfl_sync(~0u, found, holder);
-        chunk = __shfl_sync(~0u, left, holder);
-        tokens = min(__shfl_sync(~0u, here, holder) - chunk * a.chunk, a.chunk);
         w_tile = (expert * a.row_tiles + tile0) * kMats;
     }
     const uint32_t n_cols = (tokens * P + 7) / 8 * 8;
@@ -306,6 +321,11 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     const uint32_t tmem = c.tmem;
     const uint32_t steps = kt1 - kt0;   // of K; gate and up tiles of a step follow each other
 
+    // a column's row of pieces; columns past the last token repeat it
+    auto row_of = [&](uint32_t i) {
+        const uint32_t pair = c.pairs[min(i / P, tokens - 1)];
+        return (MODE == kGateUp ? pair / a.top_k : pair) * P + (i / P < tokens ? i % P : 0);
+    };
     // no copy may land after this CTA has left: the last round's barriers, on the way out of an abort
     auto drain = [&](uint32_t issued) {
         for (uint32_t it = issued > stages ? issued - stages : 0; it < issued; it++)
@@ -314,6 +334,9 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     };
 
     if (warp == 0 && elect_one()) {
+        // KIND 8's kernel before makes pieces and has seen all earlier work done; before KIND 4's may be any kernel,
+        // one that writes the weights too
+        if (MODE == kDense && KIND == 4) grid_dep_wait();
         // ---- weight tiles and their scales: the order of the tiles in memory, but gate and up in turn ----
         // (a copy that unpacks counts the bytes that it read, 64 a row, for either kind)
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
@@ -337,61 +360,66 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
     weights_out:
         if (*abort) drain(issued);
-    } else if (warp == 6 && elect_one()) {
+    } else if (warp == 6) {
         // ---- activation columns and, for dense products, their scales ----
-        if (MODE == kDense && KIND == 8) grid_dep_wait();  // the pieces
-        const uint32_t st0 = smem_u32(ring) + kA, full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
-        uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;
-        const uint32_t tx = MODE == kDense ? (KIND == 8 ? a.b_box_bytes : sfb_tiles * a.b_box_bytes) + sfb_tiles * kMxScaleTile
-                                           : n_cols * 128;
-        const uint32_t row = MODE == kDense && KIND == 8 ? tok0 / a.group * 256 + tok0 % a.group * P : tok0;
-        if (MODE != kDense && !mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605)) goto columns_out;
-        if (MODE == kDense) {
-            const bool two = sfb_tiles > 1;
-            const uint32_t next_x = a.kt * 128, next_sf = a.kt * kMxScaleTile;   // the second tile of 128 columns
-            const uint8_t *sf = a.x_scales + ((size_t)(row / 128) * a.kt + kt0) * kMxScaleTile;
-            int x = KIND == 8 ? (int)(kt0 * 128) : (int)((row / 128 * a.kt + kt0) * 128);
-            for (uint32_t step = 0; step < steps; step++, x += 128, sf += kMxScaleTile) {
-                if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
-                mbar_expect(full, tx);
-                if (KIND == 8) {
-                    tma_2d(st, &xmap, x, (int)row, full);
-                } else {
-                    tma_2d(st, &xmap, 0, x, full);
-                    if (two) tma_2d(st + a.b_box_bytes, &xmap, 0, x + (int)next_x, full);
+        const bool listed = MODE == kDense || mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605);
+        if (MODE != kDense && listed)
+            for (uint32_t i = lane; i < n_cols; i += 32) c.rows[i] = (int32_t)row_of(i);
+        __syncwarp();
+        if (listed && elect_one()) {
+            if (MODE == kDense) grid_dep_wait();  // the pieces, or codes
+            const uint32_t st0 = smem_u32(ring) + kA, full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
+            uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;
+            const uint32_t tx = MODE == kDense ? (KIND == 8 ? a.b_box_bytes : sfb_tiles * a.b_box_bytes) + sfb_tiles * kMxScaleTile
+                                               : n_cols * 128;
+            const uint32_t row = MODE == kDense && KIND == 8 ? tok0 / a.group * 256 + tok0 % a.group * P : tok0;
+            if (MODE == kDense) {
+                const bool two = sfb_tiles > 1;
+                const uint32_t next_x = a.kt * 128, next_sf = a.kt * kMxScaleTile;   // the second tile of 128 columns
+                const uint8_t *sf = a.x_scales + ((size_t)(row / 128) * a.kt + kt0) * kMxScaleTile;
+                int x = KIND == 8 ? (int)(kt0 * 128) : (int)((row / 128 * a.kt + kt0) * 128);
+                for (uint32_t step = 0; step < steps; step++, x += 128, sf += kMxScaleTile) {
+                    if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
+                    mbar_expect(full, tx);
+                    if (KIND == 8) {
+                        tma_2d(st, &xmap, x, (int)row, full);
+                    } else {
+                        tma_2d(st, &xmap, 0, x, full);
+                        if (two) tma_2d(st + a.b_box_bytes, &xmap, 0, x + (int)next_x, full);
+                    }
+                    bulk_copy(st + b_bytes + kMxScaleTile, sf, kMxScaleTile, full);
+                    if (two) bulk_copy(st + b_bytes + 2 * kMxScaleTile, sf + next_sf, kMxScaleTile, full);
+                    issued++;
+                    st += stage_bytes, full += 8, empty += 8;
+                    if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
                 }
-                bulk_copy(st + b_bytes + kMxScaleTile, sf, kMxScaleTile, full);
-                if (two) bulk_copy(st + b_bytes + 2 * kMxScaleTile, sf + next_sf, kMxScaleTile, full);
-                issued++;
-                st += stage_bytes, full += 8, empty += 8;
-                if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
-            }
-        } else {
-            const int4 *rows = reinterpret_cast<const int4 *>(c.rows);
-            const int4 r0 = rows[0], r1 = rows[1], r2 = rows[2], r3 = rows[3];   // most experts' columns
-            for (uint32_t tile = 0; tile < tiles; tile++) {
-                int x = (int)(kt0 * 128);
-                for (uint32_t step = 0; step < steps; step++, x += 128) {
-#pragma unroll
-                    for (uint32_t mat = 0; mat < kMats; mat++) {
-                        if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
-                        mbar_expect(full, tx);
-                        tma_gather4(st, &xmap, x, r0, full);
-                        tma_gather4(st + 512, &xmap, x, r1, full);
-                        if (n_cols > 8) {
-                            tma_gather4(st + 1024, &xmap, x, r2, full);
-                            tma_gather4(st + 1536, &xmap, x, r3, full);
+            } else {
+                const int4 *rows = reinterpret_cast<const int4 *>(c.rows);
+                const int4 r0 = rows[0], r1 = rows[1], r2 = rows[2], r3 = rows[3];   // most experts' columns
+                for (uint32_t tile = 0; tile < tiles; tile++) {
+                    int x = (int)(kt0 * 128);
+                    for (uint32_t step = 0; step < steps; step++, x += 128) {
+    #pragma unroll
+                        for (uint32_t mat = 0; mat < kMats; mat++) {
+                            if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
+                            mbar_expect(full, tx);
+                            tma_gather4(st, &xmap, x, r0, full);
+                            tma_gather4(st + 512, &xmap, x, r1, full);
+                            if (n_cols > 8) {
+                                tma_gather4(st + 1024, &xmap, x, r2, full);
+                                tma_gather4(st + 1536, &xmap, x, r3, full);
+                            }
+                            for (uint32_t i = 16; i < n_cols; i += 4) tma_gather4(st + i * 128, &xmap, x, rows[i / 4], full);
+                            issued++;
+                            st += stage_bytes, full += 8, empty += 8;
+                            if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
                         }
-                        for (uint32_t i = 16; i < n_cols; i += 4) tma_gather4(st + i * 128, &xmap, x, rows[i / 4], full);
-                        issued++;
-                        st += stage_bytes, full += 8, empty += 8;
-                        if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
                     }
                 }
             }
+        columns_out:
+            if (*abort) drain(issued);
         }
-    columns_out:
-        if (*abort) drain(issued);
     } else if (warp == 1 && elect_one()) {
         // ---- MMA ----
         const uint32_t accs = tiles > 1 ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
@@ -444,24 +472,25 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     __syncwarp();
     const bool epi = warp >= 2 && warp < 6;
     if (MODE != kDense && epi) {
-        // ---- the columns: which rows of pieces, and all their scales of this CTA's share of K ----
-        const uint32_t at = threadIdx.x - 64, pairs = a.m * a.top_k;
-        if (warp == 2) {   // the expert's pairs of this chunk, in order
+        // ---- the item's tokens, and all their scales of this CTA's share of K ----
+        const uint32_t at = threadIdx.x - 64;
+        if (MODE == kGateUp) {   // its pairs, in order: every warp looks through a quarter of them
+            const uint32_t pairs = a.m * a.top_k, quarter = up_to(pairs, 128) / 4, w = warp - 2;
+            const uint32_t from = w * quarter, to = min(from + quarter, pairs);
             uint32_t seen = 0;
-#pragma unroll 4
-            for (uint32_t i = 0; i < pairs; i += 32) {
-                const bool hit = i + lane < pairs && ids[i + lane] == expert;
-                const uint32_t mask = __ballot_sync(~0u, hit), to = seen + __popc(mask & ((1u << lane) - 1));
-                if (hit && to - chunk * a.chunk < a.chunk) c.pairs[to - chunk * a.chunk] = i + lane;
+            for (uint32_t i = from; i < to; i += 32) seen += __popc(__ballot_sync(~0u, i + lane < to && ids[i + lane] == expert));
+            if (lane == 0) c.found[w] = seen;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            seen = 0;
+            for (uint32_t i = 0; i < w; i++) seen += c.found[i];
+            for (uint32_t i = from; i < to; i += 32) {
+                const bool hit = i + lane < to && ids[i + lane] == expert;
+                const uint32_t mask = __ballot_sync(~0u, hit), nth = seen + __popc(mask & ((1u << lane) - 1)) - chunk * a.chunk;
+                if (hit && nth < a.chunk) c.pairs[nth] = i + lane;
                 seen += __popc(mask);
             }
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        auto row_of = [&](uint32_t i) {   // columns past the last token repeat it
-            const uint32_t pair = c.pairs[min(i / P, tokens - 1)];
-            return (MODE == kGateUp ? pair / a.top_k : pair) * P + (i / P < tokens ? i % P : 0);
-        };
-        if (at < n_cols) c.rows[at] = (int32_t)row_of(at);
         mbar_arrive(smem_u32(&c.rows_ready));
 #pragma unroll 4
         for (uint32_t j = at; j < n_cols * steps; j += 128) {
@@ -471,6 +500,11 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
         fence_proxy_async();  // read by the tensor core's scale copy
         mbar_arrive(smem_u32(&c.scales_ready));
+        if (MODE == kGateUp && blockIdx.x == 0 && rank == 0 && warp == 2) {
+            uint32_t *it = a.items + kItemWords * (1 + blockIdx.y);
+            if (lane < tokens) it[2 + lane] = c.pairs[lane];
+            if (lane == 0) it[0] = expert, it[1] = tokens;
+        }
     }
 
     // ---- epilogue: thread = weight row ----
@@ -571,20 +605,28 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         if (epi)
-            for (uint32_t i = rank; i < tokens; i += a.split) {
-                float g[8], u[8];   // all loads go out before the first sum
+            for (uint32_t i0 = rank; i0 < tokens; i0 += 4 * a.split) {
+                float g[4] = {}, u[4] = {};   // four tokens' loads go out before the first sum
 #pragma unroll
                 for (uint32_t r = 0; r < 8; r++) {
-                    g[r] = u[r] = 0.0f;
-                    if (r < a.split) {
-                        const float *other = cluster.map_shared_rank(red, r);
-                        g[r] = other[i * 128 + q * 32 + lane];
-                        if (MODE == kGateUp) u[r] = other[(a.nt + i) * 128 + q * 32 + lane];
+                    if (r >= a.split) break;
+                    const float *other = cluster.map_shared_rank(red, r) + q * 32 + lane;
+                    float v[4], w[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) {
+                        const uint32_t i = min(i0 + j * a.split, tokens - 1);
+                        v[j] = other[i * 128];
+                        if (MODE == kGateUp) w[j] = other[(a.nt + i) * 128];
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) {
+                        g[j] += v[j];
+                        if (MODE == kGateUp) u[j] += w[j];
                     }
                 }
 #pragma unroll
-                for (uint32_t r = 1; r < 8; r++) g[0] += g[r], u[0] += u[r];
-                finish(i, g[0], u[0]);
+                for (uint32_t j = 0; j < 4; j++)
+                    if (i0 + j * a.split < tokens) finish(i0 + j * a.split, g[j], u[j]);
             }
         __syncwarp();
         cluster.barrier_arrive();   // this CTA reads the others' shared memory no more
@@ -608,6 +650,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 template <typename T, int P, int ROWS>
 __global__ void __launch_bounds__(256) pieces_kernel(const T *x, uint32_t m, uint32_t k, uint64_t stride, uint32_t kt,
                                                      uint32_t chunks, uint32_t group, uint8_t *pieces, uint8_t *scales, bool vec) {
+    grid_dep_wait();
     grid_dep_launch();  // the product may start on its weights
     const uint32_t lane = threadIdx.x % 32, w = blockIdx.x * 8 + threadIdx.x / 32;
     const uint32_t tokens = w / chunks, chunk = w - tokens * chunks, t0 = tokens * ROWS;
@@ -673,8 +716,8 @@ uint32_t pow2_cols(uint32_t v) {
 }
 
 template <int KIND, int P, int MODE>
-cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, bool dependent,
-                   cudaStream_t s) {
+cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, cudaStream_t s) {
+    if (!a.stages || a.tmem_cols > 512) return cudaErrorInvalidConfiguration;
     auto kernel = mx_tc_kernel<KIND, P, MODE>;
     if (!once_per_device(100 + KIND * 16 + P * 4 + MODE, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess;
@@ -687,13 +730,13 @@ cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArg
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = dependent ? 1 : 0;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled(kPdlMx) ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 1;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = a.split;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = a.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, a);
 }
 
@@ -708,8 +751,8 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     a.d_cols = up_to(a.nt, 8) * P;
     const uint32_t sf_cols = 4 + (a.nt * P > 128 ? 8 : 4);
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
-    const uint32_t budget = (per_sm == 1 ? 226 : 112) * 1024 - extra;
-    const uint32_t cols = per_sm == 1 ? 512 : 256;
+    const uint32_t budget = (per_sm == 1 ? 226 : per_sm == 2 ? 112 : 74) * 1024 - extra;
+    const uint32_t cols = per_sm == 1 ? 512 : per_sm == 2 ? 256 : 128;
     const uint32_t iters = (a.kt + a.split - 1) / a.split * mats * a.per_cta;
     const uint32_t acc_cols = a.d_cols * mats * (a.per_cta > 1 ? 2 : 1);
     a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, iters});
@@ -739,9 +782,10 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.per_cta = 1;
     a.nt = p.m < kGroup ? p.m : kGroup;
     const uint32_t tt = (p.m + a.nt - 1) / a.nt;
-    const uint32_t per_sm = up_to(a.nt, 8) * P <= 128 ? 2 : 1;
     a.split = 1;
-    while (a.split < 8 && rt * tt * a.split * 2 <= 148 * per_sm && kt / (a.split * 2) >= 2 && a.nt <= 64) a.split *= 2;
+    while (a.split < 8 && rt * tt * a.split * 2 <= 148 && kt / (a.split * 2) >= 2 && a.nt <= 64) a.split *= 2;
+    if (a.split < 8 && rt * tt * a.split * 2 <= 2 * 148 && kt / a.split > 24 && a.nt <= 32) a.split *= 2;
+    const uint32_t per_sm = rt * tt * a.split > 148 && up_to(a.nt, 8) * P <= 128 ? 2 : 1;
     a.w_scales = p.w_scales;
     a.x_scales = x_scales;
     a.y = p.y;
@@ -764,7 +808,7 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
                    CU_TENSOR_MAP_SWIZZLE_64B);
     }
     if (e != cudaSuccess) return e;
-    return launch<KIND, P, kDense>(wmap, xmap, a, dim3(rt, tt, a.split), smem, KIND == 8, s);
+    return launch<KIND, P, kDense>(wmap, xmap, a, dim3(rt, tt, a.split), smem, s);
 }
 
 template <typename T, int P>
@@ -778,9 +822,8 @@ cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
     const bool many = (uint64_t)(p.m / 4) * chunks >= 148 * 64;   // as the quantiser's rule
     const uint64_t warps = many ? (uint64_t)((p.m + 3) / 4) * chunks : (uint64_t)p.m * chunks;
     auto kernel = many ? pieces_kernel<T, P, 4> : pieces_kernel<T, P, 1>;
-    kernel<<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(static_cast<const T *>(p.x), p.m, p.k, p.x_stride, kt, chunks, kGroup,
-                                                       pieces, scales, vec);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_pdl(kPdlMx, kernel, (unsigned)((warps + 7) / 8), 256, 0, s, static_cast<const T *>(p.x), p.m, p.k,
+                                     p.x_stride, kt, chunks, kGroup, pieces, scales, vec);
     return e != cudaSuccess ? e : dense<8, P>(p, pieces, scales, s);
 }
 
@@ -796,6 +839,7 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.chosen = e.ws.chosen;
     a.weight = e.ws.weight;
     a.arrived = e.ws.arrived;
+    a.items = e.ws.items;
     a.h_pieces = e.ws.h_pieces;
     a.h_scales = e.ws.h_scales;
     a.partial = e.ws.partial;
@@ -811,8 +855,7 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     // as many items as there can be: one to each chosen expert, one more for every further chunk of pairs
     const uint32_t items = slots + (pairs - slots) / a.chunk;
     a.split = 1;
-    while (a.split < 8 && a.kt / (a.split * 2) >= 2 &&
-           (a.row_tiles * slots * a.split * 2 <= 148 * 2 || a.kt / a.split > 32))
+    while (a.split < 8 && a.kt / (a.split * 2) >= 2 && (a.row_tiles * slots * a.split * 2 <= 148 || a.kt / a.split > 32))
         a.split *= 2;
     // Row tiles to a CTA: its set-up (finding its tokens, their scales) costs as much as some 100 KB of
     // weights, so it takes more tiles once there are enough to go round.
@@ -832,7 +875,7 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.kt * 128,
                piece_rows, (uint64_t)a.kt * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
-    return launch<8, P, MODE>(wmap, xmap, a, dim3((a.row_tiles + a.per_cta - 1) / a.per_cta, items, a.split), smem, true, s);
+    return launch<8, P, MODE>(wmap, xmap, a, dim3((a.row_tiles + a.per_cta - 1) / a.per_cta, items, a.split), smem, s);
 }
 
 }  // namespace

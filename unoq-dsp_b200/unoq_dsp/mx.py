@@ -34,6 +34,7 @@ class UgMx4Experts(C.Structure):
 
 
 _lib = None
+_need = {}   # (m, k, type): workspace bytes of a product with 16-bit activations
 
 
 def _library():
@@ -123,7 +124,7 @@ class MX4:
     in the ``layout`` ``"operand"`` (what :func:`matmul` reads) or ``"stored"`` (row-major, the form of
     files: (rows, ceil(k/2)) and (rows, ceil(k/32)))."""
 
-    __slots__ = ("codes", "scales", "rows", "k", "layout", "device")
+    __slots__ = ("rows", "k", "layout", "device", "_data", "_codes", "_scales")
 
     def __init__(self, codes, scales, rows, k, layout="operand"):
         if rows < 0 or k < 1:
@@ -134,11 +135,38 @@ class MX4:
                 raise ValueError(f"{name} must be {want} contiguous bytes")
         if codes.device != scales.device:
             raise ValueError("codes and scales are on two devices")
-        self._set(codes, scales, rows, k, layout, codes.device)
+        self.rows, self.k, self.layout, self.device = rows, k, layout, codes.device
+        self._data, self._codes, self._scales = (codes, scales), codes.data_ptr(), scales.data_ptr()
 
-    def _set(self, *fields):
-        self.codes, self.scales, self.rows, self.k, self.layout, self.device = fields
+    @classmethod
+    def _new(cls, rows, k, layout, device):
+        """An unwritten one: both arrays in one allocation, the codes first."""
+        code_bytes, scale_bytes = _sizes(layout == "operand", rows, k)
+        at = -(-code_bytes // 16) * 16
+        self = cls.__new__(cls)
+        self.rows, self.k, self.layout, self.device = rows, k, layout, device
+        self._data = torch.empty(at + scale_bytes, dtype=torch.uint8, device=device)
+        self._codes = self._data.data_ptr()
+        self._scales = self._codes + at
         return self
+
+    def _views(self):
+        if not isinstance(self._data, tuple):
+            code_bytes, scale_bytes = _sizes(self.layout == "operand", self.rows, self.k)
+            data = self._data
+            codes, scales = data[:code_bytes], data[data.numel() - scale_bytes:]
+            if self.layout == "stored":
+                codes, scales = codes.view(self.rows, (self.k + 1) // 2), scales.view(self.rows, (self.k + 31) // 32)
+            self._data = (codes, scales)
+        return self._data
+
+    @property
+    def codes(self):
+        return self._views()[0]
+
+    @property
+    def scales(self):
+        return self._views()[1]
 
     @property
     def shape(self):
@@ -155,8 +183,8 @@ class MX4:
         else:
             _output(out, (rows, k), dtype, device, (self.codes, self.scales))
             stride = _row_stride(out, rows, k)
-        rc = lib.ug_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), _layout(self.layout), rows, k,
-                                   out.data_ptr(), _TYPES[dtype], stride, _stream(device))
+        rc = lib.ug_mx4_dequantize(self._codes, self._scales, self.layout == "operand", rows, k, out.data_ptr(),
+                                   _TYPES[dtype], stride, _stream(device))
         if rc:
             _check(lib, rc, "MX4 dequantise")
         return out
@@ -174,17 +202,11 @@ def quantize(x, layout="operand"):
     most 6 scales; a block holding a NaN or an infinity becomes NaN."""
     x, rows, k, stride = _rows(_input(x, "x", _TYPES), "x")
     lib, code, device = _library(), _layout(layout), x.device
-    if code:
-        shapes = _sizes(code, rows, k)
-    else:
-        shapes = (rows, (k + 1) // 2), (rows, (k + 31) // 32)
-    codes = torch.empty(shapes[0], dtype=torch.uint8, device=device)
-    scales = torch.empty(shapes[1], dtype=torch.uint8, device=device)
-    rc = lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, stride, code, codes.data_ptr(), scales.data_ptr(),
-                             _stream(device))
+    q = MX4._new(rows, k, layout, device)
+    rc = lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, stride, code, q._codes, q._scales, _stream(device))
     if rc:
         _check(lib, rc, "MX4 quantise")
-    return MX4.__new__(MX4)._set(codes, scales, rows, k, layout, device)
+    return q
 
 
 def _stored_pair(codes, scales, k, what):
@@ -243,18 +265,22 @@ def matmul(a, w, dtype=None, out=None):
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=device)
     else:
-        _output(out, shape, dtype, device, (a.codes, a.scales, w.codes, w.scales) if four else (a, w.codes, w.scales))
+        _output(out, shape, dtype, device, ((a.codes, a.scales) if four else (a,)) + (w.codes, w.scales))
         if out.dim() == 2:
             stride = _row_stride(out, m, n)
     if four:
-        rc = lib.ug_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), m, w.codes.data_ptr(), w.scales.data_ptr(), n, k,
-                               out.data_ptr(), _TYPES[dtype], stride, _stream(device))
+        rc = lib.ug_mx4_matmul(a._codes, a._scales, m, w._codes, w._scales, n, k, out.data_ptr(), _TYPES[dtype], stride,
+                               _stream(device))
     else:
         x_type = _TYPES[a.dtype]
-        need = lib.ug_mx4_matmul_x16_workspace(m, k, x_type)
+        need = _need.get((m, k, x_type))
+        if need is None:
+            if len(_need) > 4096:
+                _need.clear()
+            need = _need[m, k, x_type] = lib.ug_mx4_matmul_x16_workspace(m, k, x_type)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = lib.ug_mx4_matmul_x16(a.data_ptr(), x_type, a_stride, m, w.codes.data_ptr(), w.scales.data_ptr(), n, k,
-                                   out.data_ptr(), _TYPES[dtype], stride, ws.data_ptr(), need, _stream(device))
+        rc = lib.ug_mx4_matmul_x16(a.data_ptr(), x_type, a_stride, m, w._codes, w._scales, n, k, out.data_ptr(),
+                                   _TYPES[dtype], stride, ws.data_ptr(), need, _stream(device))
     if rc:
         _check(lib, rc, "MX4 product")
     return out
