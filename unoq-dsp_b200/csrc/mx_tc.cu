@@ -715,6 +715,8 @@ uint32_t pow2_cols(uint32_t v) {
     return c;
 }
 
+#include "mx_pair.cuh"
+
 template <int KIND, int P, int MODE>
 cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, cudaStream_t s) {
     if (!a.stages || a.tmem_cols > 512) return cudaErrorInvalidConfiguration;
@@ -773,6 +775,7 @@ template <int KIND, int P>
 cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_scales, cudaStream_t s) {
     const uint32_t kt = mx_tiles(p.k), rt = mx_tiles(p.n);
     constexpr uint32_t kGroup = P == 1 ? 256 : P == 2 ? 128 : 64;   // tokens that fill 256 columns (P = 3: 192)
+    if (p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 37) return pair_product<KIND, P>(p, x, x_scales, s);
     TcArgs a{};
     a.m = p.m;
     a.n = p.n;
