@@ -7,10 +7,11 @@
  * layouts:
  *   UG_MX4_STORED   codes[r * ceil(k/2) + j/2], the even j in the low nibble, and
  *                   scales[r * ceil(k/32) + j/32]: the exchange form of files.
- *   UG_MX4_OPERAND  what the products read: 128 rows x 128 values to a tile, tiles of a row next to
- *                   each other. With T = (r / 128) * ceil(k/128) + j / 128, codes at
- *                   T * 8192 + (r % 128) * 64 + (j % 128) / 2 and scales at
- *                   T * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + (j / 32 % 4). Values past k are zero.
+ *   UG_MX4_OPERAND  what the products read, 128 rows to a tile, the tiles of 128 rows next to each other:
+ *                   codes in tiles of 256 values, ((r / 128) * K + j / 256) * 16384 + (r % 128) * 128 +
+ *                   (j % 256) / 2 with K = ceil(k/256), and scales in tiles of 128 values,
+ *                   ((r / 128) * 2K + j / 128) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + (j / 32 % 4).
+ *                   Values and scale bytes past k, up to 256 K, are zero.
  * A last block or tile may be partial: rows and k are free (k >= 1).
  *
  * Every array is DEVICE memory of one device, `stream` is a cudaStream_t of that device (NULL: its
@@ -59,7 +60,7 @@ UG_API int ug_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int la
                              void *y, int type, uint64_t stride, void *stream);
 /* `count` stored matrices of rows x k, one after another -> operand layout, each matrix's rows padded
  * to whole tiles of its own. paired = 1: rows is even, the first half of each matrix are gate rows
- * and the second half up rows; tiles alternate, 128 gate rows, then the 128 up rows beside them
+ * and the second half up rows; a tile holds 64 gate rows, then the 64 up rows beside them
  * (ug_mx4_experts reads gate_up so). Array sizes: ug_mx4_pack_rows rows of the operand layout. */
 UG_API int ug_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_t count, uint32_t rows, uint32_t k,
                        int paired, uint8_t *packed_codes, uint8_t *packed_scales, void *stream);

@@ -51,14 +51,14 @@ def operand(codes, scales, k, paired=False):
     n = codes.shape[0]
     if paired:
         half = n // 2
-        tiles = -(-half // 128)
+        tiles = -(-half // 64)
         order = []
         for t in range(tiles):
             for part in range(2):
-                order += [part * half + t * 128 + i if t * 128 + i < half else -1 for i in range(128)]
+                order += [part * half + t * 64 + i if t * 64 + i < half else -1 for i in range(64)]
     else:
         order = [r if r < n else -1 for r in range(-(-n // 128) * 128)]
-    kt = -(-k // 128)
+    kt = -(-k // 256) * 2
     out_c = torch.zeros(len(order) // 128 * kt * 8192, dtype=torch.uint8)
     out_s = torch.zeros(len(order) // 128 * kt * 512, dtype=torch.uint8)
     wide = torch.zeros(n, kt * 64, dtype=torch.uint8)
@@ -72,7 +72,7 @@ def operand(codes, scales, k, paired=False):
             continue
         for t in range(kt):
             at = (to // 128 * kt + t)
-            out_c[at * 8192 + to % 128 * 64:][:64] = wide[r, t * 64:t * 64 + 64]
+            out_c[at // 2 * 16384 + to % 128 * 128 + t % 2 * 64:][:64] = wide[r, t * 64:t * 64 + 64]
             out_s[at * 512 + to % 32 * 16 + to % 128 // 32 * 4:][:4] = ws[r, t * 4:t * 4 + 4]
     return out_c, out_s
 

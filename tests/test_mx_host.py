@@ -12,11 +12,12 @@ P = 1 << 20  # a well-aligned address that is never followed: every call here is
 
 def test_sizes(native):
     assert native.ug_mx4_codes_bytes(0, 5, 33) == 5 * 17 and native.ug_mx4_scales_bytes(0, 5, 33) == 10
-    assert native.ug_mx4_codes_bytes(1, 129, 129) == 4 * 8192 and native.ug_mx4_scales_bytes(1, 129, 129) == 4 * 512
+    assert native.ug_mx4_codes_bytes(1, 129, 257) == 4 * 16384 and native.ug_mx4_scales_bytes(1, 129, 257) == 8 * 512
+    assert native.ug_mx4_codes_bytes(1, 128, 1) == 16384 and native.ug_mx4_scales_bytes(1, 1, 256) == 1024
     assert native.ug_mx4_codes_bytes(2, 5, 33) == 0 and native.ug_mx4_scales_bytes(-1, 5, 33) == 0
-    assert native.ug_mx4_codes_bytes(1, 2 ** 32 - 1, 128) == 2 ** 25 * 8192  # past 32 bits
+    assert native.ug_mx4_codes_bytes(1, 2 ** 32 - 1, 128) == 2 ** 25 * 16384  # past 32 bits
     assert native.ug_mx4_pack_rows(3, 130, 0) == 3 * 256 and native.ug_mx4_pack_rows(3, 130, 1) == 3 * 256
-    assert native.ug_mx4_pack_rows(2, 260, 1) == 2 * 512
+    assert native.ug_mx4_pack_rows(2, 260, 1) == 2 * 384 and native.ug_mx4_pack_rows(2, 128, 1) == 256
     assert native.ug_mx4_pack_rows(2 ** 31, 130, 0) == 0  # does not fit
     assert native.ug_mx4_matmul_x16_workspace(3, 100, 0) == 0
     assert native.ug_mx4_matmul_x16_workspace(3, 100, 2) >= 6 * 128 + 512

@@ -14,7 +14,7 @@ namespace cg = cooperative_groups;
 
 // ---- quantise / dequantise -------------------------------------------------------------------
 //
-// A warp takes 256 columns (two operand tiles' width, 8 values to a lane, four lanes to a block of
+// A warp takes 256 columns (a code tile's width, 8 values to a lane, four lanes to a block of
 // 32) of ROWS consecutive rows: the loads of all of them go out first, and a row's addresses are the
 // one before's plus a constant. What bounds it is memory, once the instructions are few: with one
 // row to a thread and its indices by division, 168 instructions a thread held a matrix of 8192 x 8192
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T *x, uint32_t rows
     const uint32_t row_bytes = (k + 1) / 2, blocks = (k + 31) / 32;
     uint8_t *to = codes + (OPERAND ? mx_code_at(r0, j, kt) : (size_t)r0 * row_bytes + j / 2);
     uint8_t *st = scales + (OPERAND ? mx_scale_at(r0, j / 32, kt) : (size_t)r0 * blocks + j / 32);
-    const bool mine = OPERAND ? j / kMxTile < kt : j < k;
+    const bool mine = OPERAND || j < k;   // a code tile is written whole
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         if ((uint32_t)i >= n) break;
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T *x, uint32_t rows
             }
             if (lane % 4 == 0) *st = (uint8_t)s;
         }
-        to += OPERAND ? 64 : row_bytes;
+        to += OPERAND ? 128 : row_bytes;
         st += OPERAND ? 16 : blocks;
     }
 }
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, c
             }
             s[i] = __ldg(sf);
         }
-        from += OPERAND ? 64 : row_bytes;
+        from += OPERAND ? 128 : row_bytes;
         sf += OPERAND ? 16 : blocks;
     }
     if (!vec_out) {
@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t *codes, const u
         const uint32_t matrix = (uint32_t)(out_row / padded), pr = (uint32_t)(out_row - (uint64_t)matrix * padded);
         uint32_t r = pr;   // source row, or `rows` for padding
         if (paired) {
-            const uint32_t half = rows / 2, i = pr / 256 * 128 + pr % 128;
-            r = i < half ? i + (pr / 128 % 2 ? half : 0) : rows;
+            const uint32_t half = rows / 2, i = pr / kMxTile * kMxHalf + pr % kMxHalf;
+            r = i < half ? i + (pr % kMxTile < kMxHalf ? 0 : half) : rows;
         }
         uint32_t c = 0;
         if (r < rows) {
@@ -164,9 +164,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t *codes, const u
                 c |= b << (8 * i);
             }
         }
-        const size_t t = out_row / kMxTile * kt + tile;
+        const size_t row_tile = out_row / kMxTile, t = row_tile * kt + tile;
         const uint32_t tr = (uint32_t)(out_row % kMxTile);
-        *reinterpret_cast<uint32_t *>(out_codes + t * kMxCodeTile + tr * 64 + lane * 4) = c;
+        *reinterpret_cast<uint32_t *>(out_codes + (row_tile * (kt / 2) + tile / 2) * kMxCodeTile + tr * 128 + tile % 2 * 64 +
+                                      lane * 4) = c;
         if (lane < 4) {
             const uint32_t b = tile * 4 + lane;
             out_scales[t * kMxScaleTile + tr % 32 * 16 + tr / 32 * 4 + lane] =
@@ -343,7 +344,7 @@ template <typename T>
 cudaError_t quantize(const void *x, uint32_t rows, uint32_t k, uint64_t stride, int layout, uint8_t *codes,
                      uint8_t *scales, cudaStream_t s) {
     constexpr int kRows = sizeof(T) == 4 ? 4 : 8;
-    const uint32_t kt = mx_tiles(k), chunks = (k + 255) / 256;
+    const uint32_t kt = mx_ktiles(k), chunks = (k + 255) / 256;
     const bool vec_in = aligned(x, 16) && stride * sizeof(T) % 16 == 0;
     const bool vec_out = aligned(codes, 4) && (k + 1) / 2 % 4 == 0;
     const bool many = many_rows(rows, chunks, kRows);
@@ -357,7 +358,7 @@ template <typename T>
 cudaError_t dequantize(const uint8_t *codes, const uint8_t *scales, int layout, uint32_t rows, uint32_t k, void *y,
                        uint64_t stride, cudaStream_t s) {
     constexpr int kRows = 8;
-    const uint32_t kt = mx_tiles(k), chunks = (k + 255) / 256;
+    const uint32_t kt = mx_ktiles(k), chunks = (k + 255) / 256;
     const bool vec_in = aligned(codes, 4) && (k + 1) / 2 % 4 == 0;
     const bool vec_out = aligned(y, 16) && stride * sizeof(T) % 16 == 0;
     const bool many = many_rows(rows, chunks, kRows);
@@ -385,7 +386,7 @@ cudaError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, i
 
 cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_t count, uint32_t rows, uint32_t k,
                             int paired, uint8_t *out_codes, uint8_t *out_scales, cudaStream_t s) {
-    const uint32_t padded = (paired ? 2 * mx_tiles(rows / 2) : mx_tiles(rows)) * kMxTile, kt = mx_tiles(k);
+    const uint32_t padded = (paired ? (rows / 2 + kMxHalf - 1) / kMxHalf : mx_tiles(rows)) * kMxTile, kt = mx_ktiles(k);
     const uint64_t units = (uint64_t)count * padded * kt;
     pack_kernel<<<unit_grid(units), 256, 0, s>>>(codes, scales, rows, k, paired, padded, kt, units, out_codes, out_scales);
     return cudaGetLastError();

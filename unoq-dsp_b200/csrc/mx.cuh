@@ -1,9 +1,10 @@
 // mx.cuh -- microscaled 4-bit (MX4) operators: layouts, number conversions and launchers shared by
 // k_mx.cu (quantisation, packing, activation pieces, router), mx_tc.cu (products) and mx_abi.cu.
 //
-// Types are UgMxType (0 f32, 1 f16, 2 bf16). Operand layout: tiles of 128 rows x 128 values, one
-// tile's codes 8192 contiguous bytes and its scales 512, in the order that the tensor cores' scale
-// copy takes (unoq_mx.h).
+// Types are UgMxType (0 f32, 1 f16, 2 bf16). Operand layout: code tiles of 128 rows x 256 values, 128
+// contiguous bytes a row (copies of 128-byte rows run at 18.3 TB/s from L2, of 64-byte rows at 13.7),
+// and scale tiles of 128 rows x 128 values, 512 bytes in the order that the tensor cores' scale copy
+// takes (unoq_mx.h).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -14,19 +15,22 @@
 
 namespace uq {
 
-constexpr int kMxTile = 128;          // rows and values of an operand tile
-constexpr int kMxCodeTile = 8192;     // bytes of its codes
-constexpr int kMxScaleTile = 512;     // bytes of its scales
+constexpr int kMxTile = 128;          // rows of a tile, values of a scale tile
+constexpr int kMxCodeTile = 16384;    // bytes of a code tile, 128 x 256
+constexpr int kMxScaleTile = 512;     // bytes of a scale tile, 128 x 128
+constexpr int kMxHalf = 64;           // gate rows, and up rows, of a tile of paired matrices
 constexpr int kMxHiddenPieces = 3;    // pieces of the hidden vector of ug_mx4_experts
 constexpr int kMxRouterCluster = 8;   // CTAs that share one token's router product
 
 __host__ __device__ inline uint32_t mx_tiles(uint32_t n) { return (n + kMxTile - 1) / kMxTile; }
+// Scale tiles along a row of k values, two to a code tile.
+__host__ __device__ inline uint32_t mx_ktiles(uint32_t k) { return (k + 255) / 256 * 2; }
 // Pieces of a 16-bit value: 4 significant bits each, so two hold a bf16 (8) and three an f16 (11).
 __host__ __device__ inline int mx_pieces(int type) { return type == 2 ? 2 : 3; }
 
 #ifdef __CUDACC__
 __device__ __forceinline__ size_t mx_code_at(uint32_t r, uint32_t j, uint32_t kt) {
-    return ((size_t)(r / kMxTile) * kt + j / kMxTile) * kMxCodeTile + (r % kMxTile) * 64 + (j % kMxTile) / 2;
+    return ((size_t)(r / kMxTile) * (kt / 2) + j / 256) * kMxCodeTile + (r % kMxTile) * 128 + j % 256 / 2;
 }
 __device__ __forceinline__ size_t mx_scale_at(uint32_t r, uint32_t b, uint32_t kt) {
     return ((size_t)(r / kMxTile) * kt + b / 4) * kMxScaleTile + (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4;

@@ -68,8 +68,8 @@ int launched(cudaError_t e) {
     return fail(2001, cudaGetErrorString(e));
 }
 
-// rows x k with ceil(k/128) tiles each: counted in 32 bits by the kernels
-bool sizes_ok(uint64_t rows, uint32_t k) { return k >= 1 && rows * uq::mx_tiles(k) < (1ull << 31) && k <= (1u << 30); }
+// rows x k with so many tiles each: counted in 32 bits by the kernels
+bool sizes_ok(uint64_t rows, uint32_t k) { return k >= 1 && k <= (1u << 30) && rows * uq::mx_ktiles(k) < (1ull << 31); }
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -113,13 +113,13 @@ extern "C" {
 
 size_t ug_mx4_codes_bytes(int layout, uint32_t rows, uint32_t k) {
     if (layout == UG_MX4_STORED) return (size_t)rows * ((k + 1ull) / 2);
-    if (layout == UG_MX4_OPERAND) return (size_t)((rows + 127ull) / 128) * ((k + 127ull) / 128) * uq::kMxCodeTile;
+    if (layout == UG_MX4_OPERAND) return (size_t)((rows + 127ull) / 128) * ((k + 255ull) / 256) * uq::kMxCodeTile;
     return 0;
 }
 
 size_t ug_mx4_scales_bytes(int layout, uint32_t rows, uint32_t k) {
     if (layout == UG_MX4_STORED) return (size_t)rows * ((k + 31ull) / 32);
-    if (layout == UG_MX4_OPERAND) return (size_t)((rows + 127ull) / 128) * ((k + 127ull) / 128) * uq::kMxScaleTile;
+    if (layout == UG_MX4_OPERAND) return (size_t)((rows + 127ull) / 128) * ((k + 255ull) / 256) * 2 * uq::kMxScaleTile;
     return 0;
 }
 
@@ -153,7 +153,7 @@ int ug_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int layout, u
 }
 
 uint32_t ug_mx4_pack_rows(uint32_t count, uint32_t rows, int paired) {
-    const uint64_t per = paired ? 256ull * ((rows / 2 + 127ull) / 128) : 128ull * ((rows + 127ull) / 128);
+    const uint64_t per = paired ? 128ull * ((rows / 2 + 63ull) / 64) : 128ull * ((rows + 127ull) / 128);
     const uint64_t all = per * count;
     return all < (1ull << 32) ? (uint32_t)all : 0;
 }

@@ -1,16 +1,16 @@
 // mx_pair.cuh -- the MX4 product of many tokens (included by mx_tc.cu): pairs of CTAs.
 //
 // At 256 columns a tile of mx_tc_kernel reads 26 KB of operands per 128 x 256 x 128 block, 102 bytes a
-// cycle and SM at the rate of the 4-bit tensor cores, several times what the L2 delivers (about 36 here).
+// cycle and SM at the rate of the 4-bit tensor cores; the L2 delivers 64 (18.3 TB/s measured).
 // A pair of CTAs (tcgen05 cta_group::2) multiplies 256 weight rows by 256 columns: each CTA loads its own
 // 128 rows and half of the columns, both tensor cores read both halves, and the traffic falls to
-// 17 KB for twice the work. The kernel is persistent, one pair to two SMs. Its epilogue (8 warps) first
+// 17 KB for as much work of an SM. The kernel is persistent, one pair to two SMs. Its epilogue (8 warps) first
 // takes a tile's accumulators into registers, which gives TMEM back to the MMAs within some hundred
 // cycles, and writes them while the next tile is multiplied.
 #pragma once
 
 struct PairArgs {
-    uint32_t m, n, kt, rt;                // tokens, weight rows, tiles along K, row tiles
+    uint32_t m, n, steps, kw, rt;         // tokens, weight rows, stages and code tiles along K, row tiles
     uint32_t row_pairs, tiles;            // pairs of row tiles; times token tiles
     uint32_t stages, stage_bytes, group;
     void *y;
@@ -81,10 +81,10 @@ template <int KIND, int P>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     mx_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap, const PairArgs a) {
-    constexpr uint32_t kA = KIND == 8 ? 16384 : 8192;              // one weight tile in shared memory
     constexpr uint32_t kTokens = P == 1 ? 256 : P == 2 ? 128 : 64, kN = kTokens * P;
-    constexpr uint32_t kB = kN / 2 * (KIND == 8 ? 128 : 64);       // this CTA's half of the columns
-    constexpr uint32_t kSfCols = 4 + 8;
+    constexpr uint32_t kB = kN / 2 * 128;                          // this CTA's half of the columns
+    constexpr uint32_t kSub = KIND == 8 ? 1 : 2, kSf = kSub * kMxScaleTile;   // scales of a stage, per 128 rows
+    constexpr uint32_t kSfCols = kSub * (4 + 8);
     extern __shared__ uint8_t raw[];
     uint8_t *base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     PairCtrl &c = *reinterpret_cast<PairCtrl *>(base);
@@ -131,12 +131,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1;
         for (uint32_t t = pair; t < a.tiles; t += pairs) {
             // the row tile past an odd number of them: past the matrix, zeros
-            int y = (int)((2 * (t % a.row_pairs) + rank) * a.kt);
-            for (uint32_t k = 0; k < a.kt; k++, y++) {
+            const uint32_t tile = 2 * (t % a.row_pairs) + rank;
+            int x = 0, y = (int)(tile * a.kw * 128), sf = (int)(tile * 2 * a.kw);
+            for (uint32_t k = 0; k < a.steps; k++, sf += kSub) {
                 if (!mbar_poll(empty, phase, abort, 611)) goto weights_out;
-                if (rank == 0) mbar_expect(smem_u32(&c.full[s]), 2 * (kMxCodeTile + kMxScaleTile));
-                pair_tma_2d(st, &wmap, 0, y * 128, full);
-                pair_tma_2d(st + kA + kB, &wsmap, 0, y, full);
+                // an unpacking copy counts what it reads
+                if (rank == 0) mbar_expect(smem_u32(&c.full[s]), 2 * ((KIND == 8 ? kMxCodeTile / 2 : kMxCodeTile) + kSf));
+                pair_tma_2d(st, &wmap, x, y, full);
+                pair_tma_2d(st + kA + kB, &wsmap, 0, sf, full);
+                if (KIND == 8) x ^= 128;
+                if (x == 0) y += 128;
                 st += stage_bytes, full += 8, empty += 8;
                 if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
             }
@@ -151,13 +155,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         for (uint32_t t = pair; t < a.tiles; t += pairs) {
             const int tt = (int)(t / a.row_pairs);   // 256 rows of codes or pieces, two scale tiles, to a token tile
             const int row = tt * 256 + (int)rank * (int)(kN / 2);
-            int x = KIND == 8 ? 0 : (2 * tt + (int)rank) * (int)a.kt * 128;
-            for (uint32_t k = 0; k < a.kt; k++, x += 128) {
+            int x = KIND == 8 ? 0 : (2 * tt + (int)rank) * (int)a.kw * 128;
+            for (uint32_t k = 0; k < a.steps; k++, x += 128) {
                 if (!mbar_poll(empty, phase, abort, 618)) goto columns_out;
-                if (rank == 0) mbar_expect(smem_u32(&c.full[s]), 2 * (kB + 2 * kMxScaleTile));
+                if (rank == 0) mbar_expect(smem_u32(&c.full[s]), 2 * (kB + 2 * kSf));
                 if (KIND == 8) pair_tma_2d(st, &xmap, x, row, full);
                 else pair_tma_2d(st, &xmap, 0, x, full);
-                pair_tma_3d(st + kB + kMxScaleTile, &xsmap, 0, (int)k, 2 * tt, full);
+                pair_tma_3d(st + kB + kSf, &xsmap, 0, (int)(k * kSub), 2 * tt, full);
                 st += stage_bytes, full += 8, empty += 8;
                 if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
             }
@@ -166,29 +170,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (*abort) drain();
     } else if (warp == 1 && rank == 0 && elect_one()) {
         // ---- MMA of the pair ----
-        const uint32_t types = KIND == 8 ? (5u << 7) : (1u << 7) | (1u << 10);
-        const uint32_t idesc = types | (kN >> 3) << 17 | 1u << 23 | 2u << 27;   // e8m0 scales, M = 256
+        const uint32_t idesc = scaled_instr_desc<KIND>(256, kN);
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         const uint32_t sf0 = tmem + kN;
         uint32_t st = st0, full = full0, empty = empty0, sfa = sf0, s = 0, phase = 0, nth = 0;
         bool ok = true;
         for (uint32_t t = pair; ok && t < a.tiles; t += pairs, nth++) {
             if (nth && !mbar_poll(smem_u32(&c.acc_empty), (nth - 1) & 1, abort, 617)) break;
-            for (uint32_t k = 0; k < a.kt; k++) {
+            for (uint32_t k = 0; k < a.steps; k++) {
                 if (!mbar_poll(full, phase, abort, 612)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t b = st + kA, sf = b + kB, sfb = sfa + 4;
-                pair_scales_to_tmem(sfa, sf);
-                pair_scales_to_tmem(sfb, sf + kMxScaleTile);
-                pair_scales_to_tmem(sfb + 4, sf + 2 * kMxScaleTile);
-                const uint64_t ad = operand_desc<KIND>(st), bd = operand_desc<KIND>(b);
+                const uint32_t b = st + kA, sf = b + kB, sfb = sfa + 4 * kSub;
 #pragma unroll
-                for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
-                    const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
-                    pair_mma<KIND>(tmem, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa, sfb, k | j);
+                for (uint32_t h = 0; h < kSub; h++) {
+                    pair_scales_to_tmem(sfa + 4 * h, sf + h * kMxScaleTile);
+                    pair_scales_to_tmem(sfb + 8 * h, sf + kSf + h * kMxScaleTile);
+                    pair_scales_to_tmem(sfb + 8 * h + 4, sf + 2 * kSf + h * kMxScaleTile);
+                }
+                const uint64_t ad = smem_desc(st), bd = smem_desc(b);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {   // 32 bytes of each row at a time
+                    const uint32_t h = KIND == 8 ? 0 : j / 2, id = KIND == 8 ? j : j % 2 * 2;   // which scale bytes
+                    pair_mma<KIND>(tmem, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa + 4 * h, sfb + 8 * h, k | j);
                 }
                 pair_commit(empty);
                 st += stage_bytes, full += 8, empty += 8, sfa += kSfCols;
@@ -238,36 +244,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
 template <int KIND, int P>
 cudaError_t pair_product(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_scales, cudaStream_t s) {
-    constexpr uint32_t kTokens = P == 1 ? 256 : P == 2 ? 128 : 64, kN = kTokens * P;
-    constexpr uint32_t kB = kN / 2 * (KIND == 8 ? 128 : 64);
+    constexpr uint32_t kTokens = P == 1 ? 256 : P == 2 ? 128 : 64, kN = kTokens * P, kB = kN / 2 * 128, kSub = KIND == 8 ? 1 : 2;
     PairArgs a{};
     a.m = p.m;
     a.n = p.n;
-    a.kt = mx_tiles(p.k);
+    a.kw = mx_ktiles(p.k) / 2;
+    a.steps = KIND == 8 ? mx_tiles(p.k) : a.kw;
     a.rt = mx_tiles(p.n);
     a.row_pairs = (a.rt + 1) / 2;
     a.tiles = a.row_pairs * ((p.m + kTokens - 1) / kTokens);
-    a.stage_bytes = (KIND == 8 ? 16384 : 8192) + kB + 2048;
-    a.stages = std::min<uint32_t>({(226 * 1024 - 1024 - kCtrlBytes) / a.stage_bytes, (512 - kN) / 12, (uint32_t)kMaxStages});
+    a.stage_bytes = kA + kB + up_to(3 * kSub * kMxScaleTile, 1024);
+    a.stages = std::min<uint32_t>({(226 * 1024 - 1024 - kCtrlBytes) / a.stage_bytes, (512 - kN) / (12 * kSub), (uint32_t)kMaxStages});
     a.y = p.y;
     a.type = p.type;
     a.stride = p.stride;
     CUtensorMap wmap, xmap, wsmap, xsmap;
     const uint64_t rows = KIND == 8 ? mx_piece_rows(p.m, p.x_type) : (uint64_t)mx_tiles(p.m) * 128;
-    cudaError_t e = encode_weights<KIND>(&wmap, p.w_codes, (uint64_t)a.rt * a.kt);
+    cudaError_t e = encode_weights<KIND>(&wmap, p.w_codes, (uint64_t)a.rt * a.kw);
     if (e != cudaSuccess) return e;
     if (KIND == 8)
-        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)a.kt * 128, rows, (uint64_t)a.kt * 128, 128, kN / 2,
+        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)a.steps * 128, rows, (uint64_t)a.steps * 128, 128, kN / 2,
                    CU_TENSOR_MAP_SWIZZLE_128B);
     else
-        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 64, rows * a.kt, 64, 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
+        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 128, rows * a.kw, 128, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (e != cudaSuccess) return e;
-    // scale tiles as rows of 128 words; the columns' two tiles of a step in one copy
-    e = encode(&wsmap, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.w_scales, 128, (uint64_t)a.rt * a.kt, kMxScaleTile, 128, 1,
+    // scale tiles as rows of 128 words; a stage's for both tiles of columns in one copy
+    e = encode(&wsmap, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.w_scales, 128, (uint64_t)a.rt * 2 * a.kw, kMxScaleTile, 128, kSub,
                CU_TENSOR_MAP_SWIZZLE_NONE);
     if (e != cudaSuccess) return e;
-    const cuuint64_t dims[3] = {128, a.kt, (rows + 127) / 128}, strides[2] = {kMxScaleTile, (cuuint64_t)a.kt * kMxScaleTile};
-    const cuuint32_t box[3] = {128, 1, 2}, ones[3] = {1, 1, 1};
+    const cuuint64_t along = a.steps * kSub;
+    const cuuint64_t dims[3] = {128, along, (rows + 127) / 128}, strides[2] = {kMxScaleTile, along * kMxScaleTile};
+    const cuuint32_t box[3] = {128, kSub, 2}, ones[3] = {1, 1, 1};
     if (encoder()(&xsmap, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t *>(x_scales), dims, strides, box, ones,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)

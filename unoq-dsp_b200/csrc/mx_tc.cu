@@ -5,20 +5,23 @@
 // are the M side whatever the number of tokens, so a single token streams the same weight tiles
 // as a prompt does, and its column count N is the multiple of 8 that holds it. Two kinds:
 //
-//   KIND 4  kind::mxf4: both sides e2m1, 64 values per instruction.
+//   KIND 4  kind::mxf4: both sides e2m1, 64 values per instruction, 256 to a stage.
 //   KIND 8  kind::mxf8f6f4: weights e2m1 (TMA unpacks each 4-bit code to a byte of shared memory),
-//           activations e4m3. A 16-bit activation is not rounded to e4m3: it is split into P pieces of
-//           four significant bits, x = 2^s (p0 + p1 / 16 + p2 / 256) (P = 2 holds bf16's 8 bits, 3
-//           f16's 11), each piece a column of its own whose block scale carries its power of 16;
-//           the epilogue adds the P columns in 32 bits. Few tokens leave the columns unused
+//           activations e4m3, 128 values to a stage. A 16-bit activation is not rounded to e4m3: it is
+//           split into P pieces of four significant bits, x = 2^s (p0 + p1 / 16 + p2 / 256) (P = 2 holds
+//           bf16's 8 bits, 3 f16's 11), each piece a column of its own whose block scale carries its
+//           power of 16; the epilogue adds the P columns in 32 bits. Few tokens leave the columns unused
 //           otherwise, and a 16-bit tensor-core product would need the weights expanded in registers.
+//
+// In either kind a stage is 128 weight rows of 128 bytes and N columns of 128 bytes in shared memory
+// (SWIZZLE_128B) and takes four MMAs.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 
 #include "device_state.hpp"
 #include "mx.cuh"
-#include "tc_common.cuh"
+#include "mx_mma.cuh"
 
 namespace uq {
 namespace {
@@ -30,187 +33,57 @@ constexpr int kThreads = 224;      // warp 0: weight copies, warp 1: MMA, warps 
 constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
 constexpr int kItemWords = 2 + 32; // an item: expert, tokens, the pairs
 constexpr int kChunk = 32;         // most tokens of one expert that one CTA takes
+constexpr uint32_t kA = 16384;     // one weight tile in shared memory
 
 __host__ __device__ constexpr uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
 enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
 
 struct TcArgs {
-    uint32_t m, n, kt;        // tokens, weight rows of one matrix, tiles along K
+    uint32_t m, n;            // tokens, weight rows of one matrix
+    uint32_t steps, kw;       // stages along K (256 values in KIND 4, 128 in KIND 8), code tiles along K
     uint32_t nt;              // tokens of a full CTA tile
     uint32_t group;           // tokens per 256 rows of pieces (KIND 8, kDense)
     uint32_t stages, split;   // ring depth; CTAs of a cluster that share a tile's K
-    uint32_t stage_bytes, b_bytes, b_box_bytes, tmem_cols, d_cols, ring_bytes;
+    uint32_t stage_bytes, b_bytes, b_box_bytes, tmem_cols, d_cols, ring_bytes, row_tiles;
     const uint8_t *w_scales, *x_scales;
     void *y;
     int type;
     uint64_t stride;
     // experts
-    uint32_t top_k, row_tiles, per_cta, chunk, head_bytes;   // head: the choices and the columns' scales
+    uint32_t top_k, per_cta, chunk, head_bytes;   // head: the choices, the columns' scales, gate and up values
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
     uint32_t *items;          // the gate / up product's work items, for the down product
     uint8_t *h_pieces, *h_scales;
+    uint32_t h_steps;         // scale words along a hidden row
     float *partial;
 };
 
 struct Ctrl {
     unsigned long long full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+    unsigned long long rows_ready, scales_ready, spare;
     uint32_t tmem;
     int abort;
-    unsigned long long rows_ready, scales_ready, spare;
     uint32_t pairs[kChunk], found[4];
     alignas(16) int32_t rows[kChunk * 4];
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 
-// One thread of a converged warp. The copy and MMA threads are chosen so, and not by their lane number: the
-// compiler then knows that one thread runs, and issues a copy in about 15 cycles, not 55.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-
-// Bounded wait that polls instead of suspending: what the copy and MMA threads wait for is mostly there, or
-// comes within some hundred cycles, and a wait with a suspension limit costs 63 cycles even then, a
-// plain one 27.
-__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int *abort, int code) {
-    for (int i = 0; i < 64; i++) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok)
-                     : "r"(bar), "r"(parity)
-                     : "memory");
-        if (ok) return true;
-    }
-    return mbar_wait(bar, parity, abort, code);
-}
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
-        : "memory");
-}
-// Four rows of 128 bytes from anywhere in the matrix (the map's box is one row high).
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int c0, int4 r, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5, %6}], [%7];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
-}
-
-// One 512-byte scale tile (128 rows x 4 blocks) into 4 TMEM columns, repeated for the four lane quarters.
-__device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t smem) {
-    const uint64_t desc = (uint64_t)((smem >> 4) & 0x3FFF) | (1ull << 16) | (8ull << 32) | (1ull << 46);
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc));
-}
-
-template <int KIND>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
-    if (KIND == 8) return smem_desc(addr);  // 128-byte rows, SWIZZLE_128B
-    // 64-byte rows, SWIZZLE_64B, 8-row atoms 512 bytes apart
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (32ull << 32) | (1ull << 46) | (4ull << 61);
-}
-
-template <int KIND>
-__device__ __forceinline__ uint32_t scaled_instr_desc(uint32_t n) {
-    const uint32_t types = KIND == 8 ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);  // e2m1 x e4m3 | e2m1 x e2m1
-    return types | (n >> 3) << 17 | 1u << 23 | 1u << 27;                                 // e8m0 scales, M = 128
-}
-
-template <int KIND>
-__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                           uint32_t acc) {
-    if (KIND == 8)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc));
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc));
-}
-
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr));
-}
-template <int N>
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));  // no use moves above the wait
-}
-
-// N tokens' values of this thread's weight row: the P columns of each, added in 32 bits, the
-// smallest piece first.
-template <int P, int N>
-__device__ __forceinline__ void load_tokens(uint32_t addr, float (&v)[N]) {
-    uint32_t r[N * P];
-#pragma unroll
-    for (int p = 0; p < N * P / 8; p++) tmem_ld8(addr + 8 * p, r + 8 * p);
-    tmem_wait(r);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        v[i] = __uint_as_float(r[i * P + P - 1]);
-#pragma unroll
-        for (int p = P - 2; p >= 0; p--) v[i] += __uint_as_float(r[i * P + p]);
-    }
-}
-
-__device__ __forceinline__ void put_as(void *y, int type, size_t at, float v) {
-    if (type == 0) static_cast<float *>(y)[at] = v;
-    else if (type == 1) static_cast<__half *>(y)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
-}
-
-// `count` tokens' values of one weight row (this thread's), rows of y `stride` apart: the 32 lanes of a
-// warp write 32 neighbouring values of a token.
-template <typename T, int N>
-__device__ __forceinline__ void put_tokens(T *p, uint64_t stride, const float (&v)[N], uint32_t count) {
-    if (count >= N) {
-#pragma unroll
-        for (int i = 0; i < N; i++, p += stride) *p = mx_to<T>(v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++, p += stride)
-            if ((uint32_t)i < count) *p = mx_to<T>(v[i]);
-    }
-}
-template <int N>
-__device__ __forceinline__ void put_tokens_as(void *y, int type, size_t at, uint64_t stride, const float (&v)[N], uint32_t count) {
-    if (type == 0) put_tokens(static_cast<float *>(y) + at, stride, v, count);
-    else if (type == 1) put_tokens(static_cast<__half *>(y) + at, stride, v, count);
-    else put_tokens(static_cast<__nv_bfloat16 *>(y) + at, stride, v, count);
-}
-
 template <int KIND, int P, int MODE>
 __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__ CUtensorMap wmap,
                                                          const __grid_constant__ CUtensorMap xmap, const TcArgs a) {
-    constexpr uint32_t kA = KIND == 8 ? 16384 : 8192;   // one weight tile in shared memory
-    constexpr uint32_t kMats = MODE == kGateUp ? 2 : 1;  // weight tiles per step of K: gate and up
+    constexpr uint32_t kSub = KIND == 8 ? 1 : 2;                  // scale tiles of a stage, per 128 rows
+    constexpr uint32_t kSf = kSub * kMxScaleTile;
+    constexpr uint32_t kWeightTx = (KIND == 8 ? kMxCodeTile / 2 : kMxCodeTile) + kSf;  // an unpacking copy counts what it reads
     extern __shared__ uint8_t raw[];
     uint8_t *base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     Ctrl &c = *reinterpret_cast<Ctrl *>(base);
-    // experts: tokens of each, the chosen expert of every pair, the columns' scales
+    // experts: tokens of each, the chosen expert of every pair, the columns' scales, gate and up values
     uint32_t *counts = reinterpret_cast<uint32_t *>(base + kCtrlBytes);
     uint8_t *ids = base + kCtrlBytes + 1024;
-    uint8_t *sfb_all = ids + (MODE == kDense ? 0 : up_to(a.m * a.top_k, kMxScaleTile));
+    uint8_t *sfb_all = ids + (MODE == kGateUp ? up_to(a.m * a.top_k, kMxScaleTile) : 0);
     uint8_t *ring = base + kCtrlBytes + (MODE == kDense ? 0 : a.head_bytes);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = blockIdx.z;
@@ -235,23 +108,45 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     }
 
     // ---- what this CTA computes ----
-    const uint32_t tile0 = blockIdx.x * a.per_cta, tiles = min(a.per_cta, a.row_tiles - tile0);  // 128 rows each
+    const uint32_t tile0 = blockIdx.x * a.per_cta, tiles = min(a.per_cta, a.row_tiles - tile0);
     uint32_t w_tile = tile0;
     uint32_t tokens, tok0 = 0, expert = 0, chunk = 0;  // columns: tokens, or a chunk of one expert's pairs
-    const uint32_t kt0 = a.kt * rank / a.split, kt1 = a.kt * (rank + 1) / a.split;
-    if (MODE == kDense) {
+    uint32_t mine = 0;                                 // lanes (pairs) of the expert, where one warp holds all pairs
+    const uint32_t k0 = a.steps * rank / a.split, k1 = a.steps * (rank + 1) / a.split;
+    const uint32_t pairs = MODE == kDense ? 0 : a.m * a.top_k;
+    const bool one_warp = MODE == kGateUp && pairs <= 32 && a.m <= a.chunk;
+    if constexpr (MODE == kDense) {
         tok0 = blockIdx.y * a.nt;
         tokens = min(a.nt, a.m - tok0);
     } else {
-        // Work items: every chosen expert's tokens in chunks, experts in order. The gate / up product
-        // finds its item from the choices themselves, in shared memory, and leaves the list to the
-        // down product.
+        // Work items: every chosen expert's tokens in chunks. The gate / up product finds its item from the
+        // choices themselves and leaves the list to the down product.
         const uint32_t item = blockIdx.y;
-        if (MODE == kGateUp) {
-            const uint32_t pairs = a.m * a.top_k;
+        if constexpr (MODE == kDown) {
+            grid_dep_wait();  // the items and the hidden vectors
+            const uint32_t *it = a.items + kItemWords * (1 + item);
+            const uint32_t total = __ldcg(a.items), of = __ldcg(it), pair = __ldcg(it + 2 + lane);
+            tokens = __ldcg(it + 1);
+            if (item >= total) return;
+            expert = of;
+            if (warp == 2) c.pairs[lane] = pair;
+        } else if (one_warp) {
+            // few pairs: a lane each in every warp, experts in the order of their first choice
+            grid_dep_wait();  // the router's choice
+            const uint32_t id = (uint32_t)lane < pairs ? (uint32_t)__ldcg(a.chosen + lane) : 0xFFFFu;
+            const uint32_t same = __match_any_sync(~0u, id);
+            const uint32_t firsts = __ballot_sync(~0u, (uint32_t)lane < pairs && __ffs(same) - 1 == lane);
+            if (item == 0 && blockIdx.x == 0 && rank == 0 && threadIdx.x == 0) a.items[0] = __popc(firsts);
+            if (item >= __popc(firsts)) return;  // the same in the whole cluster
+            const int first = (int)__fns(firsts, 0, (int)item + 1);
+            expert = __shfl_sync(~0u, id, first);
+            mine = __shfl_sync(~0u, same, first);
+            tokens = __popc(mine);
+        } else {
+            // experts in order, counted in shared memory
             for (uint32_t i = threadIdx.x; i < 256; i += kThreads) counts[i] = 0;
             __syncthreads();
-            grid_dep_wait();  // the router's choice
+            grid_dep_wait();
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < pairs; i += kThreads) {
                 const uint32_t e = (uint32_t)__ldcg(a.chosen + i);
@@ -273,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
             if (item == 0 && blockIdx.x == 0 && rank == 0 && threadIdx.x == 31) a.items[0] = upto;
             const uint32_t holders = __ballot_sync(~0u, item < upto);
-            if (!holders) return;  // the same in the whole cluster
+            if (!holders) return;
             uint32_t left = item - (upto - items), found = 0, here = 0;
             bool open = true;
 #pragma unroll
@@ -290,23 +185,15 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             expert = __shfl_sync(~0u, found, holder);
             chunk = __shfl_sync(~0u, left, holder);
             tokens = min(__shfl_sync(~0u, here, holder) - chunk * a.chunk, a.chunk);
-        } else {
-            grid_dep_wait();  // the items and the hidden vectors
-            const uint32_t *it = a.items + kItemWords * (1 + item);
-            const uint32_t total = __ldcg(a.items), of = __ldcg(it), pair = __ldcg(it + 2 + lane);
-            tokens = __ldcg(it + 1);
-            if (item >= total) return;
-            expert = of;
-            if (warp == 2) c.pairs[lane] = pair;
         }
-        w_tile = (expert * a.row_tiles + tile0) * kMats;
+        w_tile = expert * a.row_tiles + tile0;
     }
     const uint32_t n_cols = (tokens * P + 7) / 8 * 8;
-    const uint32_t sfb_tiles = MODE == kDense ? (n_cols + 127) / 128 : 1;
-    const uint32_t sf_cols = 4 + (a.nt * P > 128 ? 8 : 4);
+    const uint32_t col_tiles = MODE == kDense ? (n_cols + 127) / 128 : 1;
+    const uint32_t sfb_cols = a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
     // the experts' ring is as deep as this expert's few tokens allow
     const uint32_t b_bytes = MODE == kDense ? a.b_bytes : n_cols * 128;
-    const uint32_t stage_bytes = MODE == kDense ? a.stage_bytes : kA + 1024 + b_bytes;
+    const uint32_t stage_bytes = MODE == kDense ? a.stage_bytes : kA + b_bytes + 1024;
     const uint32_t stages = MODE == kDense ? a.stages : min(a.stages, a.ring_bytes / stage_bytes);
 
     if (warp == 1) {
@@ -318,8 +205,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     __syncthreads();
     tc_fence_after();
     if (MODE == kGateUp) grid_dep_launch();  // every CTA holds its TMEM: the next kernel's may come
-    const uint32_t tmem = c.tmem;
-    const uint32_t steps = kt1 - kt0;   // of K; gate and up tiles of a step follow each other
+    const uint32_t tmem = c.tmem, steps = k1 - k0;
 
     // a column's row of pieces; columns past the last token repeat it
     auto row_of = [&](uint32_t i) {
@@ -334,28 +220,27 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     };
 
     if (warp == 0 && elect_one()) {
+        // ---- weight tiles and their scales, in the order of memory ----
         // KIND 8's kernel before makes pieces and has seen all earlier work done; before KIND 4's may be any kernel,
         // one that writes the weights too
         if (MODE == kDense && KIND == 4) grid_dep_wait();
-        // ---- weight tiles and their scales: the order of the tiles in memory, but gate and up in turn ----
-        // (a copy that unpacks counts the bytes that it read, 64 a row, for either kind)
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;   // phase 1: not yet used
         for (uint32_t tile = 0; tile < tiles; tile++) {
-            const size_t first = (size_t)(w_tile + tile * kMats) * a.kt + kt0;
-            int y = (int)(first * 128);
-            const uint8_t *sf = a.w_scales + first * kMxScaleTile;
-            for (uint32_t step = 0; step < steps; step++, y += 128, sf += kMxScaleTile) {
-#pragma unroll
-                for (uint32_t i = 0; i < kMats; i++) {
-                    if (!mbar_poll(empty, phase, abort, 601)) goto weights_out;
-                    mbar_expect(full, kMxCodeTile + kMxScaleTile);
-                    tma_2d(st, &wmap, 0, y + (int)(i * a.kt * 128), full);
-                    bulk_copy(st + kA + b_bytes, sf + i * a.kt * kMxScaleTile, kMxScaleTile, full);
-                    issued++;
-                    st += stage_bytes, full += 8, empty += 8;
-                    if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
-                }
+            const uint32_t wt = w_tile + tile;
+            int x = KIND == 8 ? (int)(k0 % 2 * 128) : 0;   // KIND 8: a half of a code tile
+            int y = (int)((wt * a.kw + (KIND == 8 ? k0 / 2 : k0)) * 128);
+            const uint8_t *sf = a.w_scales + ((size_t)wt * 2 * a.kw + kSub * k0) * kMxScaleTile;
+            for (uint32_t step = 0; step < steps; step++, sf += kSf) {
+                if (!mbar_poll(empty, phase, abort, 601)) goto weights_out;
+                mbar_expect(full, kWeightTx);
+                tma_2d(st, &wmap, x, y, full);
+                bulk_copy(st + kA + b_bytes, sf, kSf, full);
+                if (KIND == 8) x ^= 128;
+                if (x == 0) y += 128;
+                issued++;
+                st += stage_bytes, full += 8, empty += 8;
+                if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
             }
         }
     weights_out:
@@ -370,25 +255,24 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             if (MODE == kDense) grid_dep_wait();  // the pieces, or codes
             const uint32_t st0 = smem_u32(ring) + kA, full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
             uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;
-            const uint32_t tx = MODE == kDense ? (KIND == 8 ? a.b_box_bytes : sfb_tiles * a.b_box_bytes) + sfb_tiles * kMxScaleTile
-                                               : n_cols * 128;
-            const uint32_t row = MODE == kDense && KIND == 8 ? tok0 / a.group * 256 + tok0 % a.group * P : tok0;
             if (MODE == kDense) {
-                const bool two = sfb_tiles > 1;
-                const uint32_t next_x = a.kt * 128, next_sf = a.kt * kMxScaleTile;   // the second tile of 128 columns
-                const uint8_t *sf = a.x_scales + ((size_t)(row / 128) * a.kt + kt0) * kMxScaleTile;
-                int x = KIND == 8 ? (int)(kt0 * 128) : (int)((row / 128 * a.kt + kt0) * 128);
-                for (uint32_t step = 0; step < steps; step++, x += 128, sf += kMxScaleTile) {
+                const bool two = col_tiles > 1;   // 128 columns and more: a second tile of scales, and of KIND 4 codes
+                const uint32_t tx = (KIND == 8 ? a.b_box_bytes : col_tiles * a.b_box_bytes) + col_tiles * kSf;
+                const uint32_t row = KIND == 8 ? tok0 / a.group * 256 + tok0 % a.group * P : tok0;
+                const uint32_t row_sf = (KIND == 8 ? a.steps : 2 * a.kw) * kMxScaleTile;   // scales of 128 rows
+                const uint8_t *sf = a.x_scales + (size_t)(row / 128) * row_sf + k0 * kSf;
+                int x = KIND == 8 ? (int)(k0 * 128) : (int)((row / 128 * a.kw + k0) * 128);
+                for (uint32_t step = 0; step < steps; step++, x += 128, sf += kSf) {
                     if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
                     mbar_expect(full, tx);
                     if (KIND == 8) {
                         tma_2d(st, &xmap, x, (int)row, full);
                     } else {
                         tma_2d(st, &xmap, 0, x, full);
-                        if (two) tma_2d(st + a.b_box_bytes, &xmap, 0, x + (int)next_x, full);
+                        if (two) tma_2d(st + a.b_box_bytes, &xmap, 0, x + (int)(a.kw * 128), full);
                     }
-                    bulk_copy(st + b_bytes + kMxScaleTile, sf, kMxScaleTile, full);
-                    if (two) bulk_copy(st + b_bytes + 2 * kMxScaleTile, sf + next_sf, kMxScaleTile, full);
+                    bulk_copy(st + b_bytes + kSf, sf, kSf, full);
+                    if (two) bulk_copy(st + b_bytes + 2 * kSf, sf + row_sf, kSf, full);
                     issued++;
                     st += stage_bytes, full += 8, empty += 8;
                     if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
@@ -397,23 +281,20 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 const int4 *rows = reinterpret_cast<const int4 *>(c.rows);
                 const int4 r0 = rows[0], r1 = rows[1], r2 = rows[2], r3 = rows[3];   // most experts' columns
                 for (uint32_t tile = 0; tile < tiles; tile++) {
-                    int x = (int)(kt0 * 128);
+                    int x = (int)(k0 * 128);
                     for (uint32_t step = 0; step < steps; step++, x += 128) {
-    #pragma unroll
-                        for (uint32_t mat = 0; mat < kMats; mat++) {
-                            if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
-                            mbar_expect(full, tx);
-                            tma_gather4(st, &xmap, x, r0, full);
-                            tma_gather4(st + 512, &xmap, x, r1, full);
-                            if (n_cols > 8) {
-                                tma_gather4(st + 1024, &xmap, x, r2, full);
-                                tma_gather4(st + 1536, &xmap, x, r3, full);
-                            }
-                            for (uint32_t i = 16; i < n_cols; i += 4) tma_gather4(st + i * 128, &xmap, x, rows[i / 4], full);
-                            issued++;
-                            st += stage_bytes, full += 8, empty += 8;
-                            if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
+                        if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
+                        mbar_expect(full, n_cols * 128);
+                        tma_gather4(st, &xmap, x, r0, full);
+                        tma_gather4(st + 512, &xmap, x, r1, full);
+                        if (n_cols > 8) {
+                            tma_gather4(st + 1024, &xmap, x, r2, full);
+                            tma_gather4(st + 1536, &xmap, x, r3, full);
                         }
+                        for (uint32_t i = 16; i < n_cols; i += 4) tma_gather4(st + i * 128, &xmap, x, rows[i / 4], full);
+                        issued++;
+                        st += stage_bytes, full += 8, empty += 8;
+                        if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
                     }
                 }
             }
@@ -423,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     } else if (warp == 1 && elect_one()) {
         // ---- MMA ----
         const uint32_t accs = tiles > 1 ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
-        const uint32_t sf_tmem = tmem + a.d_cols * kMats * accs, idesc = scaled_instr_desc<KIND>(n_cols);
+        const uint32_t sf_tmem = tmem + a.d_cols * accs, idesc = scaled_instr_desc<KIND>(128, n_cols);
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         // each stage has scale columns of its own: they are rewritten only after its MMAs are done
         uint32_t st = st0, full = full0, empty = empty0, sfa = sf_tmem, s = 0, phase = 0;
@@ -433,29 +314,32 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 ok = false;
                 break;
             }
-            const uint32_t d0 = tmem + (tile & 1) * kMats * a.d_cols;
+            const uint32_t d = tmem + (tile & 1) * a.d_cols;
             uint32_t sfb_smem = smem_u32(sfb_all);
-            for (uint32_t it = 0; it < steps * kMats; it++) {
+            for (uint32_t step = 0; step < steps; step++) {
                 if (!mbar_poll(full, phase, abort, 602)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t b = st + kA, sf = b + b_bytes, sfb = sfa + 4;
-                scales_to_tmem(sfa, sf);
-                if (MODE == kDense) {
-                    scales_to_tmem(sfb, sf + kMxScaleTile);
-                    if (sfb_tiles > 1) scales_to_tmem(sfb + 4, sf + 2 * kMxScaleTile);
-                } else {
-                    scales_to_tmem(sfb, sfb_smem);
-                    if (kMats == 1 || it % 2) sfb_smem += kMxScaleTile;
-                }
-                const uint64_t ad = operand_desc<KIND>(st), bd = operand_desc<KIND>(b);
-                const uint32_t d = d0 + (kMats == 2 ? it % 2 * a.d_cols : 0);
+                const uint32_t b = st + kA, sf = b + b_bytes, sfb = sfa + 4 * kSub;
 #pragma unroll
-                for (uint32_t j = 0; j < (KIND == 8 ? 4 : 2); j++) {   // 32 bytes of each row at a time
-                    const uint32_t id = KIND == 8 ? j : 2 * j;         // which of the four scale bytes
-                    mma_scaled<KIND>(d, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa, sfb, it >= kMats || j);
+                for (uint32_t h = 0; h < kSub; h++) {
+                    scales_to_tmem(sfa + 4 * h, sf + h * kMxScaleTile);
+                    if (MODE == kDense) {
+                        scales_to_tmem(sfb + sfb_cols * h, sf + kSf + h * kMxScaleTile);
+                        if (col_tiles > 1) scales_to_tmem(sfb + sfb_cols * h + 4, sf + 2 * kSf + h * kMxScaleTile);
+                    } else {
+                        scales_to_tmem(sfb, sfb_smem);
+                    }
+                }
+                sfb_smem += kMxScaleTile;
+                const uint64_t ad = smem_desc(st), bd = smem_desc(b);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {   // 32 bytes of each row at a time
+                    const uint32_t h = KIND == 8 ? 0 : j / 2, id = KIND == 8 ? j : j % 2 * 2;   // which scale bytes
+                    mma_scaled<KIND>(d, ad + 2 * j, bd + 2 * j, idesc | id << 4 | id << 29, sfa + 4 * h, sfb + sfb_cols * h,
+                                     step | j);
                 }
                 mma_commit(empty);
                 st += stage_bytes, full += 8, empty += 8, sfa += sf_cols;
@@ -474,9 +358,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     if (MODE != kDense && epi) {
         // ---- the item's tokens, and all their scales of this CTA's share of K ----
         const uint32_t at = threadIdx.x - 64;
-        if (MODE == kGateUp) {   // its pairs, in order: every warp looks through a quarter of them
-            const uint32_t pairs = a.m * a.top_k, quarter = up_to(pairs, 128) / 4, w = warp - 2;
-            const uint32_t from = w * quarter, to = min(from + quarter, pairs);
+        if (MODE == kGateUp && one_warp) {
+            if (warp == 2 && (mine >> lane & 1)) c.pairs[__popc(mine & ((1u << lane) - 1))] = lane;
+        } else if (MODE == kGateUp) {   // its pairs, in order: every warp looks through a quarter of them
+            const uint32_t quarter = up_to(pairs, 128) / 4, w = warp - 2, from = w * quarter, to = min(from + quarter, pairs);
             uint32_t seen = 0;
             for (uint32_t i = from; i < to; i += 32) seen += __popc(__ballot_sync(~0u, i + lane < to && ids[i + lane] == expert));
             if (lane == 0) c.found[w] = seen;
@@ -496,7 +381,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         for (uint32_t j = at; j < n_cols * steps; j += 128) {
             const uint32_t i = j / steps, t = j - i * steps;
             *reinterpret_cast<uint32_t *>(sfb_all + t * kMxScaleTile + i % 32 * 16 + i / 32 * 4) =
-                __ldcg(reinterpret_cast<const uint32_t *>(a.x_scales) + (size_t)row_of(i) * a.kt + kt0 + t);
+                __ldcg(reinterpret_cast<const uint32_t *>(a.x_scales) + (size_t)row_of(i) * a.steps + k0 + t);
         }
         fence_proxy_async();  // read by the tensor core's scale copy
         mbar_arrive(smem_u32(&c.scales_ready));
@@ -510,34 +395,40 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     // ---- epilogue: thread = weight row ----
     const uint32_t q = warp % 4;
     uint32_t tile = tile0, row = tile0 * 128 + q * 32 + lane;   // of the tile being read
-    float *red = reinterpret_cast<float *>(ring);   // [token][128] per matrix, once the ring is idle
+    // [token][128]: a cluster's partial sums, and the gate and up values, which lie in different warps' rows
+    float *red = reinterpret_cast<float *>(MODE == kGateUp ? sfb_all + steps * kMxScaleTile : ring);
 
-    auto finish = [&](uint32_t i, float g, float u) {
-        if (MODE == kDense) {
-            if (row < a.n) put_as(a.y, a.type, (tok0 + i) * a.stride + row, g);
-        } else if (MODE == kGateUp) {
-            // The hidden value and its pieces. A warp's 32 rows are one block along the next
-            // product's K. Three pieces keep 12 bits of it: past what x and y hold in either type.
-            const float h = g / (1.0f + expf(-g)) * u;
-            const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(h) & 0x7FFFFFFFu);
-            const uint32_t s = mx_piece_scale(__uint_as_float(top), kMxHiddenPieces);
-            float left = h * __uint_as_float((254u - min(s, 253u)) << 23);
-            const size_t r = (size_t)c.pairs[i] * kMxHiddenPieces, kt = a.row_tiles;
+    // The hidden value of one of the tile's 64 and its pieces. A warp's 32 are one block along the next
+    // product's K. Three pieces keep 12 bits of it: past what x and y hold in either type.
+    auto hidden = [&](uint32_t i, float g, float u) {
+        const float h = g / (1.0f + expf(-g)) * u;
+        const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(h) & 0x7FFFFFFFu);
+        const uint32_t s = mx_piece_scale(__uint_as_float(top), kMxHiddenPieces);
+        float left = h * __uint_as_float((254u - min(s, 253u)) << 23);
+        const uint32_t at = tile * kMxHalf + q % 2 * 32 + lane;
+        const bool pad = tile + 1 == a.row_tiles && a.row_tiles % 2;   // the next product's tiles are 128 wide
+        const size_t r = (size_t)c.pairs[i] * kMxHiddenPieces;
 #pragma unroll
-            for (int p = 0; p < kMxHiddenPieces; p++) {
-                float back;
-                const uint32_t code = mx_e4m3(left, &back);
-                left = (left - back) * 16.0f;
-                a.h_pieces[(r + p) * kt * 128 + row] = s == 255 ? 0 : (uint8_t)code;
-                if (lane == 0) a.h_scales[(r + p) * kt * 4 + row / 32] = (uint8_t)mx_piece_scale_of(s, p);
+        for (int p = 0; p < kMxHiddenPieces; p++) {
+            float back;
+            const uint32_t code = mx_e4m3(left, &back);
+            left = (left - back) * 16.0f;
+            uint8_t *to = a.h_pieces + (r + p) * a.h_steps * 128 + at;
+            uint8_t *sf = a.h_scales + (r + p) * a.h_steps * 4 + at / 32;
+            *to = s == 255 ? 0 : (uint8_t)code;
+            if (lane == 0) *sf = (uint8_t)mx_piece_scale_of(s, p);
+            if (pad) {
+                to[kMxHalf] = 0;
+                if (lane == 0) sf[kMxHalf / 32] = 0;
             }
-        } else {
-            if (row < a.n) a.partial[(size_t)c.pairs[i] * a.n + row] = g * __ldcg(a.weight + c.pairs[i]);
         }
     };
-    // Down products lie weighted in their pairs' places. The warp that brings a token's last pair of
+    // Down products go, weighted, to their pairs' own places. The warp that brings a token's last pair of
     // these 32 rows adds the token's top_k parts in their order, so the sum does not depend on
     // who that is. Lane i counts token i in: one fence and one round of atomics for all of them.
+    auto part = [&](uint32_t i, float v) {
+        if (row < a.n) a.partial[(size_t)c.pairs[i] * a.n + row] = v * __ldcg(a.weight + c.pairs[i]);
+    };
     auto combine = [&](uint32_t first, uint32_t step) {
         __threadfence();
         __syncwarp();
@@ -550,10 +441,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             const uint32_t to = __shfl_sync(~0u, t, __ffs(mask) - 1);
             mask &= mask - 1;
             if (row < a.n) {
-                const float *part = a.partial + (size_t)to * a.top_k * a.n + row;
+                const float *parts = a.partial + (size_t)to * a.top_k * a.n + row;
                 float sum = 0.0f;
 #pragma unroll 8
-                for (uint32_t j = 0; j < a.top_k; j++) sum += __ldcg(part + (size_t)j * a.n);
+                for (uint32_t j = 0; j < a.top_k; j++) sum += __ldcg(parts + (size_t)j * a.n);
                 put_as(a.y, a.type, to * a.stride + row, sum);
             }
         }
@@ -564,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         row = tile * 128 + q * 32 + lane;
         mbar_wait(smem_u32(&c.acc_full[nth & 1]), nth / 2 & 1, abort, 604);
         tc_fence_after();
-        const uint32_t taddr = tmem + (q * 32 << 16) + (nth & 1) * kMats * a.d_cols;
+        const uint32_t taddr = tmem + (q * 32 << 16) + (nth & 1) * a.d_cols;
         if (MODE == kDense && a.split == 1) {
             constexpr uint32_t kAt = P == 1 ? 32 : P == 2 ? 16 : 8;   // tokens at a time: up to 32 columns
             uint32_t i0 = 0;
@@ -579,19 +470,15 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 if (row < a.n) put_tokens_as(a.y, a.type, (tok0 + i0) * a.stride + row, a.stride, v, tokens - i0);
             }
         } else {
+            if (MODE == kGateUp && nth) asm volatile("bar.sync 1, 128;" ::: "memory");   // the last tile's values are read
             for (uint32_t i0 = 0; i0 < tokens; i0 += 8) {
-                float g[8], u[8];
-                load_tokens<P>(taddr + i0 * P, g);
-                if (MODE == kGateUp) load_tokens<P>(taddr + a.d_cols + i0 * P, u);
+                float v[8];
+                load_tokens<P>(taddr + i0 * P, v);
 #pragma unroll
                 for (uint32_t i = 0; i < 8; i++) {
                     if (i0 + i >= tokens) break;
-                    if (MODE != kDense && a.split == 1) {
-                        finish(i0 + i, g[i], MODE == kGateUp ? u[i] : 0.0f);
-                    } else {
-                        red[(i0 + i) * 128 + q * 32 + lane] = g[i];
-                        if (MODE == kGateUp) red[(a.nt + i0 + i) * 128 + q * 32 + lane] = u[i];
-                    }
+                    if (MODE == kDown && a.split == 1) part(i0 + i, v[i]);
+                    else red[(i0 + i) * 128 + q * 32 + lane] = v[i];
                 }
             }
         }
@@ -599,24 +486,33 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&c.acc_empty[nth & 1]));
         if (MODE == kDown && a.split == 1) combine(0, 1);
+        if (MODE == kGateUp && a.split == 1) {
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (uint32_t i = q / 2; i < tokens; i += 2) {   // a warp: half of the tokens, half of the tile's 64 values
+                const float *v = red + i * 128 + q % 2 * 32 + lane;
+                hidden(i, v[0], v[kMxHalf]);
+            }
+        }
     }
     if (a.split > 1) {
         // the cluster's partial tiles, added in rank order through distributed shared memory
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
-        if (epi)
-            for (uint32_t i0 = rank; i0 < tokens; i0 += 4 * a.split) {
+        if (epi) {
+            const uint32_t first = MODE == kGateUp ? rank * 2 + q / 2 : rank, every = MODE == kGateUp ? 2 * a.split : a.split;
+            const uint32_t at = MODE == kGateUp ? q % 2 * 32 + lane : q * 32 + lane;
+            for (uint32_t i0 = first; i0 < tokens; i0 += 4 * every) {
                 float g[4] = {}, u[4] = {};   // four tokens' loads go out before the first sum
 #pragma unroll
                 for (uint32_t r = 0; r < 8; r++) {
                     if (r >= a.split) break;
-                    const float *other = cluster.map_shared_rank(red, r) + q * 32 + lane;
+                    const float *other = cluster.map_shared_rank(red, r) + at;
                     float v[4], w[4];
 #pragma unroll
                     for (uint32_t j = 0; j < 4; j++) {
-                        const uint32_t i = min(i0 + j * a.split, tokens - 1);
+                        const uint32_t i = min(i0 + j * every, tokens - 1);
                         v[j] = other[i * 128];
-                        if (MODE == kGateUp) w[j] = other[(a.nt + i) * 128];
+                        if (MODE == kGateUp) w[j] = other[i * 128 + kMxHalf];
                     }
 #pragma unroll
                     for (uint32_t j = 0; j < 4; j++) {
@@ -625,9 +521,15 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                     }
                 }
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++)
-                    if (i0 + j * a.split < tokens) finish(i0 + j * a.split, g[j], u[j]);
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t i = i0 + j * every;
+                    if (i >= tokens) break;
+                    if (MODE == kGateUp) hidden(i, g[j], u[j]);
+                    else if (MODE == kDown) part(i, g[j]);
+                    else if (row < a.n) put_as(a.y, a.type, (tok0 + i) * a.stride + row, g[j]);
+                }
             }
+        }
         __syncwarp();
         cluster.barrier_arrive();   // this CTA reads the others' shared memory no more
         if (MODE == kDown && epi) combine(rank, a.split);
@@ -701,12 +603,12 @@ cudaError_t encode(CUtensorMap *map, CUtensorMapDataType type, const void *ptr, 
     return cudaSuccess;
 }
 
-// Weight tiles: 64 bytes of codes a row, tiles of 128 rows one after another.
+// Weight tiles: 128 bytes of codes a row, tiles of 128 rows one after another. KIND 8 unpacks half a row at a time.
 template <int KIND>
 cudaError_t encode_weights(CUtensorMap *map, const uint8_t *codes, uint64_t tiles) {
     if (KIND == 8)
-        return encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, codes, 128, tiles * 128, 64, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 64, tiles * 128, 64, 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, codes, 256, tiles * 128, 128, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 128, tiles * 128, 128, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 uint32_t pow2_cols(uint32_t v) {
@@ -719,7 +621,7 @@ uint32_t pow2_cols(uint32_t v) {
 
 template <int KIND, int P, int MODE>
 cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, cudaStream_t s) {
-    if (!a.stages || a.tmem_cols > 512) return cudaErrorInvalidConfiguration;
+    if (!a.stages || a.tmem_cols > 512 || smem > 227 * 1024) return cudaErrorInvalidConfiguration;
     auto kernel = mx_tc_kernel<KIND, P, MODE>;
     if (!once_per_device(100 + KIND * 16 + P * 4 + MODE, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess;
@@ -745,49 +647,47 @@ cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArg
 // Ring depth and shared memory for `per_sm` CTAs on an SM.
 template <int KIND, int P, int MODE>
 uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
-    const uint32_t mats = MODE == kGateUp ? 2 : 1, n = up_to(a.nt * P, 8);
-    // KIND 4 copies whole boxes of 128 rows past the first 128 columns
-    a.b_bytes = KIND == 8 ? n * 128 : n <= 128 ? up_to(n * 64, 1024) : up_to(n, 128) * 64;
-    const uint32_t sf = kMxScaleTile * (1 + (MODE == kDense ? (n + 127) / 128 : 0));
-    a.stage_bytes = (KIND == 8 ? 16384 : 8192) + a.b_bytes + up_to(sf, 1024);
+    const uint32_t n = up_to(a.nt * P, 8), sub = KIND == 8 ? 1 : 2;
+    a.b_box_bytes = (KIND == 8 || n < 128 ? n : 128) * 128;       // KIND 4 copies whole tiles of 128 columns
+    a.b_bytes = KIND == 8 ? n * 128 : (n + 127) / 128 * a.b_box_bytes;
+    a.stage_bytes = kA + a.b_bytes + up_to(kMxScaleTile * sub * (1 + (MODE == kDense ? (n + 127) / 128 : 0)), 1024);
     a.d_cols = up_to(a.nt, 8) * P;
-    const uint32_t sf_cols = 4 + (a.nt * P > 128 ? 8 : 4);
+    const uint32_t sf_cols = sub * (4 + (a.nt * P > 128 ? 8 : 4));
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
     const uint32_t budget = (per_sm == 1 ? 226 : per_sm == 2 ? 112 : 74) * 1024 - extra;
     const uint32_t cols = per_sm == 1 ? 512 : per_sm == 2 ? 256 : 128;
-    const uint32_t iters = (a.kt + a.split - 1) / a.split * mats * a.per_cta;
-    const uint32_t acc_cols = a.d_cols * mats * (a.per_cta > 1 ? 2 : 1);
-    a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, iters});
+    const uint32_t acc_cols = a.d_cols * (a.per_cta > 1 ? 2 : 1);
+    a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, (a.steps + a.split - 1) / a.split * a.per_cta});
     if (MODE == kDense) {
         a.stages = std::min(a.stages, budget / a.stage_bytes);
         a.ring_bytes = a.stages * a.stage_bytes;
     } else {   // the kernel fits its stages into this by its expert's number of tokens
-        const uint32_t least = (KIND == 8 ? 16384 : 8192) + 2048;
         a.ring_bytes = std::max(std::min(budget, a.stages * a.stage_bytes), a.stage_bytes);
-        a.stages = std::min(a.stages, a.ring_bytes / least);
+        a.stages = std::min(a.stages, a.ring_bytes / (kA + 2048));
     }
     a.tmem_cols = pow2_cols(acc_cols + a.stages * sf_cols);
-    const uint32_t red = a.split > 1 ? mats * a.nt * 128 * 4 : 0;
+    const uint32_t red = MODE != kGateUp && a.split > 1 ? a.nt * 128 * 4 : 0;
     return extra + std::max(a.ring_bytes, red);
 }
 
 template <int KIND, int P>
 cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_scales, cudaStream_t s) {
-    const uint32_t kt = mx_tiles(p.k), rt = mx_tiles(p.n);
+    const uint32_t rt = mx_tiles(p.n), kw = mx_ktiles(p.k) / 2;
     constexpr uint32_t kGroup = P == 1 ? 256 : P == 2 ? 128 : 64;   // tokens that fill 256 columns (P = 3: 192)
     if (p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 37) return pair_product<KIND, P>(p, x, x_scales, s);
     TcArgs a{};
     a.m = p.m;
     a.n = p.n;
-    a.kt = kt;
+    a.kw = kw;
+    a.steps = KIND == 8 ? mx_tiles(p.k) : kw;
     a.group = kGroup;
     a.row_tiles = rt;
     a.per_cta = 1;
     a.nt = p.m < kGroup ? p.m : kGroup;
     const uint32_t tt = (p.m + a.nt - 1) / a.nt;
     a.split = 1;
-    while (a.split < 8 && rt * tt * a.split * 2 <= 148 && kt / (a.split * 2) >= 2 && a.nt <= 64) a.split *= 2;
-    if (a.split < 8 && rt * tt * a.split * 2 <= 2 * 148 && kt / a.split > 24 && a.nt <= 32) a.split *= 2;
+    while (a.split < 8 && rt * tt * a.split * 2 <= 148 && a.steps / (a.split * 2) >= 2 && a.nt <= 32) a.split *= 2;
+    if (a.split < 8 && rt * tt * a.split * 2 <= 2 * 148 && a.steps / a.split > 24 && a.nt <= 32) a.split *= 2;
     const uint32_t per_sm = rt * tt * a.split > 148 && up_to(a.nt, 8) * P <= 128 ? 2 : 1;
     a.w_scales = p.w_scales;
     a.x_scales = x_scales;
@@ -796,20 +696,14 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.stride = p.stride;
     const uint32_t smem = plan_ring<KIND, P, kDense>(a, per_sm);
     CUtensorMap wmap, xmap;
-    cudaError_t e = encode_weights<KIND>(&wmap, p.w_codes, (uint64_t)rt * kt);
+    cudaError_t e = encode_weights<KIND>(&wmap, p.w_codes, (uint64_t)rt * kw);
     if (e != cudaSuccess) return e;
-    const uint32_t n = up_to(a.nt * P, 8);
-    if (KIND == 8) {
-        const uint64_t rows = (uint64_t)(p.m / kGroup) * 256 + p.m % kGroup * P;
-        a.b_box_bytes = n * 128;
-        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)kt * 128, rows, (uint64_t)kt * 128, 128, n,
+    if (KIND == 8)
+        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)a.steps * 128, mx_piece_rows(p.m, p.x_type),
+                   (uint64_t)a.steps * 128, 128, a.b_box_bytes / 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    else
+        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 128, (uint64_t)mx_tiles(p.m) * kw * 128, 128, 128, a.b_box_bytes / 128,
                    CU_TENSOR_MAP_SWIZZLE_128B);
-    } else {
-        const uint32_t box = n < 128 ? n : 128;
-        a.b_box_bytes = box * 64;
-        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 64, (uint64_t)mx_tiles(p.m) * kt * 128, 64, 64, box,
-                   CU_TENSOR_MAP_SWIZZLE_64B);
-    }
     if (e != cudaSuccess) return e;
     return launch<KIND, P, kDense>(wmap, xmap, a, dim3(rt, tt, a.split), smem, s);
 }
@@ -832,12 +726,14 @@ cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
 
 template <int P, int MODE>
 cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
-    const uint32_t width = MODE == kGateUp ? e.d : e.f, rows = MODE == kGateUp ? e.f : e.d;
+    const uint32_t width = MODE == kGateUp ? e.d : e.f;
     TcArgs a{};
     a.m = e.tokens;
-    a.n = rows;
-    a.kt = mx_tiles(width);
-    a.row_tiles = mx_tiles(rows);
+    a.n = e.d;
+    a.steps = mx_tiles(width);
+    a.kw = mx_ktiles(width) / 2;
+    a.h_steps = mx_tiles(e.f);
+    a.row_tiles = MODE == kGateUp ? (e.f + kMxHalf - 1) / kMxHalf : mx_tiles(e.d);
     a.top_k = e.top_k;
     a.chosen = e.ws.chosen;
     a.weight = e.ws.weight;
@@ -851,32 +747,33 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.y = e.y;
     a.type = e.type;
     a.stride = e.y_stride;
-    // Tokens to a CTA: 16 where the experts get few, which leaves TMEM for a second accumulator.
+    // Tokens to a CTA: 16 where the experts get few, which leaves room for a second accumulator.
     const uint32_t pairs = e.tokens * e.top_k, slots = std::min(e.experts, pairs);
     a.chunk = pairs <= e.experts * 8 ? 16 : kChunk;
     a.nt = std::min(e.tokens, a.chunk);
     // as many items as there can be: one to each chosen expert, one more for every further chunk of pairs
     const uint32_t items = slots + (pairs - slots) / a.chunk;
     a.split = 1;
-    while (a.split < 8 && a.kt / (a.split * 2) >= 2 && (a.row_tiles * slots * a.split * 2 <= 148 || a.kt / a.split > 32))
+    while (a.split < 8 && a.steps / (a.split * 2) >= 2 && (a.row_tiles * slots * a.split * 2 <= 148 || a.steps / a.split > 32))
         a.split *= 2;
     // Row tiles to a CTA: its set-up (finding its tokens, their scales) costs as much as some 100 KB of
     // weights, so it takes more tiles once there are enough to go round.
-    const uint32_t mats0 = MODE == kGateUp ? 2 : 1, cols = up_to(a.nt, 8) * P * mats0;
+    const uint32_t cols = up_to(a.nt, 8) * P;
     a.per_cta = 1;
-    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < 4 && a.per_cta * a.kt * mats0 < 32 &&
+    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < 4 && a.per_cta * a.steps < 32 &&
            a.row_tiles * slots >= 148 * 2 * 2 * a.per_cta)
         a.per_cta *= 2;
-    a.head_bytes = up_to(1024 + up_to(pairs, kMxScaleTile) + (a.kt + a.split - 1) / a.split * kMxScaleTile, 1024);
+    a.head_bytes = 1024 + (a.steps + a.split - 1) / a.split * kMxScaleTile +
+                   (MODE == kGateUp ? up_to(pairs, kMxScaleTile) + a.nt * 512 : 0);
+    a.head_bytes = up_to(a.head_bytes, 1024);
     const uint32_t smem = plan_ring<8, P, MODE>(a, 2);
-    const uint32_t mats = MODE == kGateUp ? 2 : 1;
     CUtensorMap wmap, xmap;
     cudaError_t r = encode_weights<8>(&wmap, MODE == kGateUp ? e.gate_up_codes : e.down_codes,
-                                      (uint64_t)e.experts * a.row_tiles * mats * a.kt);
+                                      (uint64_t)e.experts * a.row_tiles * a.kw);
     if (r != cudaSuccess) return r;
-    const uint64_t piece_rows = MODE == kGateUp ? (uint64_t)e.tokens * P : (uint64_t)e.tokens * e.top_k * P;
-    r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.kt * 128,
-               piece_rows, (uint64_t)a.kt * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint64_t piece_rows = MODE == kGateUp ? (uint64_t)e.tokens * P : (uint64_t)pairs * P;
+    r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.steps * 128,
+               piece_rows, (uint64_t)a.steps * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
     return launch<8, P, MODE>(wmap, xmap, a, dim3((a.row_tiles + a.per_cta - 1) / a.per_cta, items, a.split), smem, s);
 }

@@ -114,8 +114,8 @@ def _extent(x):
 def _sizes(operand, rows, k):
     """Bytes of the codes and of the scales (ug_mx4_codes_bytes, ug_mx4_scales_bytes)."""
     if operand:
-        tiles = -(-rows // 128) * -(-k // 128)
-        return tiles * 8192, tiles * 512
+        tiles = -(-rows // 128) * -(-k // 256)
+        return tiles * 16384, tiles * 1024
     return rows * ((k + 1) // 2), rows * ((k + 31) // 32)
 
 
