@@ -178,96 +178,94 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint8_t *codes, const u
 
 // ---- router ------------------------------------------------------------------------------------
 //
-// A cluster of 8 CTAs takes TOKENS tokens: each CTA has every eighth expert, one warp to an expert's
-// products (32 lanes across d, fixed order, so logits do not depend on timing). A token's logits meet
-// in the shared memory of one of the CTAs, whose first warp selects. The same CTAs split the rows
-// into the pieces that the gate / up product reads. One token is a chain of latencies (4.5 us for 32
-// experts of 2048: 2 for the products, 0.7 for the cluster's barrier, 0.6 for the selection); with
-// many, four tokens share each router row read, which is all the L2 traffic (64 tokens, 128
-// experts: 6.4 us of products with one).
+// A cluster of 8 CTAs per token: each takes every eighth expert, one warp to an expert's product (32
+// lanes across d, fixed order, so logits do not depend on timing). The logits meet in the first CTA's
+// shared memory, whose first warp selects. The same CTAs split the token's row into the pieces that the
+// gate / up product reads. It is a chain of latencies: 4.4 us for one token and 32 experts of 2048, 2 of
+// them for the products, 0.7 for the cluster's barrier and 0.6 for the selection. Four tokens to a
+// cluster, sharing the router rows that they read, took longer at 64 tokens (13.6 us).
 
-template <typename T, int TOKENS>
+template <typename T>
 __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) router_kernel(MxExpertsArgs a, bool vec) {
     __shared__ float logits[256];
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t rank = blockIdx.x, t0 = blockIdx.y * TOKENS, tokens = min((uint32_t)TOKENS, a.tokens - t0);
-    auto started = cluster.barrier_arrive();  // the CTAs' shared memory exists for the others after the wait
+    const uint32_t rank = blockIdx.x, t = blockIdx.y;
+    auto started = cluster.barrier_arrive();  // the first CTA's shared memory exists for the others after the wait
     grid_dep_wait();
     grid_dep_launch();  // the products' set-up may begin; they wait for this kernel's results
     bool waited = false;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const T *x = static_cast<const T *>(a.x) + t0 * a.x_stride;
+    const T *x = static_cast<const T *>(a.x) + t * a.x_stride;
 
+    // A row's loads go out together before the first product: eight of 16 bytes, or sixteen single values
+    // where rows do not start on 16 bytes (1447 wide: 10.9 -> 6.1 us).
+    float *remote = cluster.map_shared_rank(logits, 0);
     for (uint32_t e = rank + kMxRouterCluster * warp; e < a.experts; e += kMxRouterCluster * 8) {
         const T *w = static_cast<const T *>(a.router) + (size_t)e * a.d;
-        float sum[TOKENS];
-#pragma unroll
-        for (int n = 0; n < TOKENS; n++) sum[n] = 0.0f;
+        float sum = 0.0f;
         if (vec) {
-#pragma unroll(TOKENS == 1 ? 8 : 2)
-            for (uint32_t i = lane * 8; i < a.d; i += 256) {
-                const uint4 p = __ldg(reinterpret_cast<const uint4 *>(w + i));
-                const T *ph = reinterpret_cast<const T *>(&p);
+            for (uint32_t i0 = lane * 8; i0 < a.d; i0 += 2048) {
+                uint4 p[8], q[8];
 #pragma unroll
-                for (int n = 0; n < TOKENS; n++) {
-                    // a token past the last repeats it
-                    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(x + min((uint32_t)n, tokens - 1) * a.x_stride + i));
-                    const T *qh = reinterpret_cast<const T *>(&q);
+                for (int c = 0; c < 8; c++) {
+                    const uint32_t i = i0 + c * 256;
+                    p[c] = i < a.d ? __ldg(reinterpret_cast<const uint4 *>(w + i)) : make_uint4(0, 0, 0, 0);
+                    q[c] = i < a.d ? __ldg(reinterpret_cast<const uint4 *>(x + i)) : make_uint4(0, 0, 0, 0);
+                }
 #pragma unroll
-                    for (int j = 0; j < 8; j++) sum[n] = fmaf(mx_float(ph[j]), mx_float(qh[j]), sum[n]);
+                for (int c = 0; c < 8; c++) {
+                    const T *ph = reinterpret_cast<const T *>(&p[c]), *qh = reinterpret_cast<const T *>(&q[c]);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) sum = fmaf(mx_float(ph[j]), mx_float(qh[j]), sum);
                 }
             }
         } else {
-#pragma unroll 4
-            for (uint32_t i = lane; i < a.d; i += 32) {
-                const float p = mx_float(w[i]);
+            for (uint32_t i0 = lane; i0 < a.d; i0 += 512) {
+                T p[16], q[16];
 #pragma unroll
-                for (int n = 0; n < TOKENS; n++)
-                    sum[n] = fmaf(p, mx_float(x[min((uint32_t)n, tokens - 1) * a.x_stride + i]), sum[n]);
+                for (int c = 0; c < 16; c++) {
+                    const uint32_t i = i0 + c * 32;
+                    p[c] = i < a.d ? w[i] : mx_to<T>(0.0f);
+                    q[c] = i < a.d ? x[i] : mx_to<T>(0.0f);
+                }
+#pragma unroll
+                for (int c = 0; c < 16; c++) sum = fmaf(mx_float(p[c]), mx_float(q[c]), sum);
             }
         }
 #pragma unroll
-        for (int n = 0; n < TOKENS; n++)
-#pragma unroll
-            for (int o = 16; o; o /= 2) sum[n] += __shfl_xor_sync(~0u, sum[n], o);
+        for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
         if (!waited) {
             cluster.barrier_wait(std::move(started));
             waited = true;
         }
-#pragma unroll
-        for (int n = 0; n < TOKENS; n++)
-            if (lane == n) cluster.map_shared_rank(logits, n)[e] = sum[n] + (a.bias ? a.bias[e] : 0.0f);
+        if (lane == 0) remote[e] = sum + (a.bias ? a.bias[e] : 0.0f);
     }
     if (!waited) cluster.barrier_wait(std::move(started));
 
-    // the rows' pieces: one warp to a block of 32 values
+    // the row's pieces: one warp to a block of 32 values
     const uint32_t kt = mx_tiles(a.d);
     const int pieces = mx_pieces(a.type);
-    for (uint32_t n = 0; n < tokens; n++) {
-        const T *row = x + n * a.x_stride;
-        for (uint32_t b = rank * 8 + warp; b < kt * 4; b += kMxRouterCluster * 8) {
-            const uint32_t i = b * 32 + lane;
-            const float v = i < a.d ? mx_float(row[i]) : 0.0f;
-            // infinity and NaN order above every number here
-            const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(v) & 0x7FFFFFFFu);
-            const uint32_t s = mx_piece_scale(__uint_as_float(top), pieces);
-            float left = v * __uint_as_float((254u - min(s, 253u)) << 23);
-            for (int p = 0; p < pieces; p++) {
-                float back;
-                const uint32_t code = mx_e4m3(left, &back);
-                left = (left - back) * 16.0f;
-                const size_t r = (size_t)(t0 + n) * pieces + p;
-                a.ws.x_pieces[r * kt * 128 + i] = s == 255 ? 0 : (uint8_t)code;
-                if (lane == 0) a.ws.x_scales[r * kt * 4 + b] = (uint8_t)mx_piece_scale_of(s, p);
-            }
+    for (uint32_t b = rank * 8 + warp; b < kt * 4; b += kMxRouterCluster * 8) {
+        const uint32_t i = b * 32 + lane;
+        const float v = i < a.d ? mx_float(x[i]) : 0.0f;
+        // infinity and NaN order above every number here
+        const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(v) & 0x7FFFFFFFu);
+        const uint32_t s = mx_piece_scale(__uint_as_float(top), pieces);
+        float left = v * __uint_as_float((254u - min(s, 253u)) << 23);
+        for (int p = 0; p < pieces; p++) {
+            float back;
+            const uint32_t code = mx_e4m3(left, &back);
+            left = (left - back) * 16.0f;
+            const size_t r = (size_t)t * pieces + p;
+            a.ws.x_pieces[r * kt * 128 + i] = s == 255 ? 0 : (uint8_t)code;
+            if (lane == 0) a.ws.x_scales[r * kt * 4 + b] = (uint8_t)mx_piece_scale_of(s, p);
         }
     }
-    const uint32_t t = t0 + rank;   // the token whose logits are here
-    if (rank < tokens)
+    if (rank == 0)
         for (uint32_t i = threadIdx.x; i < kt * 4; i += blockDim.x) a.ws.arrived[(size_t)t * kt * 4 + i] = 0;
 
     cluster.sync();
-    if (rank >= tokens || warp != 0) return;
+    if (rank != 0 || warp != 0) return;
     // selection: keys order as the logits do; a NaN is below every number, a taken expert is 0
     uint32_t key[8];
 #pragma unroll
@@ -394,11 +392,8 @@ cudaError_t launch_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_
 
 cudaError_t launch_mx4_router(const MxExpertsArgs &a, cudaStream_t s) {
     const bool vec = aligned(a.router, 16) && a.d % 8 == 0 && aligned(a.x, 16) && a.x_stride % 8 == 0;
-    const bool many = a.tokens > 16;   // 16 clusters of one token each have an SM to every CTA
-    const dim3 grid(kMxRouterCluster, many ? (a.tokens + 3) / 4 : a.tokens);
-    auto kernel = a.type == 1 ? (many ? router_kernel<__half, 4> : router_kernel<__half, 1>)
-                              : (many ? router_kernel<__nv_bfloat16, 4> : router_kernel<__nv_bfloat16, 1>);
-    return launch_pdl(kPdlMx, kernel, grid, 256, 0, s, a, vec);
+    return launch_pdl(kPdlMx, a.type == 1 ? router_kernel<__half> : router_kernel<__nv_bfloat16>,
+                      dim3(kMxRouterCluster, a.tokens), 256, 0, s, a, vec);
 }
 
 }  // namespace uq

@@ -753,9 +753,10 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.nt = std::min(e.tokens, a.chunk);
     // as many items as there can be: one to each chosen expert, one more for every further chunk of pairs
     const uint32_t items = slots + (pairs - slots) / a.chunk;
+    // K is split over a cluster only so that its scales fit: a cluster's launch and sums cost more than they
+    // save (one token, 4 of 32 experts: 18.1 us without, 18.4 to 19.5 with 2 or 4)
     a.split = 1;
-    while (a.split < 8 && a.steps / (a.split * 2) >= 2 && (a.row_tiles * slots * a.split * 2 <= 148 || a.steps / a.split > 32))
-        a.split *= 2;
+    while (a.split < 8 && a.steps / a.split > 32) a.split *= 2;
     // Row tiles to a CTA: its set-up (finding its tokens, their scales) costs as much as some 100 KB of
     // weights, so it takes more tiles once there are enough to go round.
     const uint32_t cols = up_to(a.nt, 8) * P;
