@@ -424,28 +424,34 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
     };
     // Down products go, weighted, to their pairs' own places. The warp that brings a token's last pair of
-    // these 32 rows adds the token's top_k parts in their order, so the sum does not depend on
-    // who that is. Lane i counts token i in: one fence and one round of atomics for all of them.
+    // 32 rows adds the token's top_k parts in their order, so the sum does not depend on who that is.
+    // This is done once for all tiles of the CTA: one fence, and a lane to each (tile, token)
+    // (a fence and a round of atomics after every tile took 4.4 us a tile, its MMAs 2.2).
     auto part = [&](uint32_t i, float v) {
         if (row < a.n) a.partial[(size_t)c.pairs[i] * a.n + row] = v * __ldcg(a.weight + c.pairs[i]);
     };
     auto combine = [&](uint32_t first, uint32_t step) {
         __threadfence();
         __syncwarp();
-        const uint32_t i = first + lane * step;
-        const uint32_t t = i < tokens ? c.pairs[i] / a.top_k : 0;
-        const bool last = i < tokens && atomicAdd(a.arrived + ((size_t)t * a.row_tiles + tile) * 4 + q, 1u) == a.top_k - 1;
-        uint32_t mask = __ballot_sync(~0u, last);
-        __threadfence();
-        while (mask) {
-            const uint32_t to = __shfl_sync(~0u, t, __ffs(mask) - 1);
-            mask &= mask - 1;
-            if (row < a.n) {
-                const float *parts = a.partial + (size_t)to * a.top_k * a.n + row;
-                float sum = 0.0f;
+        const uint32_t each = (tokens - first + step - 1) / step, all = first < tokens ? tiles * each : 0;
+        for (uint32_t j0 = 0; j0 < all; j0 += 32) {
+            const uint32_t j = j0 + lane, of = j / each, i = first + (j - of * each) * step;
+            const uint32_t t = j < all ? c.pairs[i] / a.top_k : 0;
+            const bool last =
+                j < all && atomicAdd(a.arrived + ((size_t)t * a.row_tiles + tile0 + of) * 4 + q, 1u) == a.top_k - 1;
+            uint32_t mask = __ballot_sync(~0u, last);
+            __threadfence();
+            while (mask) {
+                const int from = __ffs(mask) - 1;
+                const uint32_t to = __shfl_sync(~0u, t, from), at = (tile0 + __shfl_sync(~0u, of, from)) * 128 + q * 32 + lane;
+                mask &= mask - 1;
+                if (at < a.n) {
+                    const float *parts = a.partial + (size_t)to * a.top_k * a.n + at;
+                    float sum = 0.0f;
 #pragma unroll 8
-                for (uint32_t j = 0; j < a.top_k; j++) sum += __ldcg(parts + (size_t)j * a.n);
-                put_as(a.y, a.type, to * a.stride + row, sum);
+                    for (uint32_t p = 0; p < a.top_k; p++) sum += __ldcg(parts + (size_t)p * a.n);
+                    put_as(a.y, a.type, to * a.stride + at, sum);
+                }
             }
         }
     };
@@ -485,7 +491,6 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&c.acc_empty[nth & 1]));
-        if (MODE == kDown && a.split == 1) combine(0, 1);
         if (MODE == kGateUp && a.split == 1) {
             asm volatile("bar.sync 1, 128;" ::: "memory");
             for (uint32_t i = q / 2; i < tokens; i += 2) {   // a warp: half of the tokens, half of the tile's 64 values
@@ -494,6 +499,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
         }
     }
+    if (MODE == kDown && epi && a.split == 1) combine(0, 1);
     if (a.split > 1) {
         // the cluster's partial tiles, added in rank order through distributed shared memory
         cg::cluster_group cluster = cg::this_cluster();
@@ -757,17 +763,19 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     // save (one token, 4 of 32 experts: 18.1 us without, 18.4 to 19.5 with 2 or 4)
     a.split = 1;
     while (a.split < 8 && a.steps / a.split > 32) a.split *= 2;
-    // Row tiles to a CTA: its set-up (finding its tokens, their scales) costs as much as some 100 KB of
-    // weights, so it takes more tiles once there are enough to go round.
-    const uint32_t cols = up_to(a.nt, 8) * P;
+    // Row tiles to a CTA and CTAs to an SM. A CTA's set-up (its tokens, their scales) and end take as long as
+    // 100 to 200 KB of weights, so it takes more tiles once there are enough to go round, up to four of
+    // gate / up and two of down, whose end is longer and is hidden by a third CTA. 64 tokens, 128
+    // experts, d 2048, f 1024, tiles and CTAs for gate / up and down: 1, 2, 1, 2: 136 us; 2, 2, 2, 2: 125;
+    // 4, 2, 2, 2: 122; 4, 2, 2, 3: 118; 4, 2, 4, 2: 127.
+    const uint32_t cols = up_to(a.nt, 8) * P, most = MODE == kGateUp ? 4 : 2;
     a.per_cta = 1;
-    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < 4 && a.per_cta * a.steps < 32 &&
-           a.row_tiles * slots >= 148 * 2 * 2 * a.per_cta)
-        a.per_cta *= 2;
+    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < most && a.row_tiles * slots >= 148 * 2 * 2 * a.per_cta) a.per_cta *= 2;
+    const uint32_t per_sm = MODE == kDown && a.split == 1 && cols * (a.per_cta > 1 ? 2 : 1) <= 96 ? 3 : 2;
     a.head_bytes = 1024 + (a.steps + a.split - 1) / a.split * kMxScaleTile +
                    (MODE == kGateUp ? up_to(pairs, kMxScaleTile) + a.nt * 512 : 0);
     a.head_bytes = up_to(a.head_bytes, 1024);
-    const uint32_t smem = plan_ring<8, P, MODE>(a, 2);
+    const uint32_t smem = plan_ring<8, P, MODE>(a, per_sm);
     CUtensorMap wmap, xmap;
     cudaError_t r = encode_weights<8>(&wmap, MODE == kGateUp ? e.gate_up_codes : e.down_codes,
                                       (uint64_t)e.experts * a.row_tiles * a.kw);
