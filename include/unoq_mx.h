@@ -78,6 +78,7 @@ UG_API int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32
 UG_API int ug_mx4_matmul_x16(const void *x, int x_type, uint64_t x_stride, uint32_t m, const uint8_t *w_codes,
                              const uint8_t *w_scales, uint32_t n, uint32_t k, void *y, int type, uint64_t stride,
                              void *workspace, size_t workspace_bytes, void *stream);
+/* Bytes of that call's workspace; 0 (workspace may be NULL) for few rows. */
 UG_API size_t ug_mx4_matmul_x16_workspace(uint32_t m, uint32_t k, int x_type);
 
 /* A mixture-of-experts layer for a few tokens. */

@@ -142,7 +142,7 @@ def test_dequantize_leaves_the_rest_of_a_wide_output(mx):
 
 # ---- products ------------------------------------------------------------------------------------
 
-PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 3, 33), (7, 129, 127), (8, 128, 128), (16, 256, 512), (17, 200, 1000), (65, 130, 257),
+PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 3, 33), (7, 129, 127), (8, 128, 128), (9, 300, 700), (10, 140, 1500), (11, 130, 260), (16, 256, 512), (16, 1200, 2049), (17, 200, 1000), (65, 130, 257),
             (128, 256, 384), (129, 384, 640), (200, 1000, 96), (257, 515, 1023), (300, 129, 4100), (1, 4096, 4096),
             (3, 2049, 8192), (40, 4097, 2080), (600, 700, 300),
             # many tokens: pairs of CTAs, odd numbers of row tiles and ragged last tiles among them
@@ -552,14 +552,15 @@ def test_experts_workspace_contents_do_not_matter(mx, native):
 
 def test_product_workspace_contents_do_not_matter(mx, native):
     W = mx.pack(*on_gpu(weights(130, 200, 2)))
-    x = torch.randn(5, 200, generator=gen(2), device="cuda").to(torch.float16)
+    x = torch.randn(25, 200, generator=gen(2), device="cuda").to(torch.float16)
     want = mx.matmul(x, W)
-    need = native.ug_mx4_matmul_x16_workspace(5, 200, 1)
+    need = native.ug_mx4_matmul_x16_workspace(25, 200, 1)
+    assert need
     for fill in (0, 255, 127):
         ws = torch.full((need + 4096,), fill, dtype=torch.uint8, device="cuda")
-        y = torch.empty(5, 130, device="cuda", dtype=torch.float16)
+        y = torch.empty(25, 130, device="cuda", dtype=torch.float16)
         torch.cuda.synchronize()
-        rc = native.ug_mx4_matmul_x16(x.data_ptr(), 1, 200, 5, W.codes.data_ptr(), W.scales.data_ptr(), 130, 200, y.data_ptr(), 1,
+        rc = native.ug_mx4_matmul_x16(x.data_ptr(), 1, 200, 25, W.codes.data_ptr(), W.scales.data_ptr(), 130, 200, y.data_ptr(), 1,
                                       130, ws.data_ptr(), need, None)
         assert rc == 0
         torch.cuda.synchronize()

@@ -20,7 +20,9 @@ def test_sizes(native):
     assert native.ug_mx4_pack_rows(2, 260, 1) == 2 * 384 and native.ug_mx4_pack_rows(2, 128, 1) == 256
     assert native.ug_mx4_pack_rows(2 ** 31, 130, 0) == 0  # does not fit
     assert native.ug_mx4_matmul_x16_workspace(3, 100, 0) == 0
-    assert native.ug_mx4_matmul_x16_workspace(3, 100, 2) >= 6 * 128 + 512
+    assert native.ug_mx4_matmul_x16_workspace(40, 100, 2) >= 80 * 128 + 512
+    assert native.ug_mx4_matmul_x16_workspace(16, 100, 2) == 0 and native.ug_mx4_matmul_x16_workspace(17, 100, 2) > 0
+    assert native.ug_mx4_matmul_x16_workspace(10, 100, 1) == 0 and native.ug_mx4_matmul_x16_workspace(11, 100, 1) > 0
 
 
 def test_quantize_refusals(native):
@@ -67,13 +69,14 @@ def test_product_refusals(native):
     assert mm(P, P, 1, P + 8, P, 8, 32, P, 0, 8, None) == 22
     assert mm(P, P, 1, P, P, 8, 32, P + 2, 0, 8, None) == 22
     assert mm(None, None, 0, None, None, 8, 32, None, 0, 8, None) == 0
-    need = native.ug_mx4_matmul_x16_workspace(1, 32, 2)
-    assert mx(P, 0, 32, 1, P, P, 8, 32, P, 0, 8, P, need, None) == 18   # 32-bit x
-    assert mx(P, 2, 31, 1, P, P, 8, 32, P, 0, 8, P, need, None) == 18
-    assert mx(P, 2, 32, 1, P, P, 8, 32, P, 0, 8, P, need - 1, None) == 22
-    assert mx(P, 2, 32, 1, P, P, 8, 32, P, 0, 8, P + 16, need, None) == 22
-    assert mx(P, 2, 32, 1, P, P, 8, 32, P, 0, 8, None, need, None) == 22
-    assert mx(P + 1, 2, 32, 1, P, P, 8, 32, P, 0, 8, P, need, None) == 22
+    need = native.ug_mx4_matmul_x16_workspace(64, 32, 2)
+    assert mx(P, 0, 32, 64, P, P, 8, 32, P, 0, 8, P, need, None) == 18   # 32-bit x
+    assert mx(P, 2, 31, 64, P, P, 8, 32, P, 0, 8, P, need, None) == 18
+    assert mx(P, 2, 32, 64, P, P, 8, 32, P, 0, 8, P, need - 1, None) == 22
+    assert mx(P, 2, 32, 64, P, P, 8, 32, P, 0, 8, P + 16, need, None) == 22
+    assert mx(P, 2, 32, 64, P, P, 8, 32, P, 0, 8, None, need, None) == 22
+    assert mx(P + 1, 2, 32, 64, P, P, 8, 32, P, 0, 8, P, need, None) == 22
+    assert mx(P + 1, 2, 32, 1, P, P, 8, 32, P, 0, 8, None, 0, None) == 22
     assert mx(None, 2, 32, 0, None, None, 8, 32, None, 0, 8, None, 0, None) == 0
 
 

@@ -27,6 +27,8 @@ __host__ __device__ inline uint32_t mx_tiles(uint32_t n) { return (n + kMxTile -
 __host__ __device__ inline uint32_t mx_ktiles(uint32_t k) { return (k + 255) / 256 * 2; }
 // Pieces of a 16-bit value: 4 significant bits each, so two hold a bf16 (8) and three an f16 (11).
 __host__ __device__ inline int mx_pieces(int type) { return type == 2 ? 2 : 3; }
+// Whether the product splits m tokens itself: their pieces fill at most 32 columns, 16 bf16 or 10 f16 tokens.
+inline bool mx_fused(uint32_t m, int type) { return (uint64_t)m * mx_pieces(type) <= 32; }
 
 #ifdef __CUDACC__
 __device__ __forceinline__ size_t mx_code_at(uint32_t r, uint32_t j, uint32_t kt) {
@@ -185,6 +187,17 @@ __device__ __forceinline__ uint32_t mx_e4m3x2(float a, float b, float2 *back) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(p));
     *back = __half22float2(*reinterpret_cast<const __half2 *>(&h));
     return p;
+}
+
+// The next piece of eight values, as four pairs of e4m3; what it leaves of them, 16 times as large, in v.
+__device__ __forceinline__ void mx_piece8(float (&v)[8], uint32_t (&h)[4]) {
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        float2 back;
+        h[b] = mx_e4m3x2(v[2 * b], v[2 * b + 1], &back);
+        v[2 * b] = (v[2 * b] - back.x) * 16.0f;
+        v[2 * b + 1] = (v[2 * b + 1] - back.y) * 16.0f;
+    }
 }
 
 // One float to e4m3 (nearest even, saturating) and the value that it stands for.

@@ -211,7 +211,7 @@ int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32_t m, c
 }
 
 size_t ug_mx4_matmul_x16_workspace(uint32_t m, uint32_t k, int x_type) {
-    if (!is_half(x_type) || !k) return 0;
+    if (!is_half(x_type) || !k || uq::mx_fused(m, x_type)) return 0;
     const size_t rows = uq::mx_piece_rows(m, x_type), kt = (k + 127ull) / 128;
     return up(rows * kt * 128) + up((rows + 127) / 128 * kt * uq::kMxScaleTile);
 }
@@ -220,10 +220,10 @@ int ug_mx4_matmul_x16(const void *x, int x_type, uint64_t x_stride, uint32_t m, 
                       const uint8_t *w_scales, uint32_t n, uint32_t k, void *y, int type, uint64_t stride,
                       void *workspace, size_t workspace_bytes, void *stream) {
     if (!is_half(x_type) || x_stride < k) return fail(18, "ug_mx4_matmul_x16: x must be 16-bit with rows k apart or more");
-    if (m && n && (!x || !is_aligned(x, 2) || !workspace || !is_aligned(workspace, 256)))
+    const size_t need = ug_mx4_matmul_x16_workspace(m, k, x_type);
+    if (m && n && (!x || !is_aligned(x, 2) || (need && (!workspace || !is_aligned(workspace, 256)))))
         return fail(22, "ug_mx4_matmul_x16: null or misaligned x or workspace");
-    if (m && n && workspace_bytes < ug_mx4_matmul_x16_workspace(m, k, x_type))
-        return fail(22, "ug_mx4_matmul_x16: workspace too small");
+    if (m && n && workspace_bytes < need) return fail(22, "ug_mx4_matmul_x16: workspace too small");
     uq::MxProductArgs p{};
     p.x = x;
     p.x_type = x_type;
@@ -236,7 +236,7 @@ int ug_mx4_matmul_x16(const void *x, int x_type, uint64_t x_stride, uint32_t m, 
     p.y = y;
     p.type = type;
     p.stride = stride;
-    p.workspace = workspace;
+    p.workspace = need ? workspace : nullptr;
     return product(p, stream, "ug_mx4_matmul_x16: type, sizes, stride or pointers out of range");
 }
 

@@ -18,6 +18,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_state.hpp"
 #include "mx.cuh"
@@ -37,7 +38,7 @@ constexpr uint32_t kA = 16384;     // one weight tile in shared memory
 
 __host__ __device__ constexpr uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
-enum Mode { kDense = 0, kGateUp = 1, kDown = 2 };
+enum Mode { kDense = 0, kGateUp = 1, kDown = 2, kFused = 3 };   // kFused: dense, 16-bit activations split in the kernel
 
 struct TcArgs {
     uint32_t m, n;            // tokens, weight rows of one matrix
@@ -50,6 +51,11 @@ struct TcArgs {
     void *y;
     int type;
     uint64_t stride;
+    // kFused
+    const void *x;
+    uint32_t k;
+    uint64_t x_stride;
+    bool x_vec;
     // experts
     uint32_t top_k, per_cta, chunk, head_bytes;   // head: the choices, the columns' scales, gate and up values
     const int32_t *chosen;
@@ -74,6 +80,7 @@ static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 template <int KIND, int P, int MODE>
 __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__ CUtensorMap wmap,
                                                          const __grid_constant__ CUtensorMap xmap, const TcArgs a) {
+    constexpr bool kExperts = MODE == kGateUp || MODE == kDown;
     constexpr uint32_t kSub = KIND == 8 ? 1 : 2;                  // scale tiles of a stage, per 128 rows
     constexpr uint32_t kSf = kSub * kMxScaleTile;
     constexpr uint32_t kWeightTx = (KIND == 8 ? kMxCodeTile / 2 : kMxCodeTile) + kSf;  // an unpacking copy counts what it reads
@@ -84,7 +91,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     uint32_t *counts = reinterpret_cast<uint32_t *>(base + kCtrlBytes);
     uint8_t *ids = base + kCtrlBytes + 1024;
     uint8_t *sfb_all = ids + (MODE == kGateUp ? up_to(a.m * a.top_k, kMxScaleTile) : 0);
-    uint8_t *ring = base + kCtrlBytes + (MODE == kDense ? 0 : a.head_bytes);
+    uint8_t *ring = base + kCtrlBytes + (kExperts ? a.head_bytes : 0);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = blockIdx.z;
     volatile int *abort = &c.abort;
@@ -113,9 +120,9 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     uint32_t tokens, tok0 = 0, expert = 0, chunk = 0;  // columns: tokens, or a chunk of one expert's pairs
     uint32_t mine = 0;                                 // lanes (pairs) of the expert, where one warp holds all pairs
     const uint32_t k0 = a.steps * rank / a.split, k1 = a.steps * (rank + 1) / a.split;
-    const uint32_t pairs = MODE == kDense ? 0 : a.m * a.top_k;
+    const uint32_t pairs = kExperts ? a.m * a.top_k : 0;
     const bool one_warp = MODE == kGateUp && pairs <= 32 && a.m <= a.chunk;
-    if constexpr (MODE == kDense) {
+    if constexpr (!kExperts) {
         tok0 = blockIdx.y * a.nt;
         tokens = min(a.nt, a.m - tok0);
     } else {
@@ -189,12 +196,12 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         w_tile = expert * a.row_tiles + tile0;
     }
     const uint32_t n_cols = (tokens * P + 7) / 8 * 8;
-    const uint32_t col_tiles = MODE == kDense ? (n_cols + 127) / 128 : 1;
+    const uint32_t col_tiles = kExperts ? 1 : (n_cols + 127) / 128;
     const uint32_t sfb_cols = a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
     // the experts' ring is as deep as this expert's few tokens allow
-    const uint32_t b_bytes = MODE == kDense ? a.b_bytes : n_cols * 128;
-    const uint32_t stage_bytes = MODE == kDense ? a.stage_bytes : kA + b_bytes + 1024;
-    const uint32_t stages = MODE == kDense ? a.stages : min(a.stages, a.ring_bytes / stage_bytes);
+    const uint32_t b_bytes = kExperts ? n_cols * 128 : a.b_bytes;
+    const uint32_t stage_bytes = kExperts ? kA + b_bytes + 1024 : a.stage_bytes;
+    const uint32_t stages = kExperts ? min(a.stages, a.ring_bytes / stage_bytes) : a.stages;
 
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
@@ -221,9 +228,9 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 
     if (warp == 0 && elect_one()) {
         // ---- weight tiles and their scales, in the order of memory ----
-        // KIND 8's kernel before makes pieces and has seen all earlier work done; before KIND 4's may be any kernel,
-        // one that writes the weights too
-        if (MODE == kDense && KIND == 4) grid_dep_wait();
+        // The kernel before may be any, one that writes the weights too; but the one that makes pieces has seen
+        // all earlier work done.
+        if (MODE == kFused || (MODE == kDense && KIND == 4)) grid_dep_wait();
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;   // phase 1: not yet used
         for (uint32_t tile = 0; tile < tiles; tile++) {
@@ -245,10 +252,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
     weights_out:
         if (*abort) drain(issued);
-    } else if (warp == 6) {
+    } else if (warp == 6 && MODE != kFused) {
         // ---- activation columns and, for dense products, their scales ----
-        const bool listed = MODE == kDense || mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605);
-        if (MODE != kDense && listed)
+        const bool listed = !kExperts || mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605);
+        if (kExperts && listed)
             for (uint32_t i = lane; i < n_cols; i += 32) c.rows[i] = (int32_t)row_of(i);
         __syncwarp();
         if (listed && elect_one()) {
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         // each stage has scale columns of its own: they are rewritten only after its MMAs are done
         uint32_t st = st0, full = full0, empty = empty0, sfa = sf_tmem, s = 0, phase = 0;
-        bool ok = MODE == kDense || mbar_wait(smem_u32(&c.scales_ready), 0, abort, 606);
+        bool ok = !kExperts || mbar_wait(smem_u32(&c.scales_ready), 0, abort, 606);
         for (uint32_t tile = 0; ok && tile < tiles; tile++) {
             if (tile >= 2 && !mbar_poll(smem_u32(&c.acc_empty[tile & 1]), (tile / 2 & 1) ^ 1, abort, 607)) {
                 ok = false;
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
 #pragma unroll
                 for (uint32_t h = 0; h < kSub; h++) {
                     scales_to_tmem(sfa + 4 * h, sf + h * kMxScaleTile);
-                    if (MODE == kDense) {
+                    if (!kExperts) {
                         scales_to_tmem(sfb + sfb_cols * h, sf + kSf + h * kMxScaleTile);
                         if (col_tiles > 1) scales_to_tmem(sfb + sfb_cols * h + 4, sf + 2 * kSf + h * kMxScaleTile);
                     } else {
@@ -355,7 +362,66 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     }
     __syncwarp();
     const bool epi = warp >= 2 && warp < 6;
-    if (MODE != kDense && epi) {
+    if constexpr (MODE == kFused) {
+        // ---- the columns of at most 32 pieces, made here (a launch of its own for them costs 2.5 us of the host's
+        // time): a warp to every fourth stage, 16 lanes to a token's 128 values of it ----
+        using T = typename std::conditional<P == 2, __nv_bfloat16, __half>::type;
+        constexpr uint32_t kPasses = 32 / P / 2;   // two tokens each
+        if (epi) {
+            grid_dep_wait();
+            const uint32_t l16 = lane % 16, passes = (tokens + 1) / 2;
+            MxRaw<T> raw[kPasses];   // of the warp's next stage
+            auto load = [&](uint32_t step, uint32_t n) {
+                const uint32_t j = (k0 + step) * 128 + l16 * 8, left = step < steps && j < a.k ? a.k - j : 0;
+                const uint32_t t = n * 2 + lane / 16;
+                const T *p = static_cast<const T *>(a.x) + t * a.x_stride + j;
+                if (a.x_vec && left >= 8 && t < tokens) raw[n].load(p);
+                else raw[n].load_some(p, t < tokens ? left : 0);
+            };
+            const uint32_t w = warp - 2;
+#pragma unroll
+            for (uint32_t n = 0; n < kPasses; n++)
+                if (n < passes) load(w, n);
+            uint32_t s = w, phase = 1;
+            while (s >= stages) s -= stages, phase ^= 1;
+            for (uint32_t step = w; step < steps; step += 4) {
+                if (!__all_sync(~0u, mbar_poll(smem_u32(&c.empty[s]), phase, abort, 609))) break;
+                const uint32_t b = smem_u32(ring + s * stage_bytes) + kA, sf = b + b_bytes + kSf;
+#pragma unroll
+                for (uint32_t n = 0; n < kPasses; n++) {
+                    if (n >= passes) break;
+                    const uint32_t t = n * 2 + lane / 16;
+                    uint32_t top = raw[n].top();
+                    top = max(top, __shfl_xor_sync(~0u, top, 1));
+                    top = max(top, __shfl_xor_sync(~0u, top, 2));
+                    const uint32_t sc = mx_piece_scale(__uint_as_float(raw[n].top_bits(top)), P);
+                    float v[8];
+                    raw[n].values(v, __uint_as_float((254u - min(sc, 253u)) << 23));
+                    load(step + 4, n);
+#pragma unroll
+                    for (uint32_t p = 0; p < P; p++) {
+                        uint32_t h[4];
+                        mx_piece8(v, h);
+                        if (t >= tokens) continue;
+                        if (sc == 255) h[0] = h[1] = h[2] = h[3] = 0;
+                        const uint32_t r = t * P + p;   // column; SWIZZLE_128B: its 16-byte chunks by its place in eight
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(b + r * 128 + ((l16 / 2 ^ (r & 7)) << 4) + l16 % 2 * 8),
+                                     "r"(h[0] | h[1] << 16), "r"(h[2] | h[3] << 16)
+                                     : "memory");
+                        if (l16 % 4 == 0)
+                            asm volatile("st.shared.u8 [%0], %1;" ::"r"(sf + r * 16 + l16 / 4), "r"(mx_piece_scale_of(sc, p)) : "memory");
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&c.full[s]));
+                s += 4;
+                while (s >= stages) s -= stages, phase ^= 1;
+            }
+        }
+        __syncwarp();
+    }
+    if (kExperts && epi) {
         // ---- the item's tokens, and all their scales of this CTA's share of K ----
         const uint32_t at = threadIdx.x - 64;
         if (MODE == kGateUp && one_warp) {
@@ -462,7 +528,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         mbar_wait(smem_u32(&c.acc_full[nth & 1]), nth / 2 & 1, abort, 604);
         tc_fence_after();
         const uint32_t taddr = tmem + (q * 32 << 16) + (nth & 1) * a.d_cols;
-        if (MODE == kDense && a.split == 1) {
+        if (!kExperts && a.split == 1) {
             constexpr uint32_t kAt = P == 1 ? 32 : P == 2 ? 16 : 8;   // tokens at a time: up to 32 columns
             uint32_t i0 = 0;
             for (; i0 + kAt <= up_to(tokens, 8); i0 += kAt) {
@@ -581,13 +647,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(const T *x, uint32_t m, uin
 #pragma unroll
         for (int p = 0; p < P; p++, r++, to += (size_t)kt * 128) {
             uint32_t h[4];
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                float2 back;
-                h[b] = mx_e4m3x2(v[2 * b], v[2 * b + 1], &back);
-                v[2 * b] = (v[2 * b] - back.x) * 16.0f;
-                v[2 * b + 1] = (v[2 * b + 1] - back.y) * 16.0f;
-            }
+            mx_piece8(v, h);
             if (mine) {
                 *reinterpret_cast<uint2 *>(to) = s == 255 ? make_uint2(0, 0) : make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
                 if (lane % 4 == 0) scales[mx_scale_at(r, j / 32, kt)] = (uint8_t)mx_piece_scale_of(s, p);
@@ -654,9 +714,10 @@ cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArg
 template <int KIND, int P, int MODE>
 uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t n = up_to(a.nt * P, 8), sub = KIND == 8 ? 1 : 2;
+    const bool experts = MODE == kGateUp || MODE == kDown;
     a.b_box_bytes = (KIND == 8 || n < 128 ? n : 128) * 128;       // KIND 4 copies whole tiles of 128 columns
     a.b_bytes = KIND == 8 ? n * 128 : (n + 127) / 128 * a.b_box_bytes;
-    a.stage_bytes = kA + a.b_bytes + up_to(kMxScaleTile * sub * (1 + (MODE == kDense ? (n + 127) / 128 : 0)), 1024);
+    a.stage_bytes = kA + a.b_bytes + up_to(kMxScaleTile * sub * (1 + (experts ? 0 : (n + 127) / 128)), 1024);
     a.d_cols = up_to(a.nt, 8) * P;
     const uint32_t sf_cols = sub * (4 + (a.nt * P > 128 ? 8 : 4));
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
@@ -664,7 +725,7 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t cols = per_sm == 1 ? 512 : per_sm == 2 ? 256 : 128;
     const uint32_t acc_cols = a.d_cols * (a.per_cta > 1 ? 2 : 1);
     a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, (a.steps + a.split - 1) / a.split * a.per_cta});
-    if (MODE == kDense) {
+    if (!experts) {
         a.stages = std::min(a.stages, budget / a.stage_bytes);
         a.ring_bytes = a.stages * a.stage_bytes;
     } else {   // the kernel fits its stages into this by its expert's number of tokens
@@ -676,11 +737,12 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     return extra + std::max(a.ring_bytes, red);
 }
 
-template <int KIND, int P>
+// x, x_scales: MX4 codes (KIND 4) or pieces (KIND 8), or null for MODE kFused.
+template <int KIND, int P, int MODE>
 cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_scales, cudaStream_t s) {
     const uint32_t rt = mx_tiles(p.n), kw = mx_ktiles(p.k) / 2;
     constexpr uint32_t kGroup = P == 1 ? 256 : P == 2 ? 128 : 64;   // tokens that fill 256 columns (P = 3: 192)
-    if (p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 37) return pair_product<KIND, P>(p, x, x_scales, s);
+    if (MODE == kDense && p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 37) return pair_product<KIND, P>(p, x, x_scales, s);
     TcArgs a{};
     a.m = p.m;
     a.n = p.n;
@@ -700,22 +762,29 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.y = p.y;
     a.type = p.type;
     a.stride = p.stride;
-    const uint32_t smem = plan_ring<KIND, P, kDense>(a, per_sm);
+    a.x = p.x;
+    a.k = p.k;
+    a.x_stride = p.x_stride;
+    a.x_vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.x_stride % 8 == 0;
+    const uint32_t smem = plan_ring<KIND, P, MODE>(a, per_sm);
     CUtensorMap wmap, xmap;
     cudaError_t e = encode_weights<KIND>(&wmap, p.w_codes, (uint64_t)rt * kw);
     if (e != cudaSuccess) return e;
-    if (KIND == 8)
+    if (MODE == kFused)
+        xmap = wmap;   // not read
+    else if (KIND == 8)
         e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)a.steps * 128, mx_piece_rows(p.m, p.x_type),
                    (uint64_t)a.steps * 128, 128, a.b_box_bytes / 128, CU_TENSOR_MAP_SWIZZLE_128B);
     else
         e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 128, (uint64_t)mx_tiles(p.m) * kw * 128, 128, 128, a.b_box_bytes / 128,
                    CU_TENSOR_MAP_SWIZZLE_128B);
     if (e != cudaSuccess) return e;
-    return launch<KIND, P, kDense>(wmap, xmap, a, dim3(rt, tt, a.split), smem, s);
+    return launch<KIND, P, MODE>(wmap, xmap, a, dim3(rt, tt, a.split), smem, s);
 }
 
 template <typename T, int P>
 cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
+    if (mx_fused(p.m, p.x_type)) return dense<8, P, kFused>(p, nullptr, nullptr, s);
     const uint32_t kt = mx_tiles(p.k), chunks = (p.k + 255) / 256;
     constexpr uint32_t kGroup = P == 2 ? 128 : 64;
     uint8_t *pieces = static_cast<uint8_t *>(p.workspace);
@@ -727,7 +796,7 @@ cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
     auto kernel = many ? pieces_kernel<T, P, 4> : pieces_kernel<T, P, 1>;
     const cudaError_t e = launch_pdl(kPdlMx, kernel, (unsigned)((warps + 7) / 8), 256, 0, s, static_cast<const T *>(p.x), p.m, p.k,
                                      p.x_stride, kt, chunks, kGroup, pieces, scales, vec);
-    return e != cudaSuccess ? e : dense<8, P>(p, pieces, scales, s);
+    return e != cudaSuccess ? e : dense<8, P, kDense>(p, pieces, scales, s);
 }
 
 template <int P, int MODE>
@@ -795,7 +864,7 @@ size_t mx_piece_rows(uint32_t m, int x_type) {
 }
 
 cudaError_t launch_mx4_product(const MxProductArgs &a, cudaStream_t s) {
-    if (!a.x) return dense<4, 1>(a, a.a_codes, a.a_scales, s);
+    if (!a.x) return dense<4, 1, kDense>(a, a.a_codes, a.a_scales, s);
     if (a.x_type == 1) return dense_x16<__half, 3>(a, s);
     return dense_x16<__nv_bfloat16, 2>(a, s);
 }

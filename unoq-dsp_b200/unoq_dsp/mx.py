@@ -124,7 +124,7 @@ class MX4:
     in the ``layout`` ``"operand"`` (what :func:`matmul` reads) or ``"stored"`` (row-major, the form of
     files: (rows, ceil(k/2)) and (rows, ceil(k/32)))."""
 
-    __slots__ = ("rows", "k", "layout", "device", "_data", "_codes", "_scales")
+    __slots__ = ("rows", "k", "layout", "device", "_data", "_any", "_codes", "_scales")
 
     def __init__(self, codes, scales, rows, k, layout="operand"):
         if rows < 0 or k < 1:
@@ -136,18 +136,19 @@ class MX4:
         if codes.device != scales.device:
             raise ValueError("codes and scales are on two devices")
         self.rows, self.k, self.layout, self.device = rows, k, layout, codes.device
-        self._data, self._codes, self._scales = (codes, scales), codes.data_ptr(), scales.data_ptr()
+        self._data, self._any = (codes, scales), codes   # _any: a tensor to allocate beside
+        self._codes, self._scales = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _new(cls, rows, k, layout, device):
-        """An unwritten one: both arrays in one allocation, the codes first."""
+    def _new(cls, rows, k, layout, beside):
+        """An unwritten one on the device of `beside`: both arrays in one allocation, the codes first."""
         code_bytes, scale_bytes = _sizes(layout == "operand", rows, k)
-        at = -(-code_bytes // 16) * 16
+        at = (code_bytes + 15) & ~15
         self = cls.__new__(cls)
-        self.rows, self.k, self.layout, self.device = rows, k, layout, device
-        self._data = torch.empty(at + scale_bytes, dtype=torch.uint8, device=device)
-        self._codes = self._data.data_ptr()
-        self._scales = self._codes + at
+        self._data = self._any = data = beside.new_empty(at + scale_bytes, dtype=torch.uint8)
+        self.rows, self.k, self.layout, self.device = rows, k, layout, data.device
+        self._codes = codes = data.data_ptr()
+        self._scales = codes + at
         return self
 
     def _views(self):
@@ -179,7 +180,7 @@ class MX4:
         lib, rows, k, device = _library(), self.rows, self.k, self.device
         stride = k
         if out is None:
-            out = torch.empty((rows, k), dtype=dtype, device=device)
+            out = self._any.new_empty((rows, k), dtype=dtype)
         else:
             _output(out, (rows, k), dtype, device, (self.codes, self.scales))
             stride = _row_stride(out, rows, k)
@@ -201,9 +202,9 @@ def quantize(x, layout="operand"):
     2^(floor(log2 of its largest magnitude) - 2); values go to the nearest e2m1 (ties to even), at
     most 6 scales; a block holding a NaN or an infinity becomes NaN."""
     x, rows, k, stride = _rows(_input(x, "x", _TYPES), "x")
-    lib, code, device = _library(), _layout(layout), x.device
-    q = MX4._new(rows, k, layout, device)
-    rc = lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, stride, code, q._codes, q._scales, _stream(device))
+    lib, code = _library(), _layout(layout)
+    q = MX4._new(rows, k, layout, x)
+    rc = lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, stride, code, q._codes, q._scales, _stream(q.device))
     if rc:
         _check(lib, rc, "MX4 quantise")
     return q
@@ -263,7 +264,7 @@ def matmul(a, w, dtype=None, out=None):
         raise ValueError(f"a has rows of {k} on {a.device}, w of {w.k} on {device}")
     stride = n
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = w._any.new_empty(shape, dtype=dtype)
     else:
         _output(out, shape, dtype, device, ((a.codes, a.scales) if four else (a,)) + (w.codes, w.scales))
         if out.dim() == 2:
@@ -278,9 +279,9 @@ def matmul(a, w, dtype=None, out=None):
             if len(_need) > 4096:
                 _need.clear()
             need = _need[m, k, x_type] = lib.ug_mx4_matmul_x16_workspace(m, k, x_type)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = w._any.new_empty(need) if need else None   # bytes
         rc = lib.ug_mx4_matmul_x16(a.data_ptr(), x_type, a_stride, m, w._codes, w._scales, n, k, out.data_ptr(),
-                                   _TYPES[dtype], stride, ws.data_ptr(), need, _stream(device))
+                                   _TYPES[dtype], stride, ws.data_ptr() if need else None, need, _stream(device))
     if rc:
         _check(lib, rc, "MX4 product")
     return out
@@ -340,7 +341,7 @@ class Experts:
             raise ValueError(f"at most {MAX_TOKENS} tokens, not {t}")
         stride = d
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=device)
+            out = x.new_empty(shape)
         else:
             _output(out, shape, x.dtype, device, (x, self.router, *self.gate_up, *self.down))
             if out.dim() == 2:
@@ -352,7 +353,7 @@ class Experts:
         need = self._need.get(t)
         if need is None:
             need = self._need[t] = self._lib.ug_mx4_experts_workspace(self._ref, t)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = self.down[0].new_empty(need)   # bytes
         rc = self._lib.ug_mx4_experts(self._ref, x.data_ptr(), x_stride, t, out.data_ptr(), stride,
                                       chosen.data_ptr() if return_choice else None,
                                       weights.data_ptr() if return_choice else None, ws.data_ptr(), need, _stream(device))
