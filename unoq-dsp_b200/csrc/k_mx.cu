@@ -331,9 +331,9 @@ unsigned unit_grid(uint64_t units) {
     return (unsigned)(need < 148 * 16 ? need : 148 * 16);
 }
 
-// Rows to a warp: 8 (4 in 32 bits) once that still leaves every SM a full set of 64 warps, else one,
+// Rows to a warp: 8 (4 in 32 bits) once that still leaves every SM 32 warps, else one,
 // so that small matrices spread over the GPU.
-bool many_rows(uint32_t rows, uint32_t chunks, int each) { return (uint64_t)(rows / each) * chunks >= 148 * 64; }
+bool many_rows(uint32_t rows, uint32_t chunks, int each) { return (uint64_t)(rows / each) * chunks >= 148 * 32; }
 unsigned row_grid(uint32_t rows, uint32_t chunks, int each) {
     return (unsigned)((((uint64_t)rows + each - 1) / each * chunks + 7) / 8);
 }

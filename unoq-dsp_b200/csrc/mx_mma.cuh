@@ -15,19 +15,26 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-// Bounded wait that polls instead of suspending: what the copy and MMA threads wait for is mostly there, or
-// comes within some hundred cycles, and a wait with a suspension limit costs 63 cycles even then, a
-// plain one 27.
+// Bounded wait that polls: what is waited for is mostly there, or comes within some hundred cycles, and a
+// wait with a suspension limit costs 63 cycles even then, a plain one 27, and wakes later.
 __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int *abort, int code) {
-    for (int i = 0; i < 64; i++) {
+    long long start = 0;
+    for (uint32_t i = 0;; i++) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok)
                      : "r"(bar), "r"(parity)
                      : "memory");
         if (ok) return true;
+        if (i % 64 != 63) continue;
+        if (*abort) return false;
+        if (!start) start = clock64();
+        if (clock64() - start > kTimeoutCycles) {
+            *abort = 1;
+            atomicCAS(&g_tc_error, 0, code);
+            return false;
+        }
     }
-    return mbar_wait(bar, parity, abort, code);
 }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)

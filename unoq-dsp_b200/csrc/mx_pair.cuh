@@ -16,6 +16,7 @@ struct PairArgs {
     void *y;
     int type;
     uint64_t stride;
+    bool wide;                            // 16-bit y whose rows start on 16 bytes
 };
 
 struct PairCtrl {
@@ -24,6 +25,7 @@ struct PairCtrl {
     int abort;
 };
 
+constexpr uint32_t kPairOut = 32 * 256;   // 32 tokens of a tile's 128 16-bit values, for each half of the epilogue
 constexpr int kPairThreads = 352;   // warp 0: weight copies, 1: MMA, 2-9: epilogue, 10: activation copies
 
 __device__ __forceinline__ uint32_t in_leader(uint32_t smem) {   // the same place in the pair's first CTA
@@ -88,7 +90,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     extern __shared__ uint8_t raw[];
     uint8_t *base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     PairCtrl &c = *reinterpret_cast<PairCtrl *>(base);
-    uint8_t *ring = base + kCtrlBytes;
+    uint8_t *out = base + kCtrlBytes, *ring = out + 2 * kPairOut;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = blockIdx.x % 2, pair = blockIdx.x / 2, pairs = gridDim.x / 2;
     volatile int *abort = &c.abort;
@@ -215,7 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         uint32_t nth = 0;
         for (uint32_t t = pair; t < a.tiles; t += pairs, nth++) {
             const uint32_t rp = t % a.row_pairs, tt = t / a.row_pairs;
-            if (!mbar_wait(smem_u32(&c.acc_full), nth & 1, abort, 615)) break;
+            if (!mbar_poll(smem_u32(&c.acc_full), nth & 1, abort, 615)) break;
             tc_fence_after();
             const uint32_t taddr = tmem + (q * 32 << 16) + half * kMine * P;
             float v[kMine];
@@ -230,7 +232,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(in_leader(smem_u32(&c.acc_empty)));
             const uint32_t row = (2 * rp + rank) * 128 + q * 32 + lane, tok = tt * kTokens + half * kMine;
-            if (row < a.n && tok < a.m) put_tokens_as(a.y, a.type, tok * a.stride + row, a.stride, v, a.m - tok);
+            if (!a.wide) {
+                if (row < a.n && tok < a.m) put_tokens_as(a.y, a.type, tok * a.stride + row, a.stride, v, a.m - tok);
+                continue;
+            }
+            // 32 tokens at a time through shared memory, so that 16 lanes write a token's 256 bytes: a warp's own 32
+            // rows would go out as half lines, which took the loads 10 us of 4096 x 8192 x 4096's 62
+            constexpr uint32_t kOut = kMine < 32 ? kMine : 32;
+            const uint32_t row0 = (2 * rp + rank) * 128, at = q * 32 + lane;
+            uint16_t *to = reinterpret_cast<uint16_t *>(out + half * kPairOut);
+#pragma unroll
+            for (uint32_t i0 = 0; i0 < kMine; i0 += kOut) {
+                if (tok + i0 >= a.m) break;   // the same for all of the half
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");   // the tokens before are out
+#pragma unroll
+                for (uint32_t j = 0; j < kOut; j++) {
+                    const float f = v[i0 + j];
+                    to[j * 128 + at] = a.type == 1 ? __half_as_ushort(__float2half_rn(f)) : __bfloat16_as_ushort(__float2bfloat16_rn(f));
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+#pragma unroll
+                for (uint32_t j = at / 16; j < kOut; j += 8) {
+                    const uint32_t t = tok + i0 + j, r = row0 + at % 16 * 8;
+                    if (t >= a.m || r >= a.n) continue;
+                    const uint16_t *from = to + j * 128 + at % 16 * 8;
+                    uint16_t *y = static_cast<uint16_t *>(a.y) + t * a.stride + r;
+                    if (r + 8 <= a.n) *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(from);
+                    else
+                        for (uint32_t b = 0; r + b < a.n; b++) y[b] = from[b];
+                }
+            }
         }
     }
     __syncwarp();
@@ -254,7 +285,9 @@ cudaError_t pair_product(const MxProductArgs &p, const uint8_t *x, const uint8_t
     a.row_pairs = (a.rt + 1) / 2;
     a.tiles = a.row_pairs * ((p.m + kTokens - 1) / kTokens);
     a.stage_bytes = kA + kB + up_to(3 * kSub * kMxScaleTile, 1024);
-    a.stages = std::min<uint32_t>({(226 * 1024 - 1024 - kCtrlBytes) / a.stage_bytes, (512 - kN) / (12 * kSub), (uint32_t)kMaxStages});
+    a.wide = p.type != 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.stride % 8 == 0;
+    const uint32_t extra = 1024 + kCtrlBytes + 2 * kPairOut;
+    a.stages = std::min<uint32_t>({(226 * 1024 - extra) / a.stage_bytes, (512 - kN) / (12 * kSub), (uint32_t)kMaxStages});
     a.y = p.y;
     a.type = p.type;
     a.stride = p.stride;
@@ -286,5 +319,5 @@ cudaError_t pair_product(const MxProductArgs &p, const uint8_t *x, const uint8_t
         return cudaErrorInvalidValue;
     const uint32_t sms = (uint32_t)current_sm_count() / 2 * 2;
     return launch_pdl(kPdlMx, kernel, dim3(std::min(2 * a.tiles, sms)), dim3(kPairThreads),
-                      (size_t)1024 + kCtrlBytes + a.stages * a.stage_bytes, s, wmap, xmap, wsmap, xsmap, a);
+                      (size_t)extra + a.stages * a.stage_bytes, s, wmap, xmap, wsmap, xsmap, a);
 }

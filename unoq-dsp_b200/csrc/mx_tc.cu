@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         if (*abort) drain(issued);
     } else if (warp == 6 && MODE != kFused) {
         // ---- activation columns and, for dense products, their scales ----
-        const bool listed = !kExperts || mbar_wait(smem_u32(&c.rows_ready), 0, abort, 605);
+        const bool listed = !kExperts || mbar_poll(smem_u32(&c.rows_ready), 0, abort, 605);
         if (kExperts && listed)
             for (uint32_t i = lane; i < n_cols; i += 32) c.rows[i] = (int32_t)row_of(i);
         __syncwarp();
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         // each stage has scale columns of its own: they are rewritten only after its MMAs are done
         uint32_t st = st0, full = full0, empty = empty0, sfa = sf_tmem, s = 0, phase = 0;
-        bool ok = !kExperts || mbar_wait(smem_u32(&c.scales_ready), 0, abort, 606);
+        bool ok = !kExperts || mbar_poll(smem_u32(&c.scales_ready), 0, abort, 606);
         for (uint32_t tile = 0; ok && tile < tiles; tile++) {
             if (tile >= 2 && !mbar_poll(smem_u32(&c.acc_empty[tile & 1]), (tile / 2 & 1) ^ 1, abort, 607)) {
                 ok = false;
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     for (uint32_t nth = 0; epi && nth < tiles; nth++) {
         tile = tile0 + nth;
         row = tile * 128 + q * 32 + lane;
-        mbar_wait(smem_u32(&c.acc_full[nth & 1]), nth / 2 & 1, abort, 604);
+        mbar_poll(smem_u32(&c.acc_full[nth & 1]), nth / 2 & 1, abort, 604);
         tc_fence_after();
         const uint32_t taddr = tmem + (q * 32 << 16) + (nth & 1) * a.d_cols;
         if (!kExperts && a.split == 1) {
@@ -791,7 +791,7 @@ cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
     const size_t rows = mx_piece_rows(p.m, p.x_type);
     uint8_t *scales = pieces + (rows * kt * 128 + 255) / 256 * 256;
     const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.x_stride % 8 == 0;
-    const bool many = (uint64_t)(p.m / 4) * chunks >= 148 * 64;   // as the quantiser's rule
+    const bool many = (uint64_t)(p.m / 4) * chunks >= 148 * 32;   // as the quantiser's rule
     const uint64_t warps = many ? (uint64_t)((p.m + 3) / 4) * chunks : (uint64_t)p.m * chunks;
     auto kernel = many ? pieces_kernel<T, P, 4> : pieces_kernel<T, P, 1>;
     const cudaError_t e = launch_pdl(kPdlMx, kernel, (unsigned)((warps + 7) / 8), 256, 0, s, static_cast<const T *>(p.x), p.m, p.k,
