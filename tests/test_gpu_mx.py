@@ -146,7 +146,8 @@ PRODUCTS = [(1, 1, 1), (1, 8, 32), (2, 3, 33), (7, 129, 127), (8, 128, 128), (9,
             (128, 256, 384), (129, 384, 640), (200, 1000, 96), (257, 515, 1023), (300, 129, 4100), (1, 4096, 4096),
             (3, 2049, 8192), (40, 4097, 2080), (600, 700, 300),
             # many tokens: pairs of CTAs, odd numbers of row tiles and ragged last tiles among them
-            (1100, 2400, 300), (700, 2433, 1000), (330, 2433, 129), (2000, 2700, 640), (1025, 4800, 65)]
+            (1100, 2400, 300), (700, 2433, 1000), (330, 2433, 129), (2000, 2700, 640), (1025, 4800, 65), (2048, 2304, 520),
+            (513, 8200, 70)]
 
 
 def whole(rows, k, seed, narrow):

@@ -742,7 +742,10 @@ template <int KIND, int P, int MODE>
 cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_scales, cudaStream_t s) {
     const uint32_t rt = mx_tiles(p.n), kw = mx_ktiles(p.k) / 2;
     constexpr uint32_t kGroup = P == 1 ? 256 : P == 2 ? 128 : 64;   // tokens that fill 256 columns (P = 3: 192)
-    if (MODE == kDense && p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 37) return pair_product<KIND, P>(p, x, x_scales, s);
+    // Pairs of CTAs once their tiles go round most of the 74: bf16 x, 512 x 8192 x 1024 (128 tiles) 11.8 us against
+    // 14.4 in single CTAs, 512 x 4096 x 4096 (64) 17.7 against 18.5, 1024 x 1024 x 4096 (32) 19.0 against 14.3.
+    if (MODE == kDense && p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 64)
+        return pair_product<KIND, P>(p, x, x_scales, s);
     TcArgs a{};
     a.m = p.m;
     a.n = p.n;
@@ -751,8 +754,14 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.group = kGroup;
     a.row_tiles = rt;
     a.per_cta = 1;
-    a.nt = p.m < kGroup ? p.m : kGroup;
+    // 128 columns to a single CTA, two of which share an SM, rather than 256 (bf16 x, 128 x 4096 x 4096: 10.5 us, 15.1);
+    // the pieces of f16 start on scale tiles every 64 tokens
+    constexpr uint32_t kMost = P == 1 ? 128 : 64;
+    a.nt = p.m < kMost ? p.m : kMost;
     const uint32_t tt = (p.m + a.nt - 1) / a.nt;
+    // K over a cluster while that leaves a CTA an SM to itself, and once more where each still streams more than 200 KB
+    // of weights (one token, 8192 x 8192: 2: 11.3 us, 4: 10.0, 8: 15.4; 16 tokens in 4 bits, 4096 x 4096: 2: 6.7, 4: 6.0,
+    // 8: 8.5). More than 32 tokens' sums cost what they save (48 x 4096 x 4096: 1: 9.9, 2: 11.0, 4: 9.5).
     a.split = 1;
     while (a.split < 8 && rt * tt * a.split * 2 <= 148 && a.steps / (a.split * 2) >= 2 && a.nt <= 32) a.split *= 2;
     if (a.split < 8 && rt * tt * a.split * 2 <= 2 * 148 && a.steps / a.split > 24 && a.nt <= 32) a.split *= 2;
