@@ -65,6 +65,7 @@ struct TcArgs {
     uint8_t *h_pieces, *h_scales;
     uint32_t h_steps;         // scale words along a hidden row
     float *partial;
+    bool combine;             // the down product adds the pairs' parts itself
 };
 
 struct Ctrl {
@@ -73,7 +74,8 @@ struct Ctrl {
     uint32_t tmem;
     int abort;
     uint32_t pairs[kChunk], found[4];
-    alignas(16) int32_t rows[kChunk * 4];
+    float weights[kChunk];
+    alignas(16) int32_t rows[kChunk * 3];   // of pieces, at most three to a token
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (MODE == kGateUp) grid_dep_launch();  // every CTA holds its TMEM: the next kernel's may come
+    if (kExperts) grid_dep_launch();  // every CTA holds its TMEM: the next kernel's may come
     const uint32_t tmem = c.tmem, steps = k1 - k0;
 
     // a column's row of pieces; columns past the last token repeat it
@@ -451,6 +453,10 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
         fence_proxy_async();  // read by the tensor core's scale copy
         mbar_arrive(smem_u32(&c.scales_ready));
+        if (MODE == kDown) {
+            if (at < tokens) c.weights[at] = __ldcg(a.weight + c.pairs[at]);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
         if (MODE == kGateUp && blockIdx.x == 0 && rank == 0 && warp == 2) {
             uint32_t *it = a.items + kItemWords * (1 + blockIdx.y);
             if (lane < tokens) it[2 + lane] = c.pairs[lane];
@@ -494,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     // This is done once for all tiles of the CTA: one fence, and a lane to each (tile, token)
     // (a fence and a round of atomics after every tile took 4.4 us a tile, its MMAs 2.2).
     auto part = [&](uint32_t i, float v) {
-        if (row < a.n) a.partial[(size_t)c.pairs[i] * a.n + row] = v * __ldcg(a.weight + c.pairs[i]);
+        if (row < a.n) a.partial[(size_t)c.pairs[i] * a.n + row] = v * c.weights[i];
     };
     auto combine = [&](uint32_t first, uint32_t step) {
         __threadfence();
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
         }
     }
-    if (MODE == kDown && epi && a.split == 1) combine(0, 1);
+    if (MODE == kDown && epi && a.split == 1 && a.combine) combine(0, 1);
     if (a.split > 1) {
         // the cluster's partial tiles, added in rank order through distributed shared memory
         cg::cluster_group cluster = cg::this_cluster();
@@ -604,7 +610,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
         __syncwarp();
         cluster.barrier_arrive();   // this CTA reads the others' shared memory no more
-        if (MODE == kDown && epi) combine(rank, a.split);
+        if (MODE == kDown && epi && a.combine) combine(rank, a.split);
         __syncwarp();
         cluster.barrier_wait();
     }
@@ -654,6 +660,23 @@ __global__ void __launch_bounds__(256) pieces_kernel(const T *x, uint32_t m, uin
             }
         }
     }
+}
+
+// ---- the parts of every token's pairs, added in their order --------------------------------------
+//
+// For many pairs: in the down product nearly every CTA near the end brings last pairs, and its sums, one after
+// another, kept 64 tokens of 8 pairs 13 us longer than this kernel. Few pairs' sums cost less there.
+
+__global__ void __launch_bounds__(128) combine_kernel(const float *partial, uint32_t d, uint32_t top_k, void *y, int type,
+                                                      uint64_t stride) {
+    grid_dep_wait();
+    const uint32_t at = blockIdx.x * 128 + threadIdx.x, t = blockIdx.y;
+    if (at >= d) return;
+    const float *parts = partial + (size_t)t * top_k * d + at;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (uint32_t p = 0; p < top_k; p++) sum += __ldcg(parts + (size_t)p * d);
+    put_as(y, type, t * stride + at, sum);
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -808,6 +831,9 @@ cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
     return e != cudaSuccess ? e : dense<8, P, kDense>(p, pieces, scales, s);
 }
 
+// Whether the down product adds the pairs' parts: 32 pairs or fewer.
+bool mx_combines(const MxExpertsArgs &e) { return e.tokens * e.top_k <= 32; }
+
 template <int P, int MODE>
 cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     const uint32_t width = MODE == kGateUp ? e.d : e.f;
@@ -831,6 +857,7 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.y = e.y;
     a.type = e.type;
     a.stride = e.y_stride;
+    a.combine = mx_combines(e);
     // Tokens to a CTA: 16 where the experts get few, which leaves room for a second accumulator.
     const uint32_t pairs = e.tokens * e.top_k, slots = std::min(e.experts, pairs);
     a.chunk = pairs <= e.experts * 8 ? 16 : kChunk;
@@ -879,8 +906,11 @@ cudaError_t launch_mx4_product(const MxProductArgs &a, cudaStream_t s) {
 }
 
 cudaError_t launch_mx4_expert_products(const MxExpertsArgs &a, cudaStream_t s) {
-    const cudaError_t e = a.type == 1 ? expert_product<3, kGateUp>(a, s) : expert_product<2, kGateUp>(a, s);
-    return e != cudaSuccess ? e : expert_product<kMxHiddenPieces, kDown>(a, s);
+    cudaError_t e = a.type == 1 ? expert_product<3, kGateUp>(a, s) : expert_product<2, kGateUp>(a, s);
+    if (e == cudaSuccess) e = expert_product<kMxHiddenPieces, kDown>(a, s);
+    if (e != cudaSuccess || mx_combines(a)) return e;
+    return launch_pdl(kPdlMx, combine_kernel, dim3((a.d + 127) / 128, a.tokens), 128, 0, s, (const float *)a.ws.partial, a.d, a.top_k,
+                      a.y, a.type, a.y_stride);
 }
 
 int mx_tc_error(bool reset) {
