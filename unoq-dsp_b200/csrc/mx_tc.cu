@@ -733,7 +733,7 @@ cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArg
     return cudaLaunchKernelEx(&cfg, kernel, wmap, xmap, a);
 }
 
-// Ring depth and shared memory for `per_sm` CTAs on an SM.
+// Ring depth and shared memory for one or two (`per_sm`) CTAs on an SM.
 template <int KIND, int P, int MODE>
 uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t n = up_to(a.nt * P, 8), sub = KIND == 8 ? 1 : 2;
@@ -744,8 +744,7 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     a.d_cols = up_to(a.nt, 8) * P;
     const uint32_t sf_cols = sub * (4 + (a.nt * P > 128 ? 8 : 4));
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
-    const uint32_t budget = (per_sm == 1 ? 226 : per_sm == 2 ? 112 : 74) * 1024 - extra;
-    const uint32_t cols = per_sm == 1 ? 512 : per_sm == 2 ? 256 : 128;
+    const uint32_t budget = (per_sm == 1 ? 226 : 112) * 1024 - extra, cols = per_sm == 1 ? 512 : 256;
     const uint32_t acc_cols = a.d_cols * (a.per_cta > 1 ? 2 : 1);
     a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, (a.steps + a.split - 1) / a.split * a.per_cta});
     if (!experts) {
@@ -868,19 +867,16 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     // save (one token, 4 of 32 experts: 18.1 us without, 18.4 to 19.5 with 2 or 4)
     a.split = 1;
     while (a.split < 8 && a.steps / a.split > 32) a.split *= 2;
-    // Row tiles to a CTA and CTAs to an SM. A CTA's set-up (its tokens, their scales) and end take as long as
-    // 100 to 200 KB of weights, so it takes more tiles once there are enough to go round, up to four of
-    // gate / up and two of down, whose end is longer and is hidden by a third CTA. 64 tokens, 128
-    // experts, d 2048, f 1024, tiles and CTAs for gate / up and down: 1, 2, 1, 2: 136 us; 2, 2, 2, 2: 125;
-    // 4, 2, 2, 2: 122; 4, 2, 2, 3: 118; 4, 2, 4, 2: 127.
-    const uint32_t cols = up_to(a.nt, 8) * P, most = MODE == kGateUp ? 4 : 2;
+    // Row tiles to a CTA: its set-up (its tokens, their scales) takes as long as 100 KB of weights, so it takes up
+    // to four once there are enough to go round. 64 tokens, 128 experts, d 2048, f 1024, tiles of gate / up
+    // and of down to a CTA: 1 and 4: 114 us; 2 and 4: 103; 4 and 1: 108; 4 and 2: 102; 4 and 4: 100; 8 and 8: 99.
+    const uint32_t cols = up_to(a.nt, 8) * P;
     a.per_cta = 1;
-    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < most && a.row_tiles * slots >= 148 * 2 * 2 * a.per_cta) a.per_cta *= 2;
-    const uint32_t per_sm = MODE == kDown && a.split == 1 && cols * (a.per_cta > 1 ? 2 : 1) <= 96 ? 3 : 2;
+    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < 4 && a.row_tiles * slots >= 148 * 2 * a.per_cta) a.per_cta *= 2;
     a.head_bytes = 1024 + (a.steps + a.split - 1) / a.split * kMxScaleTile +
                    (MODE == kGateUp ? up_to(pairs, kMxScaleTile) + a.nt * 512 : 0);
     a.head_bytes = up_to(a.head_bytes, 1024);
-    const uint32_t smem = plan_ring<8, P, MODE>(a, per_sm);
+    const uint32_t smem = plan_ring<8, P, MODE>(a, 2);
     CUtensorMap wmap, xmap;
     cudaError_t r = encode_weights<8>(&wmap, MODE == kGateUp ? e.gate_up_codes : e.down_codes,
                                       (uint64_t)e.experts * a.row_tiles * a.kw);
