@@ -335,7 +335,12 @@ EXPERTS = [  # tokens, d, f, experts, top_k, normalize, type, bias
     (3, 130, 70, 5, 5, False, "f16", False), (7, 333, 129, 60, 3, False, "f16", True), (2, 1024, 384, 8, 1, True, "f16", False),
     (16, 256, 512, 16, 2, True, "bf16", False), (33, 257, 200, 4, 3, True, "bf16", False), (64, 384, 128, 128, 8, True, "bf16", False),
     (64, 128, 256, 2, 2, False, "f16", False), (128, 200, 136, 256, 16, True, "bf16", True), (128, 256, 128, 3, 1, True, "f16", False),
-    (5, 1447, 999, 12, 4, True, "bf16", False)]
+    (5, 1447, 999, 12, 4, True, "bf16", False),
+    # long rows: their scales, and so K, spread over a cluster
+    (3, 16384, 64, 2, 2, True, "bf16", False), (2, 40, 16384, 2, 1, True, "f16", False), (128, 4200, 70, 2, 2, True, "bf16", False),
+    (20, 300, 4300, 3, 2, False, "bf16", False),
+    # at most 32 pairs, and just more: the parts are added in the product, or after it
+    (16, 260, 130, 20, 2, True, "bf16", False), (11, 260, 130, 20, 3, True, "bf16", False)]
 
 
 def layer_parts(d, f, e, name, bias, seed):
@@ -435,6 +440,42 @@ def test_experts_outputs_and_refusals(mx):
         mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(gate_up), 2)
     with pytest.raises(ValueError, match="bias"):
         mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2, bias=torch.zeros(5, device="cuda"))
+
+
+# ---- offsets past 32 bits ----------------------------------------------------------------------------
+
+def test_quantize_past_32_bits(mx):
+    """A matrix of more than 2^32 bytes and 2^31 values: its last rows, and rows a long way apart."""
+    rows, k = 36000, 65536
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, k, generator=gen(1), device="cuda").to(torch.bfloat16)
+    x[:2] = torch.randn(2, k, generator=gen(2), device="cuda").to(torch.bfloat16)
+    x[2:-3] = 1.5
+    q = mx.quantize(x)
+    for part in (slice(0, 2), slice(rows - 3, rows)):
+        want = mxref.values(*mxref.stored(x[part]), k)
+        y = q.dequantize(torch.bfloat16)
+        assert torch.equal(y[part].cpu(), want.to(torch.bfloat16)) and bool((y[3:-3:997] == 1.5).all())
+        del y
+    far = torch.empty_strided((2, 64), (2 ** 31 + 8, 1), dtype=torch.bfloat16, device="cuda")
+    far.copy_(torch.randn(2, 64, generator=gen(3), device="cuda"))
+    assert torch.equal(mx.quantize(far).dequantize().cpu(), mxref.values(*mxref.stored(far), 64).to(torch.bfloat16))
+
+
+def test_products_past_32_bits(mx):
+    """Outputs of more than 2^32 bytes, from either activations; the corners against the definition."""
+    m, n, k = 60000, 40000, 64
+    c, s = weights(n // 100, k, 3)
+    w = mx.pack(c.repeat(100, 1).cuda(), s.repeat(100, 1).cuda())
+    x = torch.randn(m, k, generator=gen(4), device="cuda").to(torch.bfloat16)
+    wv = mxref.values(c, s, k)[-8:]
+    for four in (True, False):
+        y = mx.matmul(mx.quantize(x) if four else x, w)
+        for rows in (slice(0, 4), slice(m - 4, m)):
+            a = mxref.values(*mxref.stored(x[rows]), k) if four else x[rows].cpu().double()
+            want = a @ wv.t()
+            assert_within(y[rows, n - 8:], want, mxref.product_bound(a, wv, want, torch.bfloat16) + 1e-6)
+        del y
 
 
 # ---- streams, graphs, a run of them together -------------------------------------------------------

@@ -468,7 +468,9 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     const uint32_t q = warp % 4;
     uint32_t tile = tile0, row = tile0 * 128 + q * 32 + lane;   // of the tile being read
     // [token][128]: a cluster's partial sums, and the gate and up values, which lie in different warps' rows
-    float *red = reinterpret_cast<float *>(MODE == kGateUp ? sfb_all + steps * kMxScaleTile : ring);
+    // (at the same place in every CTA of the cluster, whose shares of K may differ by a step)
+    float *red =
+        reinterpret_cast<float *>(MODE == kGateUp ? sfb_all + (a.steps + a.split - 1) / a.split * kMxScaleTile : ring);
 
     // The hidden value of one of the tile's 64 and its pieces. A warp's 32 are one block along the next
     // product's K. Three pieces keep 12 bits of it: past what x and y hold in either type.
