@@ -285,6 +285,27 @@ def test_matmul_shapes_and_outputs(mx):
     assert (wide[rest] == 3).all()
 
 
+def test_quantised_weights_with_ragged_rows(mx):
+    """A quantised weight is a packed one up to the rows that pad its last tile, which no output shows."""
+    for n, k in ((1, 40), (130, 300), (257, 513), (2433, 64)):
+        w = torch.randn(n, k, generator=gen(n), device="cuda")
+        q, p = mx.quantize(w), mx.pack(*on_gpu(mxref.stored(w)), k=k)
+        for m in (1, 5, 40, 700):
+            x = torch.randn(m, k, generator=gen(m), device="cuda").to(torch.bfloat16)
+            assert torch.equal(mx.matmul(x, q), mx.matmul(x, p))
+            assert torch.equal(mx.matmul(mx.quantize(x), q), mx.matmul(mx.quantize(x), p))
+
+
+def test_an_operand_from_its_bytes(mx):
+    q = mx.quantize(torch.randn(70, 300, generator=gen(1), device="cuda"))
+    again = mx.MX4(q.codes.clone(), q.scales.clone(), 70, 300)
+    x = torch.randn(3, 300, generator=gen(2), device="cuda").to(torch.float16)
+    assert torch.equal(mx.matmul(x, q), mx.matmul(x, again)) and torch.equal(q.dequantize(), again.dequantize())
+    s = mx.quantize(torch.randn(70, 300, generator=gen(1), device="cuda"), layout="stored")
+    assert s.codes.shape == (70, 150) and s.scales.shape == (70, 10)
+    assert torch.equal(mx.pack(s.codes, s.scales).dequantize(), q.dequantize())
+
+
 def test_python_refusals(mx):
     x = torch.randn(4, 64, device="cuda").to(torch.bfloat16)
     W = mx.pack(*on_gpu(weights(16, 64, 1)))
@@ -390,6 +411,20 @@ def test_experts_ties_go_to_the_lowest_index(mx):
     sign = (x.cpu().double() @ router[0].double()) > 0
     for row, up in zip(chosen.tolist(), sign.tolist()):
         assert row == ([7, 0, 1, 2] if up else [0, 1, 2, 3])
+
+
+def test_experts_masked_by_the_bias(mx):
+    """Experts of a bias of minus infinity: chosen last, with no weight; none else is read as a number."""
+    router, gate_up, down, _ = layer_parts(128, 70, 9, "bf16", False, 4)
+    bias = torch.full((9,), -math.inf)
+    bias[[2, 6]] = 0.5
+    x = torch.randn(7, 128, generator=gen(5), device="cuda").to(torch.bfloat16)
+    parts = (router.cuda(), on_gpu(gate_up), on_gpu(down))
+    for norm in (True, False):
+        y, chosen, p = mx.Experts(*parts, 4, norm, bias.cuda())(x, return_choice=True)
+        assert {2, 6} == set(chosen[:, :2].flatten().tolist()) and chosen[:, 2:].tolist() == [[0, 1]] * 7
+        assert (p[:, 2:] == 0).all() and torch.allclose(p.sum(1), torch.ones(7, device="cuda"), atol=2 ** -20)
+        assert torch.equal(y, mx.Experts(*parts, 2, norm, bias.cuda())(x))
 
 
 def test_experts_every_token_to_one_expert(mx):

@@ -68,6 +68,16 @@ int launched(cudaError_t e) {
     return fail(2001, cudaGetErrorString(e));
 }
 
+// A launcher's result; its host bookkeeping may run out of memory, and no exception leaves a C function.
+template <typename F>
+int launch(const F &f) {
+    try {
+        return launched(f());
+    } catch (...) {
+        return fail(2001, "out of host memory");
+    }
+}
+
 // rows x k with so many tiles each: counted in 32 bits by the kernels
 bool sizes_ok(uint64_t rows, uint32_t k) { return k >= 1 && k <= (1u << 30) && rows * uq::mx_ktiles(k) < (1ull << 31); }
 
@@ -134,7 +144,7 @@ int ug_mx4_quantize(const void *x, int type, uint32_t rows, uint32_t k, uint64_t
         return fail(22, "ug_mx4_quantize: operand codes need 128-byte and scales 16-byte alignment");
     OnDevice on;
     if (int rc = on.enter({x, codes, scales})) return rc;
-    return launched(uq::launch_mx4_quantize(x, type, rows, k, stride, layout, codes, scales, static_cast<cudaStream_t>(stream)));
+    return launch([&] { return uq::launch_mx4_quantize(x, type, rows, k, stride, layout, codes, scales, static_cast<cudaStream_t>(stream)); });
 }
 
 int ug_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int layout, uint32_t rows, uint32_t k, void *y,
@@ -149,7 +159,7 @@ int ug_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int layout, u
         return fail(22, "ug_mx4_dequantize: operand codes need 128-byte and scales 16-byte alignment");
     OnDevice on;
     if (int rc = on.enter({codes, scales, y})) return rc;
-    return launched(uq::launch_mx4_dequantize(codes, scales, layout, rows, k, y, type, stride, static_cast<cudaStream_t>(stream)));
+    return launch([&] { return uq::launch_mx4_dequantize(codes, scales, layout, rows, k, y, type, stride, static_cast<cudaStream_t>(stream)); });
 }
 
 uint32_t ug_mx4_pack_rows(uint32_t count, uint32_t rows, int paired) {
@@ -173,7 +183,9 @@ int ug_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_t count, uin
         return fail(22, "ug_mx4_pack: packed codes need 128-byte and scales 16-byte alignment");
     OnDevice on;
     if (int rc = on.enter({codes, scales, packed_codes, packed_scales})) return rc;
-    return launched(uq::launch_mx4_pack(codes, scales, count, rows, k, paired, packed_codes, packed_scales, static_cast<cudaStream_t>(stream)));
+    return launch([&] {
+        return uq::launch_mx4_pack(codes, scales, count, rows, k, paired, packed_codes, packed_scales, static_cast<cudaStream_t>(stream));
+    });
 }
 
 static int product(uq::MxProductArgs &p, void *stream, const char *name) {
@@ -189,7 +201,7 @@ static int product(uq::MxProductArgs &p, void *stream, const char *name) {
         return fail(22, name);
     OnDevice on;
     if (int rc = on.enter({x, p.a_scales, p.w_codes, p.w_scales, p.y, p.workspace})) return rc;
-    return launched(uq::launch_mx4_product(p, static_cast<cudaStream_t>(stream)));
+    return launch([&] { return uq::launch_mx4_product(p, static_cast<cudaStream_t>(stream)); });
 }
 
 int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32_t m, const uint8_t *w_codes,
@@ -286,8 +298,8 @@ int ug_mx4_experts(const UgMx4Experts *layer, const void *x, uint64_t x_stride, 
     a.weights = weights;
     experts_scratch(l, tokens, static_cast<uint8_t *>(workspace), &a.ws);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (int rc = launched(uq::launch_mx4_router(a, s))) return rc;
-    return launched(uq::launch_mx4_expert_products(a, s));
+    if (int rc = launch([&] { return uq::launch_mx4_router(a, s); })) return rc;
+    return launch([&] { return uq::launch_mx4_expert_products(a, s); });
 }
 
 int ug_mx4_check(int device) {
