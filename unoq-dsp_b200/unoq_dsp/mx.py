@@ -22,7 +22,7 @@ from .native import last_error, load_library
 STORED, OPERAND = 0, 1
 MAX_TOKENS = 128
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_HALF = (torch.float16, torch.bfloat16)
+_HALF = {t: _TYPES[t] for t in (torch.float16, torch.bfloat16)}
 
 
 class UgMx4Experts(C.Structure):
@@ -65,21 +65,25 @@ def _input(x, what, types):
     return x
 
 
-def _rows(x, what):
-    """(x as rows of contiguous values, rows, k, row stride); copied only where it has to be."""
+def _rows(x, what, types):
+    """(x as rows of contiguous values, rows, k, row stride, type code); copied only where it has to be."""
+    code = types.get(x.dtype) if isinstance(x, torch.Tensor) and x.is_cuda else None
+    if code is None or x.requires_grad:
+        code = types[_input(x, what, types).dtype]
     if x.dim() != 2:
         if x.dim() < 1 or x.shape[-1] < 1:
             raise ValueError(f"{what} needs at least one value in its last axis")
         x = x.reshape(-1, x.shape[-1])
     rows, k = x.shape
-    if k < 1:
-        raise ValueError(f"{what} needs at least one value in its last axis")
     row, step = x.stride()
     if rows < 2:
         row = k
-    if (step != 1 and k > 1) or row < k:
-        x, row = x.contiguous(), k
-    return x, rows, k, row
+    if step != 1 or row < k or not k:
+        if not k:
+            raise ValueError(f"{what} needs at least one value in its last axis")
+        if k > 1 or row < k:
+            x, row = x.contiguous(), k
+    return x, rows, k, row, code
 
 
 def _row_stride(x, rows, k):
@@ -114,8 +118,8 @@ def _extent(x):
 def _sizes(operand, rows, k):
     """Bytes of the codes and of the scales (ug_mx4_codes_bytes, ug_mx4_scales_bytes)."""
     if operand:
-        tiles = -(-rows // 128) * -(-k // 256)
-        return tiles * 16384, tiles * 1024
+        tiles = (rows + 127 >> 7) * (k + 255 >> 8)
+        return tiles << 14, tiles << 10
     return rows * ((k + 1) // 2), rows * ((k + 31) // 32)
 
 
@@ -142,9 +146,9 @@ class MX4:
     @classmethod
     def _new(cls, rows, k, layout, beside):
         """An unwritten one on the device of `beside`: both arrays in one allocation, the codes first."""
+        self = cls.__new__(cls)
         code_bytes, scale_bytes = _sizes(layout == "operand", rows, k)
         at = (code_bytes + 15) & ~15
-        self = cls.__new__(cls)
         self._data = self._any = data = beside.new_empty(at + scale_bytes, dtype=torch.uint8)
         self.rows, self.k, self.layout, self.device = rows, k, layout, data.device
         self._codes = codes = data.data_ptr()
@@ -177,7 +181,7 @@ class MX4:
         """The values, (rows, k), rounded to ``dtype`` once."""
         if dtype not in _TYPES:
             raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
-        lib, rows, k, device = _library(), self.rows, self.k, self.device
+        lib, rows, k, device = _lib or _library(), self.rows, self.k, self.device
         stride = k
         if out is None:
             out = self._any.new_empty((rows, k), dtype=dtype)
@@ -201,10 +205,10 @@ def quantize(x, layout="operand"):
     """(..., k) values in 32 or 16 bits -> :class:`MX4` of their rows. Each block of 32 gets the scale
     2^(floor(log2 of its largest magnitude) - 2); values go to the nearest e2m1 (ties to even), at
     most 6 scales; a block holding a NaN or an infinity becomes NaN."""
-    x, rows, k, stride = _rows(_input(x, "x", _TYPES), "x")
-    lib, code = _library(), _layout(layout)
+    x, rows, k, stride, code = _rows(x, "x", _TYPES)
+    lib, operand = _lib or _library(), _layout(layout)
     q = MX4._new(rows, k, layout, x)
-    rc = lib.ug_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, stride, code, q._codes, q._scales, _stream(q.device))
+    rc = lib.ug_mx4_quantize(x.data_ptr(), code, rows, k, stride, operand, q._codes, q._scales, _stream(q.device))
     if rc:
         _check(lib, rc, "MX4 quantise")
     return q
@@ -246,7 +250,7 @@ def matmul(a, w, dtype=None, out=None):
     (default: a's, bfloat16 for an MX4). A NaN or an infinity in a block of ``a`` makes its row NaN."""
     if not isinstance(w, MX4) or w.layout != "operand":
         raise ValueError("w must be an MX4 in operand layout (quantize or pack)")
-    lib, n, device = _library(), w.rows, w.device
+    lib, n, device = _lib or _library(), w.rows, w.device
     four = isinstance(a, MX4)
     if four:
         if a.layout != "operand":
@@ -254,10 +258,10 @@ def matmul(a, w, dtype=None, out=None):
         m, k, dtype = a.rows, a.k, dtype or torch.bfloat16
         shape = (m, n)
     else:
-        _input(a, "a", _HALF)
+        values = a
+        a, m, k, a_stride, x_type = _rows(a, "a", _HALF)
         dtype = dtype or a.dtype
-        shape = (*a.shape[:-1], n)
-        a, m, k, a_stride = _rows(a, "a")
+        shape = (m, n) if values is a else (*values.shape[:-1], n)
     if dtype not in _TYPES:
         raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
     if k != w.k or a.device != device:
@@ -273,7 +277,6 @@ def matmul(a, w, dtype=None, out=None):
         rc = lib.ug_mx4_matmul(a._codes, a._scales, m, w._codes, w._scales, n, k, out.data_ptr(), _TYPES[dtype], stride,
                                _stream(device))
     else:
-        x_type = _TYPES[a.dtype]
         need = _need.get((m, k, x_type))
         if need is None:
             if len(_need) > 4096:
@@ -327,16 +330,17 @@ class Experts:
                                    None if bias is None else bias.data_ptr(), self.gate_up[0].data_ptr(),
                                    self.gate_up[1].data_ptr(), self.down[0].data_ptr(), self.down[1].data_ptr())
         self._lib, self._ref, self._need = _library(), C.byref(self._layer), {}
+        self._types = {router.dtype: _TYPES[router.dtype]}
         self.device = router.device
 
     def __call__(self, x, out=None, return_choice=False):
         """(..., d) of the router's type -> the same shape. ``return_choice``: also the chosen experts
         (tokens, top_k) int32, in falling order of their logits, and their float32 weights."""
-        _input(x, "x", (self.router.dtype,))
-        d, device, shape = self.d, self.device, x.shape
-        if not shape or shape[-1] != d or x.device != device:
+        d, device, values = self.d, self.device, x
+        x, t, k, x_stride, _ = _rows(x, "x", self._types)
+        shape = values.shape
+        if k != d or x.device != device:
             raise ValueError(f"x must be (..., {d}) on {device}")
-        x, t, _, x_stride = _rows(x, "x")
         if t > MAX_TOKENS:
             raise ValueError(f"at most {MAX_TOKENS} tokens, not {t}")
         stride = d
