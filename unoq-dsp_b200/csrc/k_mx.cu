@@ -79,11 +79,11 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, c
         c[i] = s[i] = 0;
         if ((uint32_t)i < n) {
             if (OPERAND || (vec_in && j + 8 <= k)) {
-                c[i] = __ldg(reinterpret_cast<const uint32_t *>(from));
+                c[i] = *reinterpret_cast<const uint32_t *>(from);
             } else {
                 for (uint32_t b = 0; b < 4 && j / 2 + b < row_bytes; b++) c[i] |= (uint32_t)from[b] << (8 * b);
             }
-            s[i] = __ldg(sf);
+            s[i] = *sf;
         }
         from += OPERAND ? 128 : row_bytes;
         sf += OPERAND ? 16 : blocks;
@@ -209,8 +209,8 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
 #pragma unroll
                 for (int c = 0; c < 8; c++) {
                     const uint32_t i = i0 + c * 256;
-                    p[c] = i < a.d ? __ldg(reinterpret_cast<const uint4 *>(w + i)) : make_uint4(0, 0, 0, 0);
-                    q[c] = i < a.d ? __ldg(reinterpret_cast<const uint4 *>(x + i)) : make_uint4(0, 0, 0, 0);
+                    p[c] = i < a.d ? *reinterpret_cast<const uint4 *>(w + i) : make_uint4(0, 0, 0, 0);
+                    q[c] = i < a.d ? *reinterpret_cast<const uint4 *>(x + i) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
                 for (int c = 0; c < 8; c++) {

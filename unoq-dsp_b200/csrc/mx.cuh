@@ -127,7 +127,7 @@ struct MxRaw {   // 16-bit types, two to a word
         }
     }
     __device__ __forceinline__ void load(const T *p) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint4 q = *reinterpret_cast<const uint4 *>(p);
         w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
     }
     __device__ __forceinline__ void load_some(const T *p, uint32_t left) {
@@ -152,7 +152,7 @@ struct MxRaw<float> {
         for (int i = 0; i < 8; i++) v[i] = __uint_as_float(w[i]) * scale;
     }
     __device__ __forceinline__ void load(const float *p) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p)), b = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+        const uint4 a = *reinterpret_cast<const uint4 *>(p), b = reinterpret_cast<const uint4 *>(p)[1];
         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
     }
     __device__ __forceinline__ void load_some(const float *p, uint32_t left) {
@@ -240,7 +240,8 @@ __device__ __forceinline__ __nv_bfloat16 mx_to<__nv_bfloat16>(float v) { return 
 
 // Every kernel below is launched programmatically (common.cuh): its first access to memory follows
 // grid_dep_wait(), and it lets the next one start only after that, so a kernel that has started
-// early never meets memory of one before the last.
+// early never meets memory of one before the last. Its loads are plain ones, not __ldg: those are for memory
+// that nobody writes while the kernel runs, and the kernel before may still write when this one starts.
 cudaError_t launch_mx4_quantize(const void *x, int type, uint32_t rows, uint32_t k, uint64_t stride, int layout,
                                 uint8_t *codes, uint8_t *scales, cudaStream_t s);
 cudaError_t launch_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int layout, uint32_t rows, uint32_t k,
