@@ -642,3 +642,25 @@ def test_product_workspace_contents_do_not_matter(mx, native):
         assert rc == 0
         torch.cuda.synchronize()
         assert torch.equal(y, want) and (ws[need:] == fill).all()
+
+
+def test_split_products_on_many_streams(mx):
+    """Short products over clusters whose CTAs share SMs: every one of them gets its tensor memory."""
+    cases = []
+    for i, (m, n, k, four) in enumerate([(1, 8192, 512, False), (16, 4096, 1024, True), (9, 2048, 1024, False), (32, 1024, 2048, True),
+                                         (3, 8192, 768, False), (20, 8192, 1024, True)]):
+        W = mx.pack(*on_gpu(weights(n, k, 40 + i)))
+        x = torch.randn(m, k, generator=gen(40 + i), device="cuda").to(torch.bfloat16)
+        a = mx.quantize(x) if four else x
+        cases.append((a, W, mx.matmul(a, W)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(12)]
+    got = []
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            a, W, want = cases[i % len(cases)]
+            with torch.cuda.stream(s):
+                got.append((mx.matmul(a, W), want))
+    torch.cuda.synchronize()
+    mx.check()
+    assert all(torch.equal(y, want) for y, want in got)

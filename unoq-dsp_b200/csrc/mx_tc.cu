@@ -712,6 +712,10 @@ uint32_t pow2_cols(uint32_t v) {
 
 template <int KIND, int P, int MODE>
 cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, cudaStream_t s) {
+    // A CTA waits for its TMEM without a limit, and a cluster's for each other: with kernels on several streams, CTAs
+    // of two clusters could each hold what the other's lack. So an SM has no more CTAs of clusters than its 512
+    // columns serve: shared memory for two with up to 256 each, or for one.
+    if (a.split > 1) smem = std::max(smem, (a.tmem_cols > 256 ? 116u : 112u) * 1024);
     if (!a.stages || a.tmem_cols > 512 || smem > 227 * 1024) return cudaErrorInvalidConfiguration;
     auto kernel = mx_tc_kernel<KIND, P, MODE>;
     if (!once_per_device(100 + KIND * 16 + P * 4 + MODE, [&] {
