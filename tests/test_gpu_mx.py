@@ -644,6 +644,21 @@ def test_product_workspace_contents_do_not_matter(mx, native):
         assert torch.equal(y, want) and (ws[need:] == fill).all()
 
 
+def test_more_rows_or_values_than_32_bits_count_are_refused(mx):
+    one = torch.ones(1, device="cuda", dtype=torch.bfloat16)
+    W = mx.quantize(one.view(1, 1))
+    for tall in (one.expand(2 ** 32 + 1, 1), one.expand(1, 2 ** 32 + 32), one.expand(2 ** 31, 1)):
+        with pytest.raises(ValueError, match="at most"):
+            mx.quantize(tall, layout="stored")
+        with pytest.raises(ValueError, match="at most"):
+            mx.matmul(tall, W)
+    byte = torch.zeros(1, device="cuda", dtype=torch.uint8)
+    with pytest.raises(ValueError, match="at most"):
+        mx.MX4(byte, byte, 2 ** 32 + 1, 1, layout="stored")
+    with pytest.raises(ValueError, match="at most"):
+        mx.pack(byte.expand(2 ** 32 + 1, 1), byte.expand(2 ** 32 + 1, 1), k=1)
+
+
 def test_split_products_on_many_streams(mx):
     """Short products over clusters whose CTAs share SMs: every one of them gets its tensor memory."""
     cases = []

@@ -21,6 +21,7 @@ from .native import last_error, load_library
 
 STORED, OPERAND = 0, 1
 MAX_TOKENS = 128
+MAX_SIZE = 2 ** 31 - 1   # rows or values of a row: the C calls count them in 32 bits
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _HALF = {t: _TYPES[t] for t in (torch.float16, torch.bfloat16)}
 
@@ -75,6 +76,8 @@ def _rows(x, what, types):
             raise ValueError(f"{what} needs at least one value in its last axis")
         x = x.reshape(-1, x.shape[-1])
     rows, k = x.shape
+    if rows > MAX_SIZE or k > MAX_SIZE:
+        raise ValueError(f"{what} may have at most {MAX_SIZE} rows of as many values")
     row, step = x.stride()
     if rows < 2:
         row = k
@@ -131,8 +134,8 @@ class MX4:
     __slots__ = ("rows", "k", "layout", "device", "_data", "_any", "_codes", "_scales")
 
     def __init__(self, codes, scales, rows, k, layout="operand"):
-        if rows < 0 or k < 1:
-            raise ValueError("rows must be 0 or more and k 1 or more")
+        if not 0 <= rows <= MAX_SIZE or not 1 <= k <= MAX_SIZE:
+            raise ValueError(f"rows must be 0 or more and k 1 or more, at most {MAX_SIZE}")
         for x, want, name in zip((codes, scales), _sizes(_layout(layout), rows, k), ("codes", "scales")):
             _input(x, name, (torch.uint8,))
             if not x.is_contiguous() or x.numel() != want:
@@ -225,6 +228,8 @@ def _stored_pair(codes, scales, k, what):
 
 
 def _pack(codes, scales, count, rows, k, paired):
+    if count * rows > MAX_SIZE or k > MAX_SIZE:
+        raise ValueError(f"a matrix may have at most {MAX_SIZE} rows of as many values")
     lib = _library()
     padded = lib.ug_mx4_pack_rows(count, rows, paired)
     out = [torch.empty(size, dtype=torch.uint8, device=codes.device) for size in _sizes(OPERAND, padded, k)]
