@@ -659,6 +659,35 @@ def test_more_rows_or_values_than_32_bits_count_are_refused(mx):
         mx.pack(byte.expand(2 ** 32 + 1, 1), byte.expand(2 ** 32 + 1, 1), k=1)
 
 
+def test_copies_have_bytes_of_their_own(mx):
+    import copy
+    import pickle
+    x = torch.randn(5, 96, generator=gen(1), device="cuda").to(torch.bfloat16)
+    W = mx.quantize(torch.randn(70, 96, generator=gen(2), device="cuda"))
+    router, gate_up, down, bias = layer_parts(96, 64, 8, "bf16", True, 5)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2, normalize=False, bias=bias.cuda())
+    want = mx.matmul(x, W), layer(x)
+    copies = [(copy.deepcopy(W), copy.deepcopy(layer)), pickle.loads(pickle.dumps((W, layer))), (copy.copy(W), copy.copy(layer))]
+    for w, other in copies[:2]:
+        assert w._codes != W._codes and other._layer.down_codes != layer._layer.down_codes
+    del W, layer, w, other
+    filler = [torch.full((1 << 16,), 255, device="cuda", dtype=torch.uint8) for _ in range(64)]   # what was freed is written over
+    for w, other in copies:
+        assert torch.equal(mx.matmul(x, w), want[0]) and torch.equal(other(x), want[1])
+    del filler
+
+
+def test_an_experts_layer_keeps_its_tensors(mx):
+    router, gate_up, down, _ = layer_parts(96, 64, 8, "bf16", False, 5)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2)
+    x = torch.randn(5, 96, generator=gen(1), device="cuda").to(torch.bfloat16)
+    want = layer(x)
+    layer.router = layer.gate_up = layer.down = None
+    filler = [torch.full((1 << 16,), 255, device="cuda", dtype=torch.uint8) for _ in range(64)]
+    assert torch.equal(layer(x), want)
+    del filler
+
+
 def test_split_products_on_many_streams(mx):
     """Short products over clusters whose CTAs share SMs: every one of them gets its tensor memory."""
     cases = []

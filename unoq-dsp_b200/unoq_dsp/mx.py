@@ -158,6 +158,9 @@ class MX4:
         self._scales = codes + at
         return self
 
+    def __reduce__(self):   # copies and pickles carry the bytes, not this one's addresses
+        return MX4, (self.codes, self.scales, self.rows, self.k, self.layout)
+
     def _views(self):
         if not isinstance(self._data, tuple):
             code_bytes, scale_bytes = _sizes(self.layout == "operand", self.rows, self.k)
@@ -329,14 +332,25 @@ class Experts:
             if x.device != router.device:
                 raise ValueError("the layer's tensors are on two devices")
         self.router, self.bias, self.top_k, self.d, self.f, self.experts = router.contiguous(), bias, top_k, d, f, e
+        self.normalize, self.device = bool(normalize), router.device
         self.gate_up = _pack(gc, gs, e, 2 * f, d, 1)
         self.down = _pack(dc, ds, e, d, f, 0)
-        self._layer = UgMx4Experts(e, top_k, d, f, int(bool(normalize)), _TYPES[router.dtype], self.router.data_ptr(),
-                                   None if bias is None else bias.data_ptr(), self.gate_up[0].data_ptr(),
-                                   self.gate_up[1].data_ptr(), self.down[0].data_ptr(), self.down[1].data_ptr())
-        self._lib, self._ref, self._need = _library(), C.byref(self._layer), {}
-        self._types = {router.dtype: _TYPES[router.dtype]}
-        self.device = router.device
+        self._bind()
+
+    def _bind(self):
+        """The C side's view of the tensors, which it keeps alive whatever becomes of the attributes."""
+        code = _TYPES[self.router.dtype]
+        self._kept = kept = (self.router, self.bias, *self.gate_up, *self.down)
+        self._layer = UgMx4Experts(self.experts, self.top_k, self.d, self.f, self.normalize, code,
+                                   *(None if x is None else x.data_ptr() for x in kept))
+        self._lib, self._ref, self._need, self._types = _library(), C.byref(self._layer), {}, {self.router.dtype: code}
+
+    def __getstate__(self):   # copies and pickles carry the tensors, not this one's addresses
+        return {name: value for name, value in self.__dict__.items() if name[0] != "_"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     def __call__(self, x, out=None, return_choice=False):
         """(..., d) of the router's type -> the same shape. ``return_choice``: also the chosen experts
@@ -352,7 +366,7 @@ class Experts:
         if out is None:
             out = x.new_empty(shape)
         else:
-            _output(out, shape, x.dtype, device, (x, self.router, *self.gate_up, *self.down))
+            _output(out, shape, x.dtype, device, (x, *(kept for kept in self._kept if kept is not None)))
             if out.dim() == 2:
                 stride = _row_stride(out, t, d)
         chosen = weights = None
@@ -362,7 +376,7 @@ class Experts:
         need = self._need.get(t)
         if need is None:
             need = self._need[t] = self._lib.ug_mx4_experts_workspace(self._ref, t)
-        ws = self.down[0].new_empty(need)   # bytes
+        ws = self._kept[-1].new_empty(need)   # bytes
         rc = self._lib.ug_mx4_experts(self._ref, x.data_ptr(), x_stride, t, out.data_ptr(), stride,
                                       chosen.data_ptr() if return_choice else None,
                                       weights.data_ptr() if return_choice else None, ws.data_ptr(), need, _stream(device))
@@ -373,6 +387,7 @@ class Experts:
 
 def check(device=None):
     """Wait for the device; raise DSPError if a kernel failed or ran out of its bounded waits."""
-    device = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    device = None if device is None else torch.device(device).index
+    device = torch.cuda.current_device() if device is None else device
     lib = _library()
     _check(lib, lib.ug_mx4_check(device), "MX4 check")
