@@ -57,7 +57,8 @@ struct TcArgs {
     uint64_t x_stride;
     bool x_vec;
     // experts
-    uint32_t top_k, per_cta, chunk, head_bytes;   // head: the choices, the columns' scales, gate and up values
+    uint32_t top_k, chunk, head_bytes;   // head: the choices, the columns' scales, gate and up values
+    bool shared;              // the items' tiles are dealt out evenly to the CTAs (grid.x); else grid: tile, item, K
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     const uint32_t rank = blockIdx.z;
     volatile int *abort = &c.abort;
 
-    if (threadIdx.x == 0) {
+    auto init_barriers = [&] {
         for (uint32_t i = 0; i < kMaxStages; i++) {
             mbar_init(smem_u32(&c.full[i]), 2);
             mbar_init(smem_u32(&c.empty[i]), 1);
@@ -110,47 +111,45 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         mbar_init(smem_u32(&c.spare), 1);
         mbar_init(smem_u32(&c.rows_ready), 128);
         mbar_init(smem_u32(&c.scales_ready), 128);
-        c.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    };
+    auto drop_barriers = [&] {   // before they are set up anew
+        for (uint32_t b = smem_u32(&c.full[0]); b <= smem_u32(&c.spare); b += 8)
+            asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(b) : "memory");
+    };
+    if (threadIdx.x == 0) {
+        init_barriers();
+        c.abort = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmap)) : "memory");
     }
 
     // ---- what this CTA computes ----
-    const uint32_t tile0 = blockIdx.x * a.per_cta, tiles = min(a.per_cta, a.row_tiles - tile0);
-    uint32_t w_tile = tile0;
-    uint32_t tokens, tok0 = 0, expert = 0, chunk = 0;  // columns: tokens, or a chunk of one expert's pairs
+    uint32_t tile0 = blockIdx.x, tiles = 1, w_tile = tile0;
+    uint32_t tokens = 0, tok0 = 0, expert = 0, chunk = 0;   // columns: tokens, or a chunk of one expert's pairs
     uint32_t mine = 0;                                 // lanes (pairs) of the expert, where one warp holds all pairs
     const uint32_t k0 = a.steps * rank / a.split, k1 = a.steps * (rank + 1) / a.split;
     const uint32_t pairs = kExperts ? a.m * a.top_k : 0;
     const bool one_warp = MODE == kGateUp && pairs <= 32 && a.m <= a.chunk;
+    // Work items: every chosen expert's tokens in chunks. The gate / up product finds its items from the
+    // choices themselves and leaves the list to the down product. A CTA takes the tiles [unit, unit_end) of all
+    // items' tiles in a row, one item after another.
+    uint32_t item = 0, unit = 0, unit_end = 1, total = 0;
+    uint32_t id = 0, same = 0, firsts = 0;             // one_warp: the lane's choice, the lanes of the same and of firsts
     if constexpr (!kExperts) {
         tok0 = blockIdx.y * a.nt;
         tokens = min(a.nt, a.m - tok0);
     } else {
-        // Work items: every chosen expert's tokens in chunks. The gate / up product finds its item from the
-        // choices themselves and leaves the list to the down product.
-        const uint32_t item = blockIdx.y;
-        if constexpr (MODE == kDown) {
+        if (MODE == kDown) {
             grid_dep_wait();  // the items and the hidden vectors
-            const uint32_t *it = a.items + kItemWords * (1 + item);
-            const uint32_t total = __ldcg(a.items), of = __ldcg(it), pair = __ldcg(it + 2 + lane);
-            tokens = __ldcg(it + 1);
-            if (item >= total) return;
-            expert = of;
-            if (warp == 2) c.pairs[lane] = pair;
+            total = __ldcg(a.items);
         } else if (one_warp) {
             // few pairs: a lane each in every warp, experts in the order of their first choice
             grid_dep_wait();  // the router's choice
-            const uint32_t id = (uint32_t)lane < pairs ? (uint32_t)__ldcg(a.chosen + lane) : 0xFFFFu;
-            const uint32_t same = __match_any_sync(~0u, id);
-            const uint32_t firsts = __ballot_sync(~0u, (uint32_t)lane < pairs && __ffs(same) - 1 == lane);
-            if (item == 0 && blockIdx.x == 0 && rank == 0 && threadIdx.x == 0) a.items[0] = __popc(firsts);
-            if (item >= __popc(firsts)) return;  // the same in the whole cluster
-            const int first = (int)__fns(firsts, 0, (int)item + 1);
-            expert = __shfl_sync(~0u, id, first);
-            mine = __shfl_sync(~0u, same, first);
-            tokens = __popc(mine);
+            id = (uint32_t)lane < pairs ? (uint32_t)__ldcg(a.chosen + lane) : 0xFFFFu;
+            same = __match_any_sync(~0u, id);
+            firsts = __ballot_sync(~0u, (uint32_t)lane < pairs && __ffs(same) - 1 == lane);
+            total = __popc(firsts);
         } else {
             // experts in order, counted in shared memory
             for (uint32_t i = threadIdx.x; i < 256; i += kThreads) counts[i] = 0;
@@ -163,7 +162,41 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 atomicAdd(&counts[e % 256], 1u);
             }
             __syncthreads();
-            uint32_t n[8], items = 0;   // every warp on its own: a lane has eight experts
+#pragma unroll
+            for (int i = 0; i < 8; i++) total += (counts[lane * 8 + i] + a.chunk - 1) / a.chunk;
+            total = __reduce_add_sync(~0u, total);
+        }
+        if (MODE == kGateUp && blockIdx.x == 0 && blockIdx.y == 0 && rank == 0 && threadIdx.x == 0) a.items[0] = total;
+        if (a.shared) {
+            const uint32_t units = total * a.row_tiles;
+            unit = units * blockIdx.x / gridDim.x;
+            unit_end = units * (blockIdx.x + 1) / gridDim.x;
+            if (unit == unit_end) return;
+        } else {
+            if (blockIdx.y >= total) return;  // the same in the whole cluster
+            unit = blockIdx.y * a.row_tiles + blockIdx.x;
+            unit_end = unit + 1;
+        }
+    }
+    // the next item of the CTA: its expert, tokens and tiles
+    auto next_item = [&] {
+        item = unit / a.row_tiles;
+        tile0 = unit - item * a.row_tiles;
+        tiles = min(a.row_tiles - tile0, unit_end - unit);
+        unit += tiles;
+        if (MODE == kDown) {
+            const uint32_t *it = a.items + kItemWords * (1 + item);
+            const uint32_t of = __ldcg(it), pair = __ldcg(it + 2 + lane);
+            tokens = __ldcg(it + 1);
+            expert = of;
+            if (warp == 2) c.pairs[lane] = pair;
+        } else if (one_warp) {
+            const int first = (int)__fns(firsts, 0, (int)item + 1);
+            expert = __shfl_sync(~0u, id, first);
+            mine = __shfl_sync(~0u, same, first);
+            tokens = __popc(mine);
+        } else {   // every warp on its own: a lane has eight experts
+            uint32_t n[8], items = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 n[i] = counts[lane * 8 + i];
@@ -175,9 +208,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 const uint32_t below = __shfl_up_sync(~0u, upto, o);
                 if (lane >= o) upto += below;
             }
-            if (item == 0 && blockIdx.x == 0 && rank == 0 && threadIdx.x == 31) a.items[0] = upto;
-            const uint32_t holders = __ballot_sync(~0u, item < upto);
-            if (!holders) return;
+            const int holder = __ffs(__ballot_sync(~0u, item < upto)) - 1;   // there is one: item < total
             uint32_t left = item - (upto - items), found = 0, here = 0;
             bool open = true;
 #pragma unroll
@@ -190,20 +221,24 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 }
                 if (open) left -= chunks;
             }
-            const int holder = __ffs(holders) - 1;
             expert = __shfl_sync(~0u, found, holder);
             chunk = __shfl_sync(~0u, left, holder);
             tokens = min(__shfl_sync(~0u, here, holder) - chunk * a.chunk, a.chunk);
         }
         w_tile = expert * a.row_tiles + tile0;
-    }
-    const uint32_t n_cols = (tokens * P + 7) / 8 * 8;
-    const uint32_t col_tiles = kExperts ? 1 : (n_cols + 127) / 128;
+    };
+    if (kExperts) next_item();
+    const uint32_t accs = a.shared ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
+    uint32_t n_cols, b_bytes, stage_bytes, stages;
     const uint32_t sfb_cols = a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
-    // the experts' ring is as deep as this expert's few tokens allow
-    const uint32_t b_bytes = kExperts ? n_cols * 128 : a.b_bytes;
-    const uint32_t stage_bytes = kExperts ? kA + b_bytes + 1024 : a.stage_bytes;
-    const uint32_t stages = kExperts ? min(a.stages, a.ring_bytes / stage_bytes) : a.stages;
+    auto shape_ring = [&] {   // the experts' ring is as deep as this expert's few tokens allow
+        n_cols = (tokens * P + 7) / 8 * 8;
+        b_bytes = kExperts ? n_cols * 128 : a.b_bytes;
+        stage_bytes = kExperts ? kA + b_bytes + 1024 : a.stage_bytes;
+        stages = kExperts ? min(a.stages, a.ring_bytes / stage_bytes) : a.stages;
+    };
+    shape_ring();
+    const uint32_t col_tiles = kExperts ? 1 : (n_cols + 127) / 128;
 
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
@@ -228,6 +263,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
     };
 
+    for (;;) {   // items; a dense product is one
     if (warp == 0 && elect_one()) {
         // ---- weight tiles and their scales, in the order of memory ----
         // The kernel before may be any, one that writes the weights too; but the one that makes pieces has seen
@@ -251,6 +287,12 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 st += stage_bytes, full += 8, empty += 8;
                 if (++s == stages) s = 0, phase ^= 1, st = st0, full = full0, empty = empty0;
             }
+        }
+        // before a next item sets the barriers up anew: the MMAs' arrivals on all of these
+        for (uint32_t i = 0; kExperts && unit != unit_end && i < stages; i++) {
+            if (!mbar_poll(empty, phase, abort, 603)) break;
+            empty += 8;
+            if (++s == stages) s = 0, phase ^= 1, empty = empty0;
         }
     weights_out:
         if (*abort) drain(issued);
@@ -312,7 +354,6 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
     } else if (warp == 1 && elect_one()) {
         // ---- MMA ----
-        const uint32_t accs = tiles > 1 ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
         const uint32_t sf_tmem = tmem + a.d_cols * accs, idesc = scaled_instr_desc<KIND>(128, n_cols);
         const uint32_t st0 = smem_u32(ring), full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
         // each stage has scale columns of its own: they are rewritten only after its MMAs are done
@@ -457,8 +498,8 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             if (at < tokens) c.weights[at] = __ldcg(a.weight + c.pairs[at]);
             asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        if (MODE == kGateUp && blockIdx.x == 0 && rank == 0 && warp == 2) {
-            uint32_t *it = a.items + kItemWords * (1 + blockIdx.y);
+        if (MODE == kGateUp && tile0 == 0 && rank == 0 && warp == 2) {
+            uint32_t *it = a.items + kItemWords * (1 + item);
             if (lane < tokens) it[2 + lane] = c.pairs[lane];
             if (lane == 0) it[0] = expert, it[1] = tokens;
         }
@@ -616,6 +657,22 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         __syncwarp();
         cluster.barrier_wait();
     }
+    if (!kExperts || unit == unit_end) break;
+    // The next item, once this one's tiles are out. All its copies and MMAs have been waited for, or the CTA gives up.
+    __syncthreads();
+    tc_fence_after();
+    const bool give_up = *abort;
+    if (threadIdx.x == 0) {
+        drop_barriers();
+        init_barriers();
+    }
+    next_item();
+    shape_ring();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (give_up) break;
+    }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
@@ -751,8 +808,9 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t sf_cols = sub * (4 + (a.nt * P > 128 ? 8 : 4));
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
     const uint32_t budget = (per_sm == 1 ? 226 : 112) * 1024 - extra, cols = per_sm == 1 ? 512 : 256;
-    const uint32_t acc_cols = a.d_cols * (a.per_cta > 1 ? 2 : 1);
-    a.stages = std::min({(cols - acc_cols) / sf_cols, (uint32_t)kMaxStages, (a.steps + a.split - 1) / a.split * a.per_cta});
+    const uint32_t acc_cols = a.d_cols * (a.shared ? 2 : 1);
+    a.stages = std::min((cols - acc_cols) / sf_cols, (uint32_t)kMaxStages);
+    if (!a.shared) a.stages = std::min(a.stages, (a.steps + a.split - 1) / a.split);
     if (!experts) {
         a.stages = std::min(a.stages, budget / a.stage_bytes);
         a.ring_bytes = a.stages * a.stage_bytes;
@@ -781,7 +839,6 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.steps = KIND == 8 ? mx_tiles(p.k) : kw;
     a.group = kGroup;
     a.row_tiles = rt;
-    a.per_cta = 1;
     // 128 columns to a single CTA, two of which share an SM, rather than 256 (bf16 x, 128 x 4096 x 4096: 10.5 us, 15.1);
     // the pieces of f16 start on scale tiles every 64 tokens
     constexpr uint32_t kMost = P == 1 ? 128 : 64;
@@ -873,12 +930,9 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     // save (one token, 4 of 32 experts: 18.1 us without, 18.4 to 19.5 with 2 or 4)
     a.split = 1;
     while (a.split < 8 && a.steps / a.split > 32) a.split *= 2;
-    // Row tiles to a CTA: its set-up (its tokens, their scales) takes as long as 100 KB of weights, so it takes up
-    // to four once there are enough to go round. 64 tokens, 128 experts, d 2048, f 1024, tiles of gate / up
-    // and of down to a CTA: 1 and 4: 114 us; 2 and 4: 103; 4 and 1: 108; 4 and 2: 102; 4 and 4: 100; 8 and 8: 99.
-    const uint32_t cols = up_to(a.nt, 8) * P;
-    a.per_cta = 1;
-    while (a.split == 1 && cols * 2 <= 200 && a.per_cta < 4 && a.row_tiles * slots >= 148 * 2 * a.per_cta) a.per_cta *= 2;
+    // Two CTAs to an SM share all items' tiles evenly once there can be more than one each.
+    const uint32_t slots_ctas = 2 * (uint32_t)current_sm_count();
+    a.shared = a.split == 1 && a.row_tiles * slots > slots_ctas;
     a.head_bytes = 1024 + (a.steps + a.split - 1) / a.split * kMxScaleTile +
                    (MODE == kGateUp ? up_to(pairs, kMxScaleTile) + a.nt * 512 : 0);
     a.head_bytes = up_to(a.head_bytes, 1024);
@@ -891,7 +945,8 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.steps * 128,
                piece_rows, (uint64_t)a.steps * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
-    return launch<8, P, MODE>(wmap, xmap, a, dim3((a.row_tiles + a.per_cta - 1) / a.per_cta, items, a.split), smem, s);
+    const dim3 grid = a.shared ? dim3(slots_ctas) : dim3(a.row_tiles, items, a.split);
+    return launch<8, P, MODE>(wmap, xmap, a, grid, smem, s);
 }
 
 }  // namespace
