@@ -708,3 +708,15 @@ def test_split_products_on_many_streams(mx):
     torch.cuda.synchronize()
     mx.check()
     assert all(torch.equal(y, want) for y, want in got)
+
+
+@pytest.mark.parametrize("t,d,f,e,top,norm,name,with_bias", [
+    # of gate and up
+    (8, 130, 1000, 20, 4, True, "bf16", False), (1, 100, 1300, 16, 16, False, "f16", True), (90, 256, 4500, 6, 2, True, "bf16", True),
+    # of down: added there, and after it
+    (8, 2000, 130, 20, 4, True, "bf16", False), (40, 2600, 70, 16, 3, True, "f16", False),
+    # of both
+    (128, 640, 420, 64, 4, False, "bf16", False)])
+def test_experts_with_more_tiles_than_ctas(mx, t, d, f, e, top, norm, name, with_bias):
+    """Every CTA takes several tiles, and goes on from one expert to the next."""
+    test_experts(mx, t, d, f, e, top, norm, name, with_bias)

@@ -58,7 +58,7 @@ struct TcArgs {
     bool x_vec;
     // experts
     uint32_t top_k, chunk, head_bytes;   // head: the choices, the columns' scales, gate and up values
-    bool shared;              // the items' tiles are dealt out evenly to the CTAs (grid.x); else grid: tile, item, K
+    bool shared;              // SHARED
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
@@ -80,7 +80,8 @@ struct Ctrl {
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 
-template <int KIND, int P, int MODE>
+// SHARED: the items' tiles are dealt out evenly to the CTAs (grid.x); else the grid is tile, item, K.
+template <int KIND, int P, int MODE, bool SHARED>
 __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__ CUtensorMap wmap,
                                                          const __grid_constant__ CUtensorMap xmap, const TcArgs a) {
     constexpr bool kExperts = MODE == kGateUp || MODE == kDown;
@@ -132,9 +133,9 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     const uint32_t pairs = kExperts ? a.m * a.top_k : 0;
     const bool one_warp = MODE == kGateUp && pairs <= 32 && a.m <= a.chunk;
     // Work items: every chosen expert's tokens in chunks. The gate / up product finds its items from the
-    // choices themselves and leaves the list to the down product. A CTA takes the tiles [unit, unit_end) of all
-    // items' tiles in a row, one item after another.
-    uint32_t item = 0, unit = 0, unit_end = 1, total = 0;
+    // choices themselves and leaves the list to the down product. SHARED: a CTA takes the tiles [unit, unit_end) of
+    // all items' tiles in a row, one item after another.
+    uint32_t item = blockIdx.y, unit = 0, unit_end = 0, total = 0;
     uint32_t id = 0, same = 0, firsts = 0;             // one_warp: the lane's choice, the lanes of the same and of firsts
     if constexpr (!kExperts) {
         tok0 = blockIdx.y * a.nt;
@@ -167,23 +168,8 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             total = __reduce_add_sync(~0u, total);
         }
         if (MODE == kGateUp && blockIdx.x == 0 && blockIdx.y == 0 && rank == 0 && threadIdx.x == 0) a.items[0] = total;
-        if (a.shared) {
-            const uint32_t units = total * a.row_tiles;
-            unit = units * blockIdx.x / gridDim.x;
-            unit_end = units * (blockIdx.x + 1) / gridDim.x;
-            if (unit == unit_end) return;
-        } else {
-            if (blockIdx.y >= total) return;  // the same in the whole cluster
-            unit = blockIdx.y * a.row_tiles + blockIdx.x;
-            unit_end = unit + 1;
-        }
     }
-    // the next item of the CTA: its expert, tokens and tiles
-    auto next_item = [&] {
-        item = unit / a.row_tiles;
-        tile0 = unit - item * a.row_tiles;
-        tiles = min(a.row_tiles - tile0, unit_end - unit);
-        unit += tiles;
+    auto find = [&] {   // the item's expert and tokens
         if (MODE == kDown) {
             const uint32_t *it = a.items + kItemWords * (1 + item);
             const uint32_t of = __ldcg(it), pair = __ldcg(it + 2 + lane);
@@ -227,8 +213,25 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         }
         w_tile = expert * a.row_tiles + tile0;
     };
-    if (kExperts) next_item();
-    const uint32_t accs = a.shared ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
+    auto next_item = [&] {
+        item = unit / a.row_tiles;
+        tile0 = unit - item * a.row_tiles;
+        tiles = min(a.row_tiles - tile0, unit_end - unit);
+        unit += tiles;
+        find();
+    };
+    if (SHARED) {
+        const uint32_t units = total * a.row_tiles;
+        unit = units * blockIdx.x / gridDim.x;
+        unit_end = units * (blockIdx.x + 1) / gridDim.x;
+        if (unit == unit_end) return;
+        next_item();
+    } else if (kExperts) {
+        if (MODE == kDown) find();   // its loads go out with the total's; past that they read the list's unused places
+        if (item >= total) return;   // the same in the whole cluster
+        if (MODE != kDown) find();
+    }
+    constexpr uint32_t accs = SHARED ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
     uint32_t n_cols, b_bytes, stage_bytes, stages;
     const uint32_t sfb_cols = a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
     auto shape_ring = [&] {   // the experts' ring is as deep as this expert's few tokens allow
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
         }
         // before a next item sets the barriers up anew: the MMAs' arrivals on all of these
-        for (uint32_t i = 0; kExperts && unit != unit_end && i < stages; i++) {
+        for (uint32_t i = 0; SHARED && unit != unit_end && i < stages; i++) {
             if (!mbar_poll(empty, phase, abort, 603)) break;
             empty += 8;
             if (++s == stages) s = 0, phase ^= 1, empty = empty0;
@@ -657,7 +660,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         __syncwarp();
         cluster.barrier_wait();
     }
-    if (!kExperts || unit == unit_end) break;
+    if (!SHARED || unit == unit_end) break;
     // The next item, once this one's tiles are out. All its copies and MMAs have been waited for, or the CTA gives up.
     __syncthreads();
     tc_fence_after();
@@ -767,15 +770,15 @@ uint32_t pow2_cols(uint32_t v) {
 
 #include "mx_pair.cuh"
 
-template <int KIND, int P, int MODE>
+template <int KIND, int P, int MODE, bool SHARED = false>
 cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, cudaStream_t s) {
     // A CTA waits for its TMEM without a limit, and a cluster's for each other: with kernels on several streams, CTAs
     // of two clusters could each hold what the other's lack. So an SM has no more CTAs of clusters than its 512
     // columns serve: shared memory for two with up to 256 each, or for one.
     if (a.split > 1) smem = std::max(smem, (a.tmem_cols > 256 ? 116u : 112u) * 1024);
     if (!a.stages || a.tmem_cols > 512 || smem > 227 * 1024) return cudaErrorInvalidConfiguration;
-    auto kernel = mx_tc_kernel<KIND, P, MODE>;
-    if (!once_per_device(100 + KIND * 16 + P * 4 + MODE, [&] {
+    auto kernel = mx_tc_kernel<KIND, P, MODE, SHARED>;
+    if (!once_per_device(100 + SHARED * 200 + KIND * 16 + P * 4 + MODE, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess;
         }))
         return cudaErrorInvalidValue;
@@ -945,8 +948,8 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.steps * 128,
                piece_rows, (uint64_t)a.steps * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
-    const dim3 grid = a.shared ? dim3(slots_ctas) : dim3(a.row_tiles, items, a.split);
-    return launch<8, P, MODE>(wmap, xmap, a, grid, smem, s);
+    if (a.shared) return launch<8, P, MODE, true>(wmap, xmap, a, dim3(slots_ctas), smem, s);
+    return launch<8, P, MODE>(wmap, xmap, a, dim3(a.row_tiles, items, a.split), smem, s);
 }
 
 }  // namespace
