@@ -57,8 +57,8 @@ struct TcArgs {
     uint64_t x_stride;
     bool x_vec;
     // experts
-    uint32_t top_k, chunk, head_bytes;   // head: the choices, the columns' scales, gate and up values
-    bool shared;              // SHARED
+    uint32_t top_k, per_cta, chunk, head_bytes;   // per_cta: row tiles (kSome); head: the choices, the columns' scales, gate and up values
+    bool shared;              // kShared
     const int32_t *chosen;
     const float *weight;
     uint32_t *arrived;
@@ -80,11 +80,13 @@ struct Ctrl {
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 
-// SHARED: the items' tiles are dealt out evenly to the CTAs (grid.x); else the grid is tile, item, K.
-template <int KIND, int P, int MODE, bool SHARED>
+// DEAL: which row tiles a CTA of the experts takes: one, or up to per_cta, of an item, the grid being tiles, item, K; or
+// its part of all items' tiles in a row (grid.x). A kernel each: the loops cost the one-tile kernel 0.3 us of 17.
+enum Deal { kOne = 0, kSome = 1, kShared = 2 };
+template <int KIND, int P, int MODE, int DEAL>
 __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__ CUtensorMap wmap,
                                                          const __grid_constant__ CUtensorMap xmap, const TcArgs a) {
-    constexpr bool kExperts = MODE == kGateUp || MODE == kDown;
+    constexpr bool kExperts = MODE == kGateUp || MODE == kDown, kDealt = DEAL == kShared;
     constexpr uint32_t kSub = KIND == 8 ? 1 : 2;                  // scale tiles of a stage, per 128 rows
     constexpr uint32_t kSf = kSub * kMxScaleTile;
     constexpr uint32_t kWeightTx = (KIND == 8 ? kMxCodeTile / 2 : kMxCodeTile) + kSf;  // an unpacking copy counts what it reads
@@ -126,14 +128,15 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     }
 
     // ---- what this CTA computes ----
-    uint32_t tile0 = blockIdx.x, tiles = 1, w_tile = tile0;
+    uint32_t tile0 = DEAL == kSome ? blockIdx.x * a.per_cta : blockIdx.x, w_tile = tile0;
+    uint32_t tiles = DEAL == kSome ? min(a.per_cta, a.row_tiles - tile0) : 1;
     uint32_t tokens = 0, tok0 = 0, expert = 0, chunk = 0;   // columns: tokens, or a chunk of one expert's pairs
     uint32_t mine = 0;                                 // lanes (pairs) of the expert, where one warp holds all pairs
     const uint32_t k0 = a.steps * rank / a.split, k1 = a.steps * (rank + 1) / a.split;
     const uint32_t pairs = kExperts ? a.m * a.top_k : 0;
     const bool one_warp = MODE == kGateUp && pairs <= 32 && a.m <= a.chunk;
     // Work items: every chosen expert's tokens in chunks. The gate / up product finds its items from the
-    // choices themselves and leaves the list to the down product. SHARED: a CTA takes the tiles [unit, unit_end) of
+    // choices themselves and leaves the list to the down product. kShared: a CTA takes the tiles [unit, unit_end) of
     // all items' tiles in a row, one item after another.
     uint32_t item = blockIdx.y, unit = 0, unit_end = 0, total = 0;
     uint32_t id = 0, same = 0, firsts = 0;             // one_warp: the lane's choice, the lanes of the same and of firsts
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         unit += tiles;
         find();
     };
-    if (SHARED) {
+    if (kDealt) {
         const uint32_t units = total * a.row_tiles;
         unit = units * blockIdx.x / gridDim.x;
         unit_end = units * (blockIdx.x + 1) / gridDim.x;
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         if (item >= total) return;   // the same in the whole cluster
         if (MODE != kDown) find();
     }
-    constexpr uint32_t accs = SHARED ? 2 : 1;   // accumulators: the epilogue reads one while the next fills
+    constexpr uint32_t accs = DEAL == kOne ? 1 : 2;   // accumulators: the epilogue reads one while the next fills
     uint32_t n_cols, b_bytes, stage_bytes, stages;
     const uint32_t sfb_cols = a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
     auto shape_ring = [&] {   // the experts' ring is as deep as this expert's few tokens allow
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
     };
 
-    for (;;) {   // items; a dense product is one
+    for (;;) {   // items (a dense product is one); the body is not indented for it
     if (warp == 0 && elect_one()) {
         // ---- weight tiles and their scales, in the order of memory ----
         // The kernel before may be any, one that writes the weights too; but the one that makes pieces has seen
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             }
         }
         // before a next item sets the barriers up anew: the MMAs' arrivals on all of these
-        for (uint32_t i = 0; SHARED && unit != unit_end && i < stages; i++) {
+        for (uint32_t i = 0; kDealt && unit != unit_end && i < stages; i++) {
             if (!mbar_poll(empty, phase, abort, 603)) break;
             empty += 8;
             if (++s == stages) s = 0, phase ^= 1, empty = empty0;
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         __syncwarp();
         cluster.barrier_wait();
     }
-    if (!SHARED || unit == unit_end) break;
+    if (!kDealt || unit == unit_end) break;
     // The next item, once this one's tiles are out. All its copies and MMAs have been waited for, or the CTA gives up.
     __syncthreads();
     tc_fence_after();
@@ -770,15 +773,15 @@ uint32_t pow2_cols(uint32_t v) {
 
 #include "mx_pair.cuh"
 
-template <int KIND, int P, int MODE, bool SHARED = false>
+template <int KIND, int P, int MODE, int DEAL = kOne>
 cudaError_t launch(const CUtensorMap &wmap, const CUtensorMap &xmap, const TcArgs &a, dim3 grid, uint32_t smem, cudaStream_t s) {
     // A CTA waits for its TMEM without a limit, and a cluster's for each other: with kernels on several streams, CTAs
     // of two clusters could each hold what the other's lack. So an SM has no more CTAs of clusters than its 512
     // columns serve: shared memory for two with up to 256 each, or for one.
     if (a.split > 1) smem = std::max(smem, (a.tmem_cols > 256 ? 116u : 112u) * 1024);
     if (!a.stages || a.tmem_cols > 512 || smem > 227 * 1024) return cudaErrorInvalidConfiguration;
-    auto kernel = mx_tc_kernel<KIND, P, MODE, SHARED>;
-    if (!once_per_device(100 + SHARED * 200 + KIND * 16 + P * 4 + MODE, [&] {
+    auto kernel = mx_tc_kernel<KIND, P, MODE, DEAL>;
+    if (!once_per_device(100 + DEAL * 200 + KIND * 16 + P * 4 + MODE, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess;
         }))
         return cudaErrorInvalidValue;
@@ -811,9 +814,9 @@ uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t sf_cols = sub * (4 + (a.nt * P > 128 ? 8 : 4));
     const uint32_t extra = 1024 + kCtrlBytes + a.head_bytes;
     const uint32_t budget = (per_sm == 1 ? 226 : 112) * 1024 - extra, cols = per_sm == 1 ? 512 : 256;
-    const uint32_t acc_cols = a.d_cols * (a.shared ? 2 : 1);
+    const uint32_t acc_cols = a.d_cols * (a.shared || a.per_cta > 1 ? 2 : 1);
     a.stages = std::min((cols - acc_cols) / sf_cols, (uint32_t)kMaxStages);
-    if (!a.shared) a.stages = std::min(a.stages, (a.steps + a.split - 1) / a.split);
+    if (!a.shared) a.stages = std::min(a.stages, (a.steps + a.split - 1) / a.split * a.per_cta);
     if (!experts) {
         a.stages = std::min(a.stages, budget / a.stage_bytes);
         a.ring_bytes = a.stages * a.stage_bytes;
@@ -842,6 +845,7 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
     a.steps = KIND == 8 ? mx_tiles(p.k) : kw;
     a.group = kGroup;
     a.row_tiles = rt;
+    a.per_cta = 1;
     // 128 columns to a single CTA, two of which share an SM, rather than 256 (bf16 x, 128 x 4096 x 4096: 10.5 us, 15.1);
     // the pieces of f16 start on scale tiles every 64 tokens
     constexpr uint32_t kMost = P == 1 ? 128 : 64;
@@ -933,9 +937,13 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     // save (one token, 4 of 32 experts: 18.1 us without, 18.4 to 19.5 with 2 or 4)
     a.split = 1;
     while (a.split < 8 && a.steps / a.split > 32) a.split *= 2;
-    // Two CTAs to an SM share all items' tiles evenly once there can be more than one each.
-    const uint32_t slots_ctas = 2 * (uint32_t)current_sm_count();
-    a.shared = a.split == 1 && a.row_tiles * slots > slots_ctas;
+    // A round of CTAs is two to an SM. Up to four tiles of an item to each while one round holds all items there can be;
+    // more tiles are dealt out evenly, from one item on to the next, which costs 4 us for each change of items
+    // (bf16, 4 of 32 experts, d 2048, f 1024, two tiles to a CTA: 16 tokens 33 us, dealt out 39; 8 of 128, four tiles: 8
+    // tokens 46, dealt out 50; seven: 16 tokens 67 dealt out, 75 in rounds of four tiles, and 64 tokens 97 and 100).
+    const uint32_t ctas = 2 * (uint32_t)current_sm_count(), each = (a.row_tiles * slots + ctas - 1) / ctas;
+    a.shared = a.split == 1 && each > 4;
+    a.per_cta = a.split == 1 && !a.shared ? each : 1;
     a.head_bytes = 1024 + (a.steps + a.split - 1) / a.split * kMxScaleTile +
                    (MODE == kGateUp ? up_to(pairs, kMxScaleTile) + a.nt * 512 : 0);
     a.head_bytes = up_to(a.head_bytes, 1024);
@@ -948,8 +956,9 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     r = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, MODE == kGateUp ? e.ws.x_pieces : e.ws.h_pieces, (uint64_t)a.steps * 128,
                piece_rows, (uint64_t)a.steps * 128, 128, 1, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != cudaSuccess) return r;
-    if (a.shared) return launch<8, P, MODE, true>(wmap, xmap, a, dim3(slots_ctas), smem, s);
-    return launch<8, P, MODE>(wmap, xmap, a, dim3(a.row_tiles, items, a.split), smem, s);
+    if (a.shared) return launch<8, P, MODE, kShared>(wmap, xmap, a, dim3(ctas), smem, s);
+    if (a.per_cta == 1) return launch<8, P, MODE>(wmap, xmap, a, dim3(a.row_tiles, items, a.split), smem, s);
+    return launch<8, P, MODE, kSome>(wmap, xmap, a, dim3((a.row_tiles + a.per_cta - 1) / a.per_cta, items), smem, s);
 }
 
 }  // namespace
