@@ -128,3 +128,62 @@ def half_step(y, dtype):
     """Half a step of dtype at |y|, and below its normal range half a step of the subnormals."""
     info = torch.finfo(dtype)
     return (info.eps / 2) * y.abs() * (1 + info.eps) + info.smallest_normal * info.eps / 2
+
+
+# ---- expert layers whose gate and up sums are exact in 32 bits ----------------------------------------
+
+NONZERO = 4   # values of a row of `down` in the layers of `whole_layer`
+
+
+def whole_layer(d, f, e, seed):
+    """(x maker, gate_up, down): activations are whole numbers -2..2 and the codes' scales two neighbouring powers of
+    two, so every gate and up sum is a multiple of half the smaller scale below 2^24 of them (48 d of them at most).
+    Its spread is about 2, where SiLU is neither linear nor zero. A row of `down` has NONZERO values, all others
+    zero, so that its sum has next to no error of its own."""
+    g = torch.Generator().manual_seed(seed)
+    low = 127 - round(math.log2(2.5 * math.sqrt(d)))
+    code = torch.randint(0, 256, (e, 2 * f, (d + 1) // 2), generator=g, dtype=torch.uint8)
+    scale = torch.randint(low, low + 2, (e, 2 * f, (d + 31) // 32), generator=g, dtype=torch.uint8)
+    wide = torch.zeros(e, d, f + f % 2, dtype=torch.uint8)
+    at = torch.randint(0, f, (e, d, NONZERO), generator=g)
+    wide.scatter_(2, at, torch.randint(1, 8, at.shape, generator=g, dtype=torch.uint8) + 8 * (at % 2).to(torch.uint8))
+    down = wide[..., 0::2] | wide[..., 1::2] << 4
+    dscale = torch.randint(126, 129, (e, d, (f + 31) // 32), generator=g, dtype=torch.uint8)
+    return (lambda t: torch.randint(-2, 3, (t, d), generator=g).double()), (code, scale), (down, dscale)
+
+
+def hidden64(x, gate_up, e, f):
+    """silu(gate) * up of every row of x through expert e, in 64 bits."""
+    gu = x @ values(gate_up[0][e], gate_up[1][e], x.shape[1]).t()
+    return gu[:, :f] * torch.sigmoid(gu[:, :f]) * gu[:, f:]
+
+
+def whole_experts(x, order, gate_up, down):
+    """(y, bound before the last rounding) of a `whole_layer` whose tokens give every one of the experts in `order`
+    (a power of two of them) the same weight, which then is exact. The bound, for each value of y:
+    * h = g / (1 + exp(-g)) * u in 32 bits: exp off by 2^-22 (2 units), sum, quotient and product by 2^-24 each: 2^-21
+    * h is held to 2^-19 of itself, or 2^-29 of the largest of its block of 32 where that is more
+    * the NONZERO products of a row and the pieces of each (_sum_error); the sum over the experts: 2^-24 for each."""
+    f, top = gate_up[0].shape[1] // 2, order.shape[1]
+    y, bound = torch.zeros_like(x), torch.zeros_like(x)
+    for e in order.unique().tolist():
+        t = (order == e).any(1).nonzero().flatten()
+        h, dn = hidden64(x[t], gate_up, e, f), values(down[0][e], down[1][e], f)
+        block = torch.nn.functional.pad(h.abs(), (0, -f % 32)).reshape(len(t), -1, 32).amax(-1)
+        dh = h.abs() * (2.0 ** -21 + 2.0 ** -19) + 2.0 ** -29 * block.repeat_interleave(32, -1)[:, :f]
+        y[t] += h @ dn.t() / top
+        bound[t] += (dh + (_sum_error(NONZERO) + top * 2.0 ** -24) * h.abs()) @ dn.abs().t() / top
+    return y, bound
+
+
+def rounding_off(got, want, bound, dtype):
+    """How far `got` of type dtype is outside of rounding `want` +- bound to dtype, in half steps (0: inside). The step
+    is the one at the nearest end of the interval, so a value one step off is seen unless the interval holds the border."""
+    info = torch.finfo(dtype)
+    near = want.abs() - bound
+    _, e = torch.frexp(near.clamp(min=info.smallest_normal))
+    half = torch.ldexp(torch.full_like(want, info.eps / 2), (e - 1))
+    # a value just under a power of two may round up to it, and one at its upper end has the step above it
+    up = torch.ldexp(torch.ones_like(want), e) - near <= half + 2 * bound
+    half = torch.where(up, 2 * half, half)
+    return (((got.cpu().double() - want).abs() - bound) / half - 1).clamp(min=0)

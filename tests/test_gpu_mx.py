@@ -720,3 +720,39 @@ def test_split_products_on_many_streams(mx):
 def test_experts_with_more_tiles_than_ctas(mx, t, d, f, e, top, norm, name, with_bias):
     """Every CTA takes several tiles, and goes on from one expert to the next."""
     test_experts(mx, t, d, f, e, top, norm, name, with_bias)
+
+
+WHOLE = [  # tokens, d, f, experts, experts of every token, type
+    (1, 64, 70, 4, 1, "f16"), (1, 2048, 1024, 8, 4, "bf16"), (7, 1447, 999, 12, 2, "f16"), (5, 300, 1500, 3, 1, "bf16"), (40, 520, 260, 2, 2, "f16"),
+    (128, 200, 136, 4, 2, "bf16"), (100, 333, 40, 2, 1, "f16"), (64, 640, 420, 64, 16, "bf16"),
+    # long rows: K spread over a cluster
+    (3, 16384, 64, 2, 2, "bf16"), (2, 40, 16384, 2, 1, "f16"), (33, 4200, 70, 2, 1, "f16"), (9, 300, 4300, 2, 2, "bf16"),
+    # several tiles to a CTA, from one expert on to the next
+    (8, 130, 1000, 20, 16, "bf16"), (90, 256, 4500, 2, 1, "f16"), (40, 2600, 70, 16, 16, "f16")]
+
+
+@pytest.mark.parametrize("t,d,f,e,top,name", WHOLE)
+def test_experts_of_exact_gate_and_up_sums(mx, t, d, f, e, top, name):
+    """Nothing but SiLU, the pieces of the hidden vector and the last rounding is off: a lost stage, a share of a cluster's
+    or a piece too few would show (test_the_bound_of_whole_layers_sees_faults)."""
+    make, gate_up, down = mxref.whole_layer(d, f, e, t + d + f)
+    x, dtype = make(t), mxref.TYPES[name]
+    layer = mx.Experts(torch.zeros(e, d, device="cuda", dtype=dtype), on_gpu(gate_up), on_gpu(down), top)
+    y, chosen, p = layer(x.to(dtype).cuda(), return_choice=True)
+    assert (chosen.cpu() == torch.arange(top)).all() and (p == 1 / top).all()   # equal logits: the lowest, alike
+    want, bound = mxref.whole_experts(x, chosen.cpu().long(), gate_up, down)
+    off = mxref.rounding_off(y, want, bound, dtype)
+    assert not (off > 0).any(), f"{int((off > 0).sum())} of {off.numel()}, worst {float(off.max()):.3g} half steps"
+    mx.check()
+
+
+@pytest.mark.parametrize("t,d,f,e,name", [(50, 700, 333, 9, "f16"), (128, 1000, 200, 40, "bf16"), (9, 2048, 1024, 32, "bf16")])
+def test_experts_of_exact_sums_each_token_its_own(mx, t, d, f, e, name):
+    """One expert to a token, whichever its router takes: its weight is 1."""
+    make, gate_up, down = mxref.whole_layer(d, f, e, t + d + f)
+    x, dtype = make(t), mxref.TYPES[name]
+    router = (torch.randn(e, d, generator=gen(t), device="cuda") / math.sqrt(d)).to(dtype)
+    y, chosen, p = mx.Experts(router, on_gpu(gate_up), on_gpu(down), 1)(x.to(dtype).cuda(), return_choice=True)
+    assert (p == 1).all() and len(chosen.unique()) > 4
+    want, bound = mxref.whole_experts(x, chosen.cpu().long(), gate_up, down)
+    assert not (mxref.rounding_off(y, want, bound, dtype) > 0).any()

@@ -143,3 +143,62 @@ def test_oracle_stored_form(k):
         assert ((w - b).abs() <= top / 4 + 1e-300).all()       # top is in [4, 8) scales: off by 1, or by 2 past 6
         small = b.abs() <= top / 4
         assert ((w - b).abs()[small] <= (top / 16).expand_as(b)[small]).all()  # under 2 scales: off by a quarter
+
+
+def _held(h, pieces):
+    """h as so many e4m3 pieces hold it, by its definition: a scale per 32, each piece 16 times finer than the one before."""
+    rows, f = h.shape
+    b = torch.nn.functional.pad(h, (0, -f % 32)).reshape(rows, -1, 32)
+    _, e = torch.frexp(b.abs().amax(-1, keepdim=True))
+    left = torch.ldexp(b, 8 - e)
+    total, unit = torch.zeros_like(left), 1.0
+    for _ in range(pieces):
+        piece = left.float().to(torch.float8_e4m3fn).double()
+        total += piece * unit
+        left, unit = (left - piece) * 16, unit / 16
+    return torch.ldexp(total, e - 8).reshape(rows, -1)[:, :f]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,f", [(64, 70), (300, 1500), (4200, 64), (16384, 64)])
+def test_the_bound_of_whole_layers_sees_faults(d, f, dtype):
+    """What a kernel could do wrong falls outside of the bound; the layer as it is documented does not."""
+    make, gate_up, down = mxref.whole_layer(d, f, 2, d + f)
+    x = make(9)
+    order = torch.tensor([[0, 1]]).expand(9, 2)
+    want, bound = mxref.whole_experts(x, order, gate_up, down)
+
+    def layer(change_h=lambda h: h, change_x=lambda x: x):
+        parts = [change_h(mxref.hidden64(change_x(x), gate_up, e, f)) @ mxref.values(down[0][e], down[1][e], f).t() for e in (0, 1)]
+        return (sum(parts) / 2).to(dtype)
+
+    def outside(y):
+        return int((mxref.rounding_off(y, want, bound, dtype) > 0).sum())
+
+    def without(step):   # 128 values of K, as a lost stage
+        def cut(x):
+            x = x.clone()
+            x[:, step * 128:step * 128 + 128] = 0
+            return x
+        return cut
+
+    assert outside(layer()) == 0 and outside(layer(lambda h: _held(h, 4))) == 0
+    assert outside(layer(lambda h: _held(h, 3))) > 0          # 14 bits
+    assert outside(layer(lambda h: _held(h, 2))) > want.numel() / 16
+    assert outside(torch.zeros_like(want)) > want.numel() * 0.9
+    assert outside(layer(change_x=without((d - 1) // 128))) > want.numel() * 0.5
+    assert outside(layer(lambda h: torch.cat((h[:, :-32], torch.zeros_like(h[:, -32:])), 1))) > 0   # a lost block
+
+
+def test_the_bound_of_whole_layers_rests_on_exact_sums():
+    for d in (1, 64, 16384):
+        make, gate_up, _ = mxref.whole_layer(d, 4, 1, d)
+        unit = 2.0 ** (int(gate_up[1].min()) - 128)
+        size = make(8).abs() @ mxref.values(gate_up[0][0], gate_up[1][0], d).abs().t() / unit
+        assert (size == size.round()).all() and float(size.max()) < 2 ** 24
+    h = torch.randn(50, 320, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    h = h * torch.exp(2 * torch.randn(h.shape, generator=torch.Generator().manual_seed(2), dtype=torch.float64))
+    top = h.abs().reshape(50, 10, 32).amax(-1).repeat_interleave(32, -1)
+    for pieces in (1, 2, 3, 4, 5):
+        off = (_held(h, pieces) - h).abs()
+        assert (off <= torch.maximum(h.abs() * 2.0 ** (1 - 5 * pieces), top * 2.0 ** (-13 - 4 * pieces))).all()

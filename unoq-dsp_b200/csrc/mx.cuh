@@ -19,7 +19,7 @@ constexpr int kMxTile = 128;          // rows of a tile, values of a scale tile
 constexpr int kMxCodeTile = 16384;    // bytes of a code tile, 128 x 256
 constexpr int kMxScaleTile = 512;     // bytes of a scale tile, 128 x 128
 constexpr int kMxHalf = 64;           // gate rows, and up rows, of a tile of paired matrices
-constexpr int kMxHiddenPieces = 3;    // pieces of the hidden vector of ug_mx4_experts
+constexpr int kMxHiddenPieces = 4;    // pieces of the hidden vector of ug_mx4_experts
 constexpr int kMxRouterCluster = 8;   // CTAs that share one token's router product
 
 __host__ __device__ inline uint32_t mx_tiles(uint32_t n) { return (n + kMxTile - 1) / kMxTile; }
@@ -257,8 +257,8 @@ struct MxExpertsScratch {
     uint32_t *arrived;    // tokens x 4 mx_tiles(d): pairs whose 32 values are written
     uint8_t *x_pieces;    // (tokens * pieces) x 128 mx_tiles(d), e4m3
     uint8_t *x_scales;    // (tokens * pieces) x 4 mx_tiles(d)
-    uint8_t *h_pieces;    // (tokens * top_k * 3) x 128 mx_tiles(f), e4m3
-    uint8_t *h_scales;    // (tokens * top_k * 3) x 4 mx_tiles(f)
+    uint8_t *h_pieces;    // (tokens * top_k * 4) x 128 mx_tiles(f), e4m3
+    uint8_t *h_scales;    // (tokens * top_k * 4) x 4 mx_tiles(f)
     float *partial;       // (tokens * top_k) x d: weighted down products
 };
 

@@ -32,8 +32,11 @@ namespace cg = cooperative_groups;
 constexpr int kMaxStages = 16;
 constexpr int kThreads = 224;      // warp 0: weight copies, warp 1: MMA, warps 2-5: epilogue, warp 6: activation copies
 constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
-constexpr int kItemWords = 2 + 32; // an item: expert, tokens, the pairs
-constexpr int kChunk = 32;         // most tokens of one expert that one CTA takes
+constexpr int kItemWords = 2 + 32; // an item: expert, tokens, the pairs (a lane each)
+// Most tokens of one expert that one CTA takes: two accumulators of 32 tokens' hidden pieces would fill its 256 columns
+// of TMEM. (With three pieces to a value and 32 tokens: 4 of 16 experts, d 4096, f 2048, 128 tokens 146 us against 168;
+// 4 of 32, d 2048, f 1024, 128 tokens 56.4, 58.6; 2 of 8, 128 tokens 46.4, 43.4.)
+constexpr int kChunk = 24;
 constexpr uint32_t kA = 16384;     // one weight tile in shared memory
 
 __host__ __device__ constexpr uint32_t up_to(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
@@ -74,9 +77,9 @@ struct Ctrl {
     unsigned long long rows_ready, scales_ready, spare;
     uint32_t tmem;
     int abort;
-    uint32_t pairs[kChunk], found[4];
+    uint32_t pairs[32], found[4];
     float weights[kChunk];
-    alignas(16) int32_t rows[kChunk * 3];   // of pieces, at most three to a token
+    alignas(16) int32_t rows[kChunk * kMxHiddenPieces];   // of pieces
 };
 static_assert(sizeof(Ctrl) <= kCtrlBytes, "control block");
 
@@ -520,7 +523,9 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
         reinterpret_cast<float *>(MODE == kGateUp ? sfb_all + (a.steps + a.split - 1) / a.split * kMxScaleTile : ring);
 
     // The hidden value of one of the tile's 64 and its pieces. A warp's 32 are one block along the next
-    // product's K. Three pieces keep 12 bits of it: past what x and y hold in either type.
+    // product's K. Four pieces hold it to 2^-19 of itself, or 2^-29 of its block's largest: where the sums in 32 bits
+    // are off by as much. Three hold it to 2^-14, which outputs in f16 show. One token through 4 of 32 experts, and 64
+    // through 8 of 128: three pieces 17.0 and 96.4 us, four 17.1 and 99.1, five (2^-24) 17.1 and 104.3.
     auto hidden = [&](uint32_t i, float g, float u) {
         const float h = g / (1.0f + expf(-g)) * u;
         const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(h) & 0x7FFFFFFFu);
