@@ -756,3 +756,27 @@ def test_experts_of_exact_sums_each_token_its_own(mx, t, d, f, e, name):
     assert (p == 1).all() and len(chosen.unique()) > 4
     want, bound = mxref.whole_experts(x, chosen.cpu().long(), gate_up, down)
     assert not (mxref.rounding_off(y, want, bound, dtype) > 0).any()
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("e,top,bad", [(9, 2, (5,)), (200, 16, (0, 33, 199)), (3, 3, (1,)), (40, 1, (39, 7))])
+def test_a_nan_logit_is_chosen_and_makes_the_output_nan(mx, e, top, bad, name, norm):
+    """As torch.sort orders them: a NaN before every number, equal ones by index. A damaged router shows in both modes."""
+    router, gate_up, down, bias = layer_parts(96, 64, e, name, True, 5)
+    x = torch.randn(6, 96, generator=gen(3), device="cuda").to(mxref.TYPES[name])
+    clean = x.cpu().double() @ router.double().t() + bias.double()
+    for broken in ("router", "bias"):
+        r, b = router.clone(), bias.clone()
+        if broken == "router":
+            r[list(bad), 50] = math.nan
+        else:
+            b[list(bad)] = math.nan
+        y, chosen, p = mx.Experts(r.cuda(), on_gpu(gate_up), on_gpu(down), top, norm, b.cuda())(x, return_choice=True)
+        assert torch.isnan(y).all() and torch.isnan(p).all()
+        order, _ = mxref.select(torch.where(torch.isin(torch.arange(e), torch.tensor(bad)), math.nan, clean), top, norm)
+        first = min(len(bad), top)
+        assert chosen[:, :first].tolist() == [sorted(bad)[:first]] * 6
+        ok = distinct(x, router, bias, e)   # all of its logits apart
+        assert torch.equal(chosen.cpu().long()[ok], order[ok]) and (ok.any() or e > 100)
+        assert all(len(set(row)) == top and 0 <= min(row) and max(row) < e for row in chosen.tolist())

@@ -266,7 +266,8 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
 
     cluster.sync();
     if (rank != 0 || warp != 0) return;
-    // selection: keys order as the logits do; a NaN is below every number, a taken expert is 0
+    // selection: keys order as the logits do; a NaN is above every number, so that it is chosen and shows in the weights
+    // and the output whichever softmax is taken; a taken expert is 0
     uint32_t key[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -275,7 +276,7 @@ __global__ void __cluster_dims__(kMxRouterCluster, 1, 1) __launch_bounds__(256) 
         if (e < a.experts) {
             const float l = logits[e];
             const uint32_t bits = __float_as_uint(l);
-            key[i] = l != l ? 1u : (bits & 0x80000000u ? ~bits : bits | 0x80000000u);
+            key[i] = l != l ? 0xFFFFFFFFu : (bits & 0x80000000u ? ~bits : bits | 0x80000000u);
             if (l == 0.0f) key[i] = 0x80000000u;  // -0 and 0 tie
         }
     }

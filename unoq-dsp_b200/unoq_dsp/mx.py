@@ -304,6 +304,7 @@ class Experts:
     ``router``: (experts, d) in 16 bits; ``bias``: (experts,) float32 added to the logits, or None.
     ``gate_up``: stored codes and scales of (experts, 2f, d), the gate's rows before the up rows;
     ``down``: those of (experts, d, f). ``normalize``: softmax over the chosen logits, else over all.
+    Ties go to the lowest index; a NaN logit comes before every number and makes its token's output NaN.
     The weights are packed once, here; the stored ones are not kept."""
 
     def __init__(self, router, gate_up, down, top_k, normalize=True, bias=None):
