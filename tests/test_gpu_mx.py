@@ -780,3 +780,28 @@ def test_a_nan_logit_is_chosen_and_makes_the_output_nan(mx, e, top, bad, name, n
         ok = distinct(x, router, bias, e)   # all of its logits apart
         assert torch.equal(chosen.cpu().long()[ok], order[ok]) and (ok.any() or e > 100)
         assert all(len(set(row)) == top and 0 <= min(row) and max(row) < e for row in chosen.tolist())
+
+
+def test_forward_mode_tangents_are_refused(mx):
+    from torch.autograd import forward_ad
+    x = torch.randn(4, 96, generator=gen(1), device="cuda").to(torch.bfloat16)
+    W = mx.quantize(torch.randn(70, 96, generator=gen(2), device="cuda"))
+    router, gate_up, down, bias = layer_parts(96, 64, 8, "bf16", True, 5)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2)
+    want = mx.matmul(x, W), layer(x), mx.quantize(x).dequantize()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        out = forward_ad.make_dual(torch.empty(4, 70, device="cuda", dtype=x.dtype), torch.ones(4, 70, device="cuda", dtype=x.dtype))
+        for call in (lambda: mx.quantize(dual), lambda: mx.matmul(dual, W), lambda: layer(dual), lambda: mx.matmul(x, W, out=out),
+                     lambda: mx.Experts(forward_ad.make_dual(router.cuda(), router.cuda()), on_gpu(gate_up), on_gpu(down), 2),
+                     lambda: mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2, bias=forward_ad.make_dual(bias.cuda(), bias.cuda()))):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+        for got, v in zip((mx.matmul(x, W), layer(x), mx.quantize(x).dequantize()), want):   # no tangent: as ever
+            assert torch.equal(got, v)
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(lambda v: mx.matmul(v, W), (x,), (x,))
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.vmap(lambda v: mx.matmul(v, W))(x)

@@ -202,3 +202,32 @@ def test_the_bound_of_whole_layers_rests_on_exact_sums():
     for pieces in (1, 2, 3, 4, 5):
         off = (_held(h, pieces) - h).abs()
         assert (off <= torch.maximum(h.abs() * 2.0 ** (1 - 5 * pieces), top * 2.0 ** (-13 - 4 * pieces))).all()
+
+
+def test_python_refuses_gradients_and_tangents():
+    from torch.autograd import forward_ad
+
+    from unoq_dsp import mx
+    x = torch.ones(2, 3)
+    mx._refuse_gradient(x, "x")
+    with pytest.raises(ValueError, match="x needs a gradient"):
+        mx._refuse_gradient(x.clone().requires_grad_(), "x")
+    with torch.no_grad():
+        mx._refuse_gradient(x.clone().requires_grad_(), "x")
+    with forward_ad.dual_level():
+        mx._refuse_gradient(x, "x")
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="x carries a tangent"):
+                mx._refuse_gradient(dual, "x")
+        mx._refuse_gradient(forward_ad.unpack_dual(dual).primal, "x")
+    seen = []
+
+    def inside(v):
+        with pytest.raises(ValueError, match="tangent"):
+            mx._refuse_gradient(v, "x")
+        seen.append(1)
+        return v
+
+    torch.func.jvp(inside, (x,), (x,))
+    assert seen == [1]

@@ -3,8 +3,8 @@
 The functions check their tensors, allocate the results (and a workspace of the call's own) with
 PyTorch's allocator and launch the kernels of include/unoq_mx.h on the current stream of the
 tensors' device, without waiting for it; all of them may be captured into a CUDA graph. They are
-for inference: an input that needs a gradient is refused while gradients are recorded. PyTorch is imported here
-only; the rest of the package does not need it.
+for inference: an input that needs a gradient is refused while gradients are recorded, and one that carries a
+forward-mode tangent always. PyTorch is imported here only; the rest of the package does not need it.
 
     w = mx.quantize(weight)                      # (n, k) -> MX4, once
     y = mx.matmul(x, w)                          # 16-bit x, 4-bit weights
@@ -15,6 +15,7 @@ only; the rest of the package does not need it.
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from .errors import DSPError
 from .native import last_error, load_library
@@ -61,15 +62,21 @@ def _input(x, what, types):
         raise ValueError(f"{what} must be a CUDA tensor")
     if x.dtype not in types:
         raise ValueError(f"{what} must be one of {', '.join(str(t) for t in types)}, not {x.dtype}")
+    _refuse_gradient(x, what)
+    return x
+
+
+def _refuse_gradient(x, what):
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} needs a gradient; the MX4 operators are for inference (use torch.no_grad())")
-    return x
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:   # torch.no_grad() keeps these
+        raise ValueError(f"{what} carries a tangent; the MX4 operators are for inference (use forward_ad.unpack_dual)")
 
 
 def _rows(x, what, types):
     """(x as rows of contiguous values, rows, k, row stride, type code); copied only where it has to be."""
     code = types.get(x.dtype) if isinstance(x, torch.Tensor) and x.is_cuda else None
-    if code is None or x.requires_grad:
+    if code is None or x.requires_grad or forward_ad._current_level >= 0:
         code = types[_input(x, what, types).dtype]
     if x.dim() != 2:
         if x.dim() < 1 or x.shape[-1] < 1:
@@ -99,8 +106,7 @@ def _output(out, shape, dtype, device, inputs):
         raise ValueError(f"out must be a tensor of shape {tuple(shape)} on {device}")
     if out.dtype != dtype:
         raise ValueError(f"out must be {dtype}")
-    if out.requires_grad and torch.is_grad_enabled():
-        raise ValueError("out needs a gradient; the MX4 operators are for inference")
+    _refuse_gradient(out, "out")
     if out.shape[-1] > 1 and out.stride(-1) != 1 or out.dim() != 2 and not out.is_contiguous() \
             or out.dim() == 2 and out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError("out needs contiguous rows that do not overlap")
