@@ -231,3 +231,18 @@ def test_python_refuses_gradients_and_tangents():
 
     torch.func.jvp(inside, (x,), (x,))
     assert seen == [1]
+
+
+def test_a_layer_is_on_the_device_of_its_tensors(native):
+    """As loading with tensors mapped to another device leaves it: the state names the old one, the tensors are elsewhere."""
+    import copy
+
+    from unoq_dsp import mx
+    layer = mx.Experts.__new__(mx.Experts)
+    state = dict(router=torch.zeros(2, 64, dtype=torch.bfloat16), bias=None, top_k=1, d=64, f=64, experts=2, normalize=True,
+                 device=torch.device("cuda", 1), gate_up=[torch.zeros(1, dtype=torch.uint8)] * 2,
+                 down=[torch.zeros(1, dtype=torch.uint8)] * 2)
+    layer.__setstate__(state)
+    assert layer.device == torch.device("cpu") and copy.copy(layer).device == layer.device
+    with pytest.raises(ValueError, match="CUDA"):
+        layer(torch.zeros(1, 64, dtype=torch.bfloat16))

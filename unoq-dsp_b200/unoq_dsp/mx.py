@@ -339,7 +339,7 @@ class Experts:
             if x.device != router.device:
                 raise ValueError("the layer's tensors are on two devices")
         self.router, self.bias, self.top_k, self.d, self.f, self.experts = router.contiguous(), bias, top_k, d, f, e
-        self.normalize, self.device = bool(normalize), router.device
+        self.normalize = bool(normalize)
         self.gate_up = _pack(gc, gs, e, 2 * f, d, 1)
         self.down = _pack(dc, ds, e, d, f, 0)
         self._bind()
@@ -347,6 +347,7 @@ class Experts:
     def _bind(self):
         """The C side's view of the tensors, which it keeps alive whatever becomes of the attributes."""
         code = _TYPES[self.router.dtype]
+        self.device = self.router.device   # a loaded layer's tensors may have been mapped to another
         self._kept = kept = (self.router, self.bias, *self.gate_up, *self.down)
         self._layer = UgMx4Experts(self.experts, self.top_k, self.d, self.f, self.normalize, code,
                                    *(None if x is None else x.data_ptr() for x in kept))
