@@ -12,7 +12,13 @@
  *                   (j % 256) / 2 with K = ceil(k/256), and scales in tiles of 128 values,
  *                   ((r / 128) * 2K + j / 128) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + (j / 32 % 4).
  *                   Values and scale bytes past k, up to 256 K, are zero.
- * A last block or tile may be partial: rows and k are free (k >= 1).
+ * A last block or tile may be partial: rows and k are free (k >= 1), as far as the kernels count in 32 bits.
+ * With T = 2 ceil(k/256), the scale tiles along a row:
+ *   quantise, dequantise       rows * T < 2^31, k <= 2^30
+ *   pack                       the same, rows being all matrices' with their padding (ug_mx4_pack_rows)
+ *   products                   k <= UG_MX4_MAX_K, m <= UG_MX4_MAX_M, (n + 127) T < 2^31, and (m + 255) T < 2^31,
+ *                              with 16-bit activations (4 m + 256) T < 2^31
+ *   experts                    the limits below
  *
  * Every array is DEVICE memory of one device, `stream` is a cudaStream_t of that device (NULL: its
  * legacy default stream). Calls check their arguments, launch on `stream` and return without

@@ -805,3 +805,27 @@ def test_forward_mode_tangents_are_refused(mx):
         torch.func.jvp(lambda v: mx.matmul(v, W), (x,), (x,))
     with pytest.raises((ValueError, RuntimeError)):
         torch.func.vmap(lambda v: mx.matmul(v, W))(x)
+
+
+def test_a_product_of_the_most_4_bit_rows(mx):
+    """2^21 rows of 32,768 values, 34 GB of codes, of which the first and the last tile are looked at."""
+    m, n, k = 2 ** 21, 40, 32768
+    codes = torch.zeros(m // 2 * k, dtype=torch.uint8, device="cuda")
+    scales = torch.full((m * k // 32,), 127, dtype=torch.uint8, device="cuda")
+    a, w = whole(128, k, 1, True), whole(n, k, 2, False)
+    tile = mx.pack(*on_gpu(a))
+    for part in (slice(0, len(tile.codes)), slice(-len(tile.codes), None)):
+        codes[part] = tile.codes
+    for part in (slice(0, len(tile.scales)), slice(-len(tile.scales), None)):
+        scales[part] = tile.scales
+    y = mx.matmul(mx.MX4(codes, scales, m, k), mx.pack(*on_gpu(w)), dtype=torch.float32)
+    want = mxref.values(*a, k) @ mxref.values(*w, k).t()   # multiples of 1/4 below 2^22
+    assert torch.equal(y[:128].cpu().double(), want) and torch.equal(y[-128:].cpu().double(), want)
+    assert not y[128:-128].any()
+    del codes, scales, y
+    big = torch.empty(1, dtype=torch.bfloat16, device="cuda")
+    for rows, k in ((2 ** 21 + 1, 40), (2 ** 21 - 1, 65536)):   # refused before the rows would be copied (275 GB)
+        with pytest.raises(ValueError, match="at most"):
+            mx.matmul(big.expand(rows, k), mx.quantize(torch.zeros(1, k, device="cuda")))
+    with pytest.raises(ValueError, match="65536"):
+        mx.matmul(mx.quantize(torch.zeros(1, 65537, device="cuda")), mx.quantize(torch.zeros(1, 65537, device="cuda")))

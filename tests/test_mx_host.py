@@ -246,3 +246,56 @@ def test_a_layer_is_on_the_device_of_its_tensors(native):
     assert layer.device == torch.device("cpu") and copy.copy(layer).device == layer.device
     with pytest.raises(ValueError, match="CUDA"):
         layer(torch.zeros(1, 64, dtype=torch.bfloat16))
+
+
+def _edge(fits, lo, hi):
+    """The largest size in [lo, hi) that fits, hi not fitting."""
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        lo, hi = (mid, hi) if fits(mid) else (lo, mid)
+    return lo
+
+
+def test_the_documented_limits_and_no_nearer_ones(native):
+    """Both sides of every joint limit, in C (18: too large; 22: the null pointer that is looked at next) and in Python."""
+    from unoq_dsp import mx
+
+    def python_takes(call, *args):
+        try:
+            call(*args)
+            return True
+        except ValueError as e:
+            assert "at most" in str(e)
+            return False
+
+    for k in (1, 256, 257, 5000, 65536, 2 ** 30):
+        tiles = 2 * -(-k // 256)
+        rows = (2 ** 31 - 1) // tiles
+        for fit, r in ((True, rows), (False, rows + 1)):
+            want = 22 if fit else 18
+            assert native.ug_mx4_quantize(None, 0, r, k, k, 0, None, None, None) == want
+            assert native.ug_mx4_dequantize(None, None, 1, r, k, None, 0, k, None) == want
+            assert python_takes(mx._fits, r, k, "x") == fit
+        assert native.ug_mx4_quantize(None, 0, 1, 2 ** 30 + 1, 2 ** 30 + 1, 0, None, None, None) == 18
+        whole = rows // 128 * 128   # pack counts whole tiles
+        if whole:
+            assert native.ug_mx4_pack(None, None, 1, whole, k, 0, None, None, None) == 22
+        assert native.ug_mx4_pack(None, None, 1, whole + 1, k, 0, None, None, None) == 18
+    for k in (1, 256, 5000, 32768, 65536):
+        tiles = 2 * -(-k // 256)
+        most = (2 ** 31 - 1) // tiles
+        for pieces, m in ((False, min(most - 255, 2 ** 21)), (True, min((most - 256) // 4, 2 ** 21))):
+            for fit, rows, cols in ((True, m, most - 127), (False, m + 1, 1), (False, 1, most - 126)):
+                want = 22 if fit else 18
+                if pieces:
+                    got = native.ug_mx4_matmul_x16(P, 2, k, rows, None, None, cols, k, None, 0, cols, P, 1 << 62, None)
+                else:
+                    got = native.ug_mx4_matmul(P, P, rows, None, None, cols, k, None, 0, cols, None)
+                assert got == want, (k, rows, cols)
+                assert python_takes(mx._product_fits, rows, cols, k, pieces) == fit
+    assert native.ug_mx4_matmul(P, P, 2 ** 21, P, P, 8, 65537, P, 0, 8, None) == 18
+    # what the Python calls look at first lets nothing past
+    for k in (1, 100, 256, 257, 65536, 2 ** 30):
+        assert _edge(lambda r: python_takes(mx._fits, r, k, "x"), 0, 2 ** 40) >= (2 ** 38 - 1) // (k + 255)
+    for m, n in ((0, 2 ** 21 - 1), (2 ** 19 - 1, 3)):
+        assert 4 * m + n < 2 ** 21 and python_takes(mx._product_fits, m, n, 65536, True)

@@ -78,7 +78,7 @@ int launch(const F &f) {
     }
 }
 
-// rows x k with so many tiles each: counted in 32 bits by the kernels
+// rows x k with so many tiles each: counted in 32 bits by the kernels (unoq_mx.h states the limit)
 bool sizes_ok(uint64_t rows, uint32_t k) { return k >= 1 && k <= (1u << 30) && rows * uq::mx_ktiles(k) < (1ull << 31); }
 
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
@@ -188,10 +188,10 @@ int ug_mx4_pack(const uint8_t *codes, const uint8_t *scales, uint32_t count, uin
     });
 }
 
-static int product(uq::MxProductArgs &p, void *stream, const char *name) {
+static int product(uq::MxProductArgs &p, bool pieces, void *stream, const char *name) {
     if (!is_type(p.type)) return fail(18, name);
-    // rows counted with their padding: whole tiles of n, up to four rows of pieces to a token of m
-    if (p.k < 1 || p.k > UG_MX4_MAX_K || p.m > UG_MX4_MAX_M || !sizes_ok((uint64_t)p.m * 4 + 256, p.k) ||
+    // rows counted with their padding: whole tiles of m and n, up to four rows of pieces to a 16-bit token of m
+    if (p.k < 1 || p.k > UG_MX4_MAX_K || p.m > UG_MX4_MAX_M || !sizes_ok(pieces ? (uint64_t)p.m * 4 + 256 : (uint64_t)p.m + 255, p.k) ||
         !sizes_ok((uint64_t)p.n + 127, p.k) || p.stride < p.n)
         return fail(18, name);
     if (!p.m || !p.n) return 0;
@@ -219,7 +219,7 @@ int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32_t m, c
     p.y = y;
     p.type = type;
     p.stride = stride;
-    return product(p, stream, "ug_mx4_matmul: type, sizes, stride or pointers out of range");
+    return product(p, false, stream, "ug_mx4_matmul: type, sizes, stride or pointers out of range");
 }
 
 size_t ug_mx4_matmul_x16_workspace(uint32_t m, uint32_t k, int x_type) {
@@ -249,7 +249,7 @@ int ug_mx4_matmul_x16(const void *x, int x_type, uint64_t x_stride, uint32_t m, 
     p.type = type;
     p.stride = stride;
     p.workspace = need ? workspace : nullptr;
-    return product(p, stream, "ug_mx4_matmul_x16: type, sizes, stride or pointers out of range");
+    return product(p, true, stream, "ug_mx4_matmul_x16: type, sizes, stride or pointers out of range");
 }
 
 size_t ug_mx4_experts_workspace(const UgMx4Experts *layer, uint32_t tokens) {

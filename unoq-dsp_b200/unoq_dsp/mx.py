@@ -22,7 +22,8 @@ from .native import last_error, load_library
 
 STORED, OPERAND = 0, 1
 MAX_TOKENS = 128
-MAX_SIZE = 2 ** 31 - 1   # rows or values of a row: the C calls count them in 32 bits
+MAX_K = 65536            # of a product
+MAX_ROWS = 2 ** 21       # of a product's activations
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _HALF = {t: _TYPES[t] for t in (torch.float16, torch.bfloat16)}
 
@@ -73,8 +74,9 @@ def _refuse_gradient(x, what):
         raise ValueError(f"{what} carries a tangent; the MX4 operators are for inference (use forward_ad.unpack_dual)")
 
 
-def _rows(x, what, types):
-    """(x as rows of contiguous values, rows, k, row stride, type code); copied only where it has to be."""
+def _rows(x, what, types, n=-1):
+    """(x as rows of contiguous values, rows, k, row stride, type code); copied only where it has to be, and not
+    before the limits of a product with n rows of weights."""
     code = types.get(x.dtype) if isinstance(x, torch.Tensor) and x.is_cuda else None
     if code is None or x.requires_grad or forward_ad._current_level >= 0:
         code = types[_input(x, what, types).dtype]
@@ -83,8 +85,10 @@ def _rows(x, what, types):
             raise ValueError(f"{what} needs at least one value in its last axis")
         x = x.reshape(-1, x.shape[-1])
     rows, k = x.shape
-    if rows > MAX_SIZE or k > MAX_SIZE:
-        raise ValueError(f"{what} may have at most {MAX_SIZE} rows of as many values")
+    if rows * (k + 255) >= 2 ** 38 or k > 2 ** 30:   # no limit is nearer: the exact ones are looked at only then
+        _fits(rows, k, what)
+    if n >= 0 and (k > MAX_K or 4 * rows + n >= 2 ** 21):
+        _product_fits(rows, n, k, True)
     row, step = x.stride()
     if rows < 2:
         row = k
@@ -94,6 +98,22 @@ def _rows(x, what, types):
         if k > 1 or row < k:
             x, row = x.contiguous(), k
     return x, rows, k, row, code
+
+
+def _fits(rows, k, what):
+    """Refuse a matrix that the C calls cannot count in 32 bits (the limits of include/unoq_mx.h)."""
+    if k > 2 ** 30 or rows * (2 * (k + 255 >> 8)) >= 2 ** 31:
+        raise ValueError(f"{what} of {rows} rows of {k}: at most 2^30 values to a row, and rows x 2 ceil(k / 256) below 2^31")
+
+
+def _product_fits(m, n, k, pieces):
+    """Refuse a product past the same limits; `pieces`: its activations are in 16 bits."""
+    if k > MAX_K or m > MAX_ROWS:
+        raise ValueError(f"a product takes at most {MAX_ROWS} rows of {MAX_K} values, not {m} of {k}")
+    tiles = 2 * (k + 255 >> 8)
+    if (4 * m + 256 if pieces else m + 255) * tiles >= 2 ** 31 or (n + 127) * tiles >= 2 ** 31:
+        raise ValueError(f"a product of {m} and {n} rows of {k}: at most 2^31 / (2 ceil(k / 256)) rows of either, with "
+                         "their padding" + (", of 16-bit activations a quarter of that" if pieces else ""))
 
 
 def _row_stride(x, rows, k):
@@ -140,8 +160,9 @@ class MX4:
     __slots__ = ("rows", "k", "layout", "device", "_data", "_any", "_codes", "_scales")
 
     def __init__(self, codes, scales, rows, k, layout="operand"):
-        if not 0 <= rows <= MAX_SIZE or not 1 <= k <= MAX_SIZE:
-            raise ValueError(f"rows must be 0 or more and k 1 or more, at most {MAX_SIZE}")
+        if rows < 0 or k < 1:
+            raise ValueError("rows must be 0 or more and k 1 or more")
+        _fits(rows, k, "a matrix")
         for x, want, name in zip((codes, scales), _sizes(_layout(layout), rows, k), ("codes", "scales")):
             _input(x, name, (torch.uint8,))
             if not x.is_contiguous() or x.numel() != want:
@@ -237,8 +258,7 @@ def _stored_pair(codes, scales, k, what):
 
 
 def _pack(codes, scales, count, rows, k, paired):
-    if count * rows > MAX_SIZE or k > MAX_SIZE:
-        raise ValueError(f"a matrix may have at most {MAX_SIZE} rows of as many values")
+    _fits(count * (rows + 127 & ~127), k, "a matrix in whole tiles")
     lib = _library()
     padded = lib.ug_mx4_pack_rows(count, rows, paired)
     out = [torch.empty(size, dtype=torch.uint8, device=codes.device) for size in _sizes(OPERAND, padded, k)]
@@ -273,13 +293,15 @@ def matmul(a, w, dtype=None, out=None):
         shape = (m, n)
     else:
         values = a
-        a, m, k, a_stride, x_type = _rows(a, "a", _HALF)
+        a, m, k, a_stride, x_type = _rows(a, "a", _HALF, n)
         dtype = dtype or a.dtype
         shape = (m, n) if values is a else (*values.shape[:-1], n)
     if dtype not in _TYPES:
         raise ValueError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}")
     if k != w.k or a.device != device:
         raise ValueError(f"a has rows of {k} on {a.device}, w of {w.k} on {device}")
+    if four and (k > MAX_K or 4 * m + n >= 2 ** 21):
+        _product_fits(m, n, k, False)
     stride = n
     if out is None:
         out = w._any.new_empty(shape, dtype=dtype)
