@@ -829,3 +829,23 @@ def test_a_product_of_the_most_4_bit_rows(mx):
             mx.matmul(big.expand(rows, k), mx.quantize(torch.zeros(1, k, device="cuda")))
     with pytest.raises(ValueError, match="65536"):
         mx.matmul(mx.quantize(torch.zeros(1, 65537, device="cuda")), mx.quantize(torch.zeros(1, 65537, device="cuda")))
+
+
+def test_outputs_in_the_buffer_of_their_input(mx):
+    W = mx.pack(*on_gpu(weights(50, 96, 4)))
+    router, gate_up, down, _ = layer_parts(64, 64, 4, "f16", False, 5)
+    layer = mx.Experts(router.cuda(), on_gpu(gate_up), on_gpu(down), 2)
+    for m in (1, 6, 40, 300):
+        buf = torch.randn(m, 200, generator=gen(m), device="cuda").to(torch.float16)
+        was = buf.clone()
+        mx.matmul(buf[:, 3:99], W, out=buf[:, 120:170])
+        assert torch.equal(buf[:, 120:170], mx.matmul(was[:, 3:99], W))
+        buf[:, 120:170] = was[:, 120:170]
+        assert torch.equal(buf, was)
+        if m <= 40:
+            layer(buf[:, :64], out=buf[:, 64:128])
+            assert torch.equal(buf[:, 64:128], layer(was[:, :64]))
+            buf[:, 64:128] = was[:, 64:128]
+            assert torch.equal(buf, was)
+        with pytest.raises(ValueError, match="overlap"):
+            mx.matmul(buf[:, 3:99], W, out=buf[:, 98:148])

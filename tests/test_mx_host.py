@@ -299,3 +299,34 @@ def test_the_documented_limits_and_no_nearer_ones(native):
         assert _edge(lambda r: python_takes(mx._fits, r, k, "x"), 0, 2 ** 40) >= (2 ** 38 - 1) // (k + 255)
     for m, n in ((0, 2 ** 21 - 1), (2 ** 19 - 1, 3)):
         assert 4 * m + n < 2 ** 21 and python_takes(mx._product_fits, m, n, 65536, True)
+
+
+def test_outputs_beside_inputs_in_one_buffer():
+    """An output overlaps an input where they share a byte, not where only their extents cross."""
+    from unoq_dsp import mx
+    buf = torch.zeros(12, 40, dtype=torch.bfloat16)
+    flat = buf.view(-1)
+
+    def takes(out, x):
+        shared = {out.data_ptr() + 2 * (i * out.stride(0) + j) for i in range(out.shape[0]) for j in range(out.shape[1])} & \
+            {x.data_ptr() + 2 * (i * x.stride(0) + j) for i in range(x.shape[0]) for j in range(x.shape[1])}
+        try:
+            mx._output(out, out.shape, out.dtype, out.device, (x,))
+            return True, not shared
+        except ValueError as e:
+            assert "overlap" in str(e)
+            return False, not shared
+
+    for lo, hi in ((0, 20), (20, 40), (21, 40), (19, 40), (5, 6), (39, 40), (0, 40)):
+        for rows in (slice(0, 12), slice(1, 12), slice(3, 4)):
+            took, apart = takes(buf[rows, lo:hi], buf[:, :20])
+            assert took == apart, (lo, hi, rows)
+    assert takes(buf[0::2], buf[1::2]) == (True, True) and takes(buf[0::2], buf[2::2]) == (False, False)
+    assert takes(buf[3:4, 20:], buf[:, :20]) == (True, True) and takes(buf[:, 20:], buf[5:6, :20]) == (True, True)
+    assert takes(buf[3:4], buf[4:5]) == (True, True)
+    # a row that reaches round the end of the other's: the last one's, and the next one's first
+    assert takes(flat[20:20 + 11 * 40].view(11, 40)[:, :30], buf[:, :20]) == (False, False)
+    other = torch.as_strided(flat, (8, 4), (50, 1), 20)   # rows of another distance: their extents decide
+    assert takes(other, buf[:, :20])[0] is False
+    for x in (flat[:40], buf[:1, :20]):
+        assert takes(buf[1:], x.view(1, -1)) == (True, True)

@@ -133,8 +133,20 @@ def _output(out, shape, dtype, device, inputs):
     lo = out.data_ptr()
     hi = lo + _extent(out)
     for x in inputs:
-        if lo < x.data_ptr() + _extent(x) and x.data_ptr() < hi:
+        if lo < x.data_ptr() + _extent(x) and x.data_ptr() < hi and not _side_by_side(out, x):
             raise ValueError("out must not overlap an input")
+
+
+def _side_by_side(a, b):
+    """Whether two matrices whose extents cross share no byte: columns of one buffer, or every other of its rows."""
+    if a.dim() != 2 or b.dim() != 2:
+        return False
+    pitches = {x.stride(0) * x.element_size() for x in (a, b) if x.shape[0] > 1}
+    if len(pitches) != 1:
+        return False
+    pitch = pitches.pop()
+    at = (b.data_ptr() - a.data_ptr()) % pitch   # of b's rows behind those of a
+    return a.shape[1] * a.element_size() <= at <= pitch - b.shape[1] * b.element_size()
 
 
 def _extent(x):
