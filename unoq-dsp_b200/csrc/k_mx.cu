@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *codes, c
 #pragma unroll
         for (int b = 0; b < 8; b++) v[b] *= scale;
         if (j + 8 <= k) {
-            if (sizeof(T) == 4) {
+            if constexpr (sizeof(T) == 4) {
                 reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
                 reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
             } else {

@@ -88,8 +88,6 @@ __device__ __forceinline__ float mx_unpack1(uint32_t code) {
 template <typename T>
 __device__ __forceinline__ uint32_t mx_pair(float a, float b);
 template <>
-__device__ __forceinline__ uint32_t mx_pair<float>(float, float) { return 0; }  // 32-bit rows take another path
-template <>
 __device__ __forceinline__ uint32_t mx_pair<__half>(float a, float b) {
     const __half2 p = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&p);
@@ -222,8 +220,6 @@ __device__ __forceinline__ uint32_t mx_piece_scale_of(uint32_t s, int p) { retur
 
 template <typename T>
 __device__ __forceinline__ float mx_float(T v);
-template <>
-__device__ __forceinline__ float mx_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float mx_float<__half>(__half v) { return __half2float(v); }
 template <>

@@ -49,7 +49,7 @@ struct TcArgs {
     uint32_t nt;              // tokens of a full CTA tile
     uint32_t group;           // tokens per 256 rows of pieces (KIND 8, kDense)
     uint32_t stages, split;   // ring depth; CTAs of a cluster that share a tile's K
-    uint32_t stage_bytes, b_bytes, b_box_bytes, tmem_cols, d_cols, ring_bytes, row_tiles;
+    uint32_t stage_bytes, b_bytes, tmem_cols, d_cols, ring_bytes, row_tiles;
     const uint8_t *w_scales, *x_scales;
     void *y;
     int type;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
     }
     constexpr uint32_t accs = DEAL == kOne ? 1 : 2;   // accumulators: the epilogue reads one while the next fills
     uint32_t n_cols, b_bytes, stage_bytes, stages;
-    const uint32_t sfb_cols = a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
+    const uint32_t sfb_cols = KIND == 8 && a.nt * P > 128 ? 8 : 4, sf_cols = kSub * (4 + sfb_cols);
     auto shape_ring = [&] {   // the experts' ring is as deep as this expert's few tokens allow
         n_cols = (tokens * P + 7) / 8 * 8;
         b_bytes = kExperts ? n_cols * 128 : a.b_bytes;
@@ -316,8 +316,8 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
             const uint32_t st0 = smem_u32(ring) + kA, full0 = smem_u32(&c.full[0]), empty0 = smem_u32(&c.empty[0]);
             uint32_t st = st0, full = full0, empty = empty0, s = 0, phase = 1, issued = 0;
             if (MODE == kDense) {
-                const bool two = col_tiles > 1;   // 128 columns and more: a second tile of scales, and of KIND 4 codes
-                const uint32_t tx = (KIND == 8 ? a.b_box_bytes : col_tiles * a.b_box_bytes) + col_tiles * kSf;
+                const bool two = KIND == 8 && col_tiles > 1;   // more than 128 columns (three pieces): a second tile of scales
+                const uint32_t tx = a.b_bytes + (two ? 2 : 1) * kSf;
                 const uint32_t row = KIND == 8 ? tok0 / a.group * 256 + tok0 % a.group * P : tok0;
                 const uint32_t row_sf = (KIND == 8 ? a.steps : 2 * a.kw) * kMxScaleTile;   // scales of 128 rows
                 const uint8_t *sf = a.x_scales + (size_t)(row / 128) * row_sf + k0 * kSf;
@@ -325,12 +325,8 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                 for (uint32_t step = 0; step < steps; step++, x += 128, sf += kSf) {
                     if (!mbar_poll(empty, phase, abort, 608)) goto columns_out;
                     mbar_expect(full, tx);
-                    if (KIND == 8) {
-                        tma_2d(st, &xmap, x, (int)row, full);
-                    } else {
-                        tma_2d(st, &xmap, 0, x, full);
-                        if (two) tma_2d(st + a.b_box_bytes, &xmap, 0, x + (int)(a.kw * 128), full);
-                    }
+                    if (KIND == 8) tma_2d(st, &xmap, x, (int)row, full);
+                    else tma_2d(st, &xmap, 0, x, full);
                     bulk_copy(st + b_bytes + kSf, sf, kSf, full);
                     if (two) bulk_copy(st + b_bytes + 2 * kSf, sf + row_sf, kSf, full);
                     issued++;
@@ -387,7 +383,7 @@ __global__ void __launch_bounds__(kThreads) mx_tc_kernel(const __grid_constant__
                     scales_to_tmem(sfa + 4 * h, sf + h * kMxScaleTile);
                     if (!kExperts) {
                         scales_to_tmem(sfb + sfb_cols * h, sf + kSf + h * kMxScaleTile);
-                        if (col_tiles > 1) scales_to_tmem(sfb + sfb_cols * h + 4, sf + 2 * kSf + h * kMxScaleTile);
+                        if (KIND == 8 && col_tiles > 1) scales_to_tmem(sfb + sfb_cols * h + 4, sf + 2 * kSf + h * kMxScaleTile);
                     } else {
                         scales_to_tmem(sfb, sfb_smem);
                     }
@@ -812,8 +808,7 @@ template <int KIND, int P, int MODE>
 uint32_t plan_ring(TcArgs &a, uint32_t per_sm) {
     const uint32_t n = up_to(a.nt * P, 8), sub = KIND == 8 ? 1 : 2;
     const bool experts = MODE == kGateUp || MODE == kDown;
-    a.b_box_bytes = (KIND == 8 || n < 128 ? n : 128) * 128;       // KIND 4 copies whole tiles of 128 columns
-    a.b_bytes = KIND == 8 ? n * 128 : (n + 127) / 128 * a.b_box_bytes;
+    a.b_bytes = n * 128;
     a.stage_bytes = kA + a.b_bytes + up_to(kMxScaleTile * sub * (1 + (experts ? 0 : (n + 127) / 128)), 1024);
     a.d_cols = up_to(a.nt, 8) * P;
     const uint32_t sf_cols = sub * (4 + (a.nt * P > 128 ? 8 : 4));
@@ -880,9 +875,9 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
         xmap = wmap;   // not read
     else if (KIND == 8)
         e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)a.steps * 128, mx_piece_rows(p.m, p.x_type),
-                   (uint64_t)a.steps * 128, 128, a.b_box_bytes / 128, CU_TENSOR_MAP_SWIZZLE_128B);
+                   (uint64_t)a.steps * 128, 128, a.b_bytes / 128, CU_TENSOR_MAP_SWIZZLE_128B);
     else
-        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 128, (uint64_t)mx_tiles(p.m) * kw * 128, 128, 128, a.b_box_bytes / 128,
+        e = encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, 128, (uint64_t)mx_tiles(p.m) * kw * 128, 128, 128, a.b_bytes / 128,
                    CU_TENSOR_MAP_SWIZZLE_128B);
     if (e != cudaSuccess) return e;
     return launch<KIND, P, MODE>(wmap, xmap, a, dim3(rt, tt, a.split), smem, s);
