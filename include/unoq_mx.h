@@ -78,8 +78,9 @@ UG_API int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32
                          const uint8_t *w_scales, uint32_t n, uint32_t k, void *y, int type, uint64_t stride,
                          void *stream);
 /* The same with 16-bit activations x (m x k, UG_F16 or UG_BF16, rows `x_stride` elements apart), which
- * are not rounded to fewer bits: a value is kept exactly while it is above 2^-12 of the largest of
- * its block of 32, and to within 2^-21 of that largest below. A block with a NaN or an infinity
+ * are not rounded to MX4 but held as 8-bit pieces on one scale to a block of 32: a value is kept exactly
+ * while it is above 2^-12 of the largest of its block, and to within 2^-21 (UG_F16: 2^-25) of that largest
+ * below, so that what is far smaller than a loud neighbour loses bits, and in the end all of them. A block with a NaN or an infinity
  * makes its row of y NaN. */
 UG_API int ug_mx4_matmul_x16(const void *x, int x_type, uint64_t x_stride, uint32_t m, const uint8_t *w_codes,
                              const uint8_t *w_scales, uint32_t n, uint32_t k, void *y, int type, uint64_t stride,

@@ -849,3 +849,30 @@ def test_outputs_in_the_buffer_of_their_input(mx):
             assert torch.equal(buf, was)
         with pytest.raises(ValueError, match="overlap"):
             mx.matmul(buf[:, 3:99], W, out=buf[:, 98:148])
+
+
+@pytest.mark.parametrize("name,floor", [("bf16", 2.0 ** -21), ("f16", 2.0 ** -25)])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 256), (10, 130, 1000), (40, 200, 520), (1100, 2400, 256)])
+def test_matmul_x16_beside_loud_values(mx, m, n, k, name, floor):
+    """One value of 2^14 in every block, facing weights of zero: what the others keep is what the header says, for
+    f16 2^-25 of the largest (its three pieces). The sum's own error is that of the pieces' magnitudes, which exceed the
+    values' by half of the first piece's least step, 2^-17 of the largest, and less for each next one."""
+    g = torch.Generator().manual_seed(m + k)
+    x = 0.02 * torch.randn(m, k, generator=g)
+    c, s = weights(n, k, n)
+    w = mxref.values(c, s, k)
+    loud = torch.arange(k) % 32 == 5
+    x[:, loud] = 2.0 ** 14
+    x = x.to(mxref.TYPES[name])
+    codes = torch.stack((c & 15, c >> 4), -1).flatten(-2)[:, :k]
+    codes[:, loud] = 0
+    codes = torch.nn.functional.pad(codes, (0, k % 2))
+    w = w * ~loud
+    W = mx.pack((codes[:, 0::2] | codes[:, 1::2] << 4).cuda(), s.cuda(), k=k)
+    a = x.double() * ~loud
+    largest = 2.0 ** 14 * (torch.arange(k) // 32 * 32 + 5 < k)
+    want = a @ w.t()
+    held = largest[None].double() @ w.abs().t()
+    bound = floor * held + mxref._sum_error(k) * (a.abs() @ w.abs().t() + 2.0 ** -16 * held)
+    for dtype in (torch.float32, mxref.TYPES[name]):
+        assert_within(mx.matmul(x.cuda(), W, dtype=dtype), want, bound + mxref.half_step(want.abs() + bound, dtype), str(dtype))

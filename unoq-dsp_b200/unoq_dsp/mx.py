@@ -7,7 +7,7 @@ for inference: an input that needs a gradient is refused while gradients are rec
 forward-mode tangent always. PyTorch is imported here only; the rest of the package does not need it.
 
     w = mx.quantize(weight)                      # (n, k) -> MX4, once
-    y = mx.matmul(x, w)                          # 16-bit x, 4-bit weights
+    y = mx.matmul(x, w)                          # 16-bit x, 4-bit weights (what x keeps: see matmul)
     y = mx.matmul(mx.quantize(x), w)             # both in 4 bits
     layer = mx.Experts(router, gate_up, down, top_k=4)
     y = layer(x)                                 # a few tokens through a mixture of experts
@@ -292,7 +292,8 @@ def pack(codes, scales, k=None):
 
 def matmul(a, w, dtype=None, out=None):
     """y = a w^T for 4-bit weights ``w`` (n x k): ``a`` is an :class:`MX4` (m x k), or 16-bit values (..., k)
-    which are not rounded to fewer bits. Sums are held in 32 bits and rounded once to ``dtype``
+    which are kept exactly down to 2^-12 of the largest of their block of 32, and below that to within 2^-21 of
+    that largest (float16: 2^-25): what is far smaller than a loud neighbour loses bits. Sums are held in 32 bits and rounded once to ``dtype``
     (default: a's, bfloat16 for an MX4). A NaN or an infinity in a block of ``a`` makes its row NaN."""
     if not isinstance(w, MX4) or w.layout != "operand":
         raise ValueError("w must be an MX4 in operand layout (quantize or pack)")
