@@ -876,3 +876,92 @@ def test_matmul_x16_beside_loud_values(mx, m, n, k, name, floor):
     bound = floor * held + mxref._sum_error(k) * (a.abs() @ w.abs().t() + 2.0 ** -16 * held)
     for dtype in (torch.float32, mxref.TYPES[name]):
         assert_within(mx.matmul(x.cuda(), W, dtype=dtype), want, bound + mxref.half_step(want.abs() + bound, dtype), str(dtype))
+
+
+def test_experts_past_32_bits(mx):
+    """256 experts of 8.6 GB of gate and up codes: the first and the last two, chosen by the bias."""
+    d, f, e = 8192, 4096, 256
+    make, gate_up, down = mxref.whole_layer(d, f, 3, 1)
+    at = [0, 254, 255]
+    parts = []
+    for small in (gate_up, down):
+        wide = tuple(torch.zeros(e, *t.shape[1:], dtype=torch.uint8, device="cuda") for t in small)
+        for to, t in zip(wide, small):
+            to[at] = t.cuda()
+        parts.append(wide)
+    bias = torch.full((e,), -math.inf)
+    router = torch.zeros(e, d, dtype=torch.bfloat16, device="cuda")
+    x = make(9)
+    for chosen in ((0, 2), (1, 2)):
+        b = bias.clone()
+        b[[at[i] for i in chosen]] = 1.0
+        layer = mx.Experts(router, *parts, 2, bias=b.cuda())
+        y, got, _ = layer(x.to(torch.bfloat16).cuda(), return_choice=True)
+        assert got.tolist() == [[at[i] for i in chosen]] * 9
+        want, bound = mxref.whole_experts(x, torch.tensor([chosen] * 9), gate_up, down)
+        assert not (mxref.rounding_off(y, want, bound, torch.bfloat16) > 0).any()
+        del layer
+
+
+def test_captured_forks_copies_and_joins(mx):
+    """A graph whose branches meet in a call, with copies and fills as the nodes before the kernels."""
+    parts = network(mx)
+    router, gate_up, down, _ = layer_parts(160, 96, 12, "bf16", False, 8)
+    other = mx.Experts(router.cuda().flip(0), on_gpu(gate_up), on_gpu(down), 2)
+    x = torch.randn(10, 128, generator=gen(7), device="cuda").to(torch.bfloat16)
+
+    def run(v, side):
+        a = v.clone()                      # a copy before a product
+        h = mx.matmul(a, parts[0])
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):      # one branch
+            q = mx.quantize(h)
+            one = mx.matmul(q, parts[1], dtype=v.dtype)
+            left = parts[2](one)
+        two = torch.zeros(10, 160, device="cuda", dtype=v.dtype)
+        mx.matmul(h, parts[1], out=two)    # the other, after a fill
+        right = other(two)
+        here.wait_stream(side)
+        both = torch.empty(20, 160, device="cuda", dtype=v.dtype)
+        mx.matmul(h, parts[1], out=both[:10])
+        both[10:] = left + right
+        return other(both), left, right
+
+    want = [t.clone() for t in run(x, torch.cuda.Stream())]
+    torch.cuda.synchronize()
+    static, side, g = x.clone(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run(static, side)
+    for _ in range(20):
+        [t.fill_(math.nan) for t in got]
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    mx.check()
+
+
+def test_the_first_calls_of_a_process_may_be_captured(mx):
+    """No call needs one before it: a fresh process whose first calls are captured."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = %r
+import torch
+from unoq_dsp import mx
+w = torch.randn(192, 128, device="cuda")
+x = torch.randn(24, 128, device="cuda").bfloat16()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+def run():
+    q = mx.quantize(w)
+    return mx.matmul(x, q), mx.matmul(mx.quantize(x), q), mx.matmul(x[:3], q), q.dequantize()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+mx.check()
+print("captured")
+""" % [p for p in sys.path if p]
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=200)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
