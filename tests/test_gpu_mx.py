@@ -728,7 +728,9 @@ WHOLE = [  # tokens, d, f, experts, experts of every token, type
     # long rows: K spread over a cluster
     (3, 16384, 64, 2, 2, "bf16"), (2, 40, 16384, 2, 1, "f16"), (33, 4200, 70, 2, 1, "f16"), (9, 300, 4300, 2, 2, "bf16"),
     # several tiles to a CTA, from one expert on to the next
-    (8, 130, 1000, 20, 16, "bf16"), (90, 256, 4500, 2, 1, "f16"), (40, 2600, 70, 16, 16, "f16")]
+    (8, 130, 1000, 20, 16, "bf16"), (90, 256, 4500, 2, 1, "f16"), (40, 2600, 70, 16, 16, "f16"),
+    # 24 tokens of an expert to a CTA: one to a tile, several tiles, dealt out
+    (44, 520, 260, 2, 1, "f16"), (48, 1447, 999, 4, 2, "bf16"), (128, 130, 1000, 6, 1, "f16"), (72, 2000, 4000, 4, 1, "bf16")]
 
 
 @pytest.mark.parametrize("t,d,f,e,top,name", WHOLE)

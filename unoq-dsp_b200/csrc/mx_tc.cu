@@ -34,8 +34,7 @@ constexpr int kThreads = 224;      // warp 0: weight copies, warp 1: MMA, warps 
 constexpr int kCtrlBytes = 1024;   // barriers, TMEM slot and, for the experts, the token list
 constexpr int kItemWords = 2 + 32; // an item: expert, tokens, the pairs (a lane each)
 // Most tokens of one expert that one CTA takes: two accumulators of 32 tokens' hidden pieces would fill its 256 columns
-// of TMEM. (With three pieces to a value and 32 tokens: 4 of 16 experts, d 4096, f 2048, 128 tokens 146 us against 168;
-// 4 of 32, d 2048, f 1024, 128 tokens 56.4, 58.6; 2 of 8, 128 tokens 46.4, 43.4.)
+// of TMEM.
 constexpr int kChunk = 24;
 constexpr uint32_t kA = 16384;     // one weight tile in shared memory
 
@@ -834,8 +833,10 @@ template <int KIND, int P, int MODE>
 cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_scales, cudaStream_t s) {
     const uint32_t rt = mx_tiles(p.n), kw = mx_ktiles(p.k) / 2;
     constexpr uint32_t kGroup = P == 1 ? 256 : P == 2 ? 128 : 64;   // tokens that fill 256 columns (P = 3: 192)
-    // Pairs of CTAs once their tiles go round most of the 74: bf16 x, 512 x 8192 x 1024 (128 tiles) 11.8 us against
-    // 14.4 in single CTAs, 512 x 4096 x 4096 (64) 17.7 against 18.5, 1024 x 1024 x 4096 (32) 19.0 against 14.3.
+    // Pairs of CTAs once their tiles go round most of the 74, whatever the form. Against single CTAs, K 4096 and 4096 weight
+    // rows: 4 bits, 128 tiles 16.2 us and 20.0, 64 10.7 and 10.8, 32 10.3 and 6.7; bf16 28.8 and 33.5, 17.2 and 18.3, 15.2 and
+    // 11.6; f16 22.0 and 25.2, 13.4 and 13.5, 12.2 and 12.4. With K 1024, 128 and 64 tiles: 4 bits 9.8 and 10.8, 7.1 and 6.2;
+    // bf16 11.5 and 14.2, 8.2 and 8.4; f16 9.6 and 12.6, 7.0 and 7.2.
     if (MODE == kDense && p.m > kGroup / 2 && (rt + 1) / 2 * ((p.m + kGroup - 1) / kGroup) >= 64)
         return pair_product<KIND, P>(p, x, x_scales, s);
     TcArgs a{};
@@ -927,9 +928,11 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     a.type = e.type;
     a.stride = e.y_stride;
     a.combine = mx_combines(e);
-    // Tokens to a CTA: 16 where the experts get few, which leaves room for a second accumulator.
+    // Tokens to a CTA: 24 where that spares the experts their second or third item, else 16, whose columns cost less (16 of
+    // 64 experts, d 2048, f 1024: 12 pairs to an expert on average 75.5 us with 16, 78.3 with 24; 14: 101, 87.5; 20: 131, 105;
+    // 24: 138, 137; 28: 145, 163; 4 of 16, d 4096, f 2048: 13: 77.5, 79.1; 16: 107, 87.7; 32: 157, 168).
     const uint32_t pairs = e.tokens * e.top_k, slots = std::min(e.experts, pairs);
-    a.chunk = pairs <= e.experts * 8 ? 16 : kChunk;
+    a.chunk = pairs > e.experts * 13 && pairs <= e.experts * kChunk ? kChunk : 16;
     a.nt = std::min(e.tokens, a.chunk);
     // as many items as there can be: one to each chosen expert, one more for every further chunk of pairs
     const uint32_t items = slots + (pairs - slots) / a.chunk;
