@@ -330,3 +330,12 @@ def test_outputs_beside_inputs_in_one_buffer():
     assert takes(other, buf[:, :20])[0] is False
     for x in (flat[:40], buf[:1, :20]):
         assert takes(buf[1:], x.view(1, -1)) == (True, True)
+
+
+def test_workspaces_of_few_rows(native):
+    """Few rows are split into pieces inside the product and need none; the longer the rows, the fewer."""
+    need = native.ug_mx4_matmul_x16_workspace
+    for x_type, pieces in ((2, 2), (1, 3)):
+        for k, columns in ((1, 32), (4096, 32), (4097, 15), (8192, 8), (16384, 4), (30000, 2), (65536, 1)):
+            m = columns // pieces
+            assert need(m, k, x_type) == 0 and need(m + 1, k, x_type) > 0

@@ -27,8 +27,14 @@ __host__ __device__ inline uint32_t mx_tiles(uint32_t n) { return (n + kMxTile -
 __host__ __device__ inline uint32_t mx_ktiles(uint32_t k) { return (k + 255) / 256 * 2; }
 // Pieces of a 16-bit value: 4 significant bits each, so two hold a bf16 (8) and three an f16 (11).
 __host__ __device__ inline int mx_pieces(int type) { return type == 2 ? 2 : 3; }
-// Whether the product splits m tokens itself: their pieces fill at most 32 columns, 16 bf16 or 10 f16 tokens.
-inline bool mx_fused(uint32_t m, int type) { return (uint64_t)m * mx_pieces(type) <= 32; }
+// Whether the product splits m tokens itself: up to 32 columns of pieces (16 bf16 or 10 f16 tokens), for long rows fewer.
+// That is one launch for two, but every CTA splits its share of the rows anew. bf16, a call, in the product and before it:
+// 4096 x 4096, 1 token 8.8 us and 13.3, 16 tokens 11.3 and 13.3 (the GPU's time alone 6.6 and 6.2, 11.2 and 6.7);
+// 2048 x 8192, 2 tokens 12.1 and 13.1, 4 13.5 and 13.2, 8 16.6 and 13.2; 8192 x 8192, 4 tokens 9.9 and 13.4, 16 18.0 and
+// 13.3; 8192 x 16384, 2 tokens 12.5 and 13.1, 6 16.3 and 13.3; 4096 x 65536, 2 tokens 26.7 and 27.8, 6 35.5 and 29.7.
+inline bool mx_fused(uint32_t m, uint32_t k, int type) {
+    return (uint64_t)m * mx_pieces(type) <= (k <= 4096 ? 32 : 65536 / k);
+}
 
 #ifdef __CUDACC__
 __device__ __forceinline__ size_t mx_code_at(uint32_t r, uint32_t j, uint32_t kt) {

@@ -223,7 +223,7 @@ int ug_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, uint32_t m, c
 }
 
 size_t ug_mx4_matmul_x16_workspace(uint32_t m, uint32_t k, int x_type) {
-    if (!is_half(x_type) || !k || uq::mx_fused(m, x_type)) return 0;
+    if (!is_half(x_type) || !k || uq::mx_fused(m, k, x_type)) return 0;
     const size_t rows = uq::mx_piece_rows(m, x_type), kt = (k + 127ull) / 128;
     return up(rows * kt * 128) + up((rows + 127) / 128 * kt * uq::kMxScaleTile);
 }

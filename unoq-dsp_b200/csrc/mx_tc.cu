@@ -886,7 +886,7 @@ cudaError_t dense(const MxProductArgs &p, const uint8_t *x, const uint8_t *x_sca
 
 template <typename T, int P>
 cudaError_t dense_x16(const MxProductArgs &p, cudaStream_t s) {
-    if (mx_fused(p.m, p.x_type)) return dense<8, P, kFused>(p, nullptr, nullptr, s);
+    if (mx_fused(p.m, p.k, p.x_type)) return dense<8, P, kFused>(p, nullptr, nullptr, s);
     const uint32_t kt = mx_tiles(p.k), chunks = (p.k + 255) / 256;
     constexpr uint32_t kGroup = P == 2 ? 128 : 64;
     uint8_t *pieces = static_cast<uint8_t *>(p.workspace);
