@@ -11,7 +11,8 @@
  *                   codes in tiles of 256 values, ((r / 128) * K + j / 256) * 16384 + (r % 128) * 128 +
  *                   (j % 256) / 2 with K = ceil(k/256), and scales in tiles of 128 values,
  *                   ((r / 128) * 2K + j / 128) * 512 + (r % 32) * 16 + (r / 32 % 4) * 4 + (j / 32 % 4).
- *                   Values and scale bytes past k, up to 256 K, are zero.
+ *                   Values and scale bytes past k, up to 256 K, are zero; rows past the last, in its
+ *                   tile, are zero from ug_mx4_pack and left as they were by ug_mx4_quantize.
  * A last block or tile may be partial: rows and k are free (k >= 1), as far as the kernels count in 32 bits.
  * With T = 2 ceil(k/256), the scale tiles along a row:
  *   quantise, dequantise       rows * T < 2^31, k <= 2^30

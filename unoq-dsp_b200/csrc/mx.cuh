@@ -240,9 +240,11 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 mx_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 #endif
 
-// Every kernel below is launched programmatically (common.cuh): its first access to memory follows
-// grid_dep_wait(), and it lets the next one start only after that, so a kernel that has started
-// early never meets memory of one before the last. Its loads are plain ones, not __ldg: those are for memory
+// The kernels below but pack_kernel, which is launched in full stream order, are launched programmatically (common.cuh):
+// a kernel's first access to memory follows grid_dep_wait(), and it lets the next one start only after that, so a
+// kernel that has started early never meets memory of one before the last. The exception are the weight copies of
+// a product that follows pieces_kernel: that kernel has waited for all before it and writes no weights, so they
+// need not wait for it. Loads are plain ones, not __ldg: those are for memory
 // that nobody writes while the kernel runs, and the kernel before may still write when this one starts.
 cudaError_t launch_mx4_quantize(const void *x, int type, uint32_t rows, uint32_t k, uint64_t stride, int layout,
                                 uint8_t *codes, uint8_t *scales, cudaStream_t s);

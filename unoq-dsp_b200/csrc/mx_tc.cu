@@ -942,8 +942,8 @@ cudaError_t expert_product(const MxExpertsArgs &e, cudaStream_t s) {
     while (a.split < 8 && a.steps / a.split > 32) a.split *= 2;
     // A round of CTAs is two to an SM. Up to four tiles of an item to each while one round holds all items there can be;
     // more tiles are dealt out evenly, from one item on to the next, which costs 4 us for each change of items
-    // (bf16, 4 of 32 experts, d 2048, f 1024, two tiles to a CTA: 16 tokens 33 us, dealt out 39; 8 of 128, four tiles: 8
-    // tokens 46, dealt out 50; seven: 16 tokens 67 dealt out, 75 in rounds of four tiles, and 64 tokens 97 and 100).
+    // (bf16, 4 of 32 experts, d 2048, f 1024, two tiles to a CTA: 16 tokens 31 us, dealt out 37; 8 of 128, four tiles: 8
+    // tokens 46, dealt out 49; seven: 16 tokens 66 dealt out, 77 in rounds of four tiles, and 64 tokens 98 and 101).
     const uint32_t ctas = 2 * (uint32_t)current_sm_count(), each = (a.row_tiles * slots + ctas - 1) / ctas;
     a.shared = a.split == 1 && each > 4;
     a.per_cta = a.split == 1 && !a.shared ? each : 1;
