@@ -102,8 +102,8 @@ typedef struct {
 
 /* y[t] = sum over the top_k experts e of token t (largest logits x[t] . router[e] + bias[e], ties to the
  * lowest index) of p_e * down_e (silu(gate_e x[t]) * (up_e x[t])). Logits, softmax and sums are held in
- * 32 bits; a hidden value is kept to within 2^-19 of itself, or 2^-29 of the largest of its block of 32
- * where that is more. Rows of x and y are x_stride and y_stride elements apart; tokens <=
+ * 32 bits; a hidden value is kept to within 2^-19 of itself, or 2^-29 of the largest of its block of 32,
+ * or 2^-137, where that is more. Rows of x and y are x_stride and y_stride elements apart; tokens <=
  * UG_MX4_MAX_TOKENS. A logit that is not a number comes before every number: its expert is chosen, and the
  * token's weights and its row of y are NaN. `chosen` and `weights` (tokens x top_k, either may be NULL) receive the experts in
  * falling order of their logits and the p_e. */

@@ -967,3 +967,11 @@ print("captured")
 """ % [p for p in sys.path if p]
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=200)
     assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(1, 130, 65536), (2, 300, 40000), (4, 200, 8193), (5, 200, 8193), (9, 130, 5000), (6, 2100, 16384), (3, 1, 30000)])
+def test_matmul_x16_few_tokens_of_long_rows(mx, m, n, k, name):
+    """Around the change from pieces made in the product to those made before it."""
+    test_matmul_x16_exact(mx, m, n, k, name)
+    test_matmul_x16(mx, m, n, k, name)
