@@ -293,8 +293,9 @@ def pack(codes, scales, k=None):
 def matmul(a, w, dtype=None, out=None):
     """y = a w^T for 4-bit weights ``w`` (n x k): ``a`` is an :class:`MX4` (m x k), or 16-bit values (..., k)
     which are kept exactly down to 2^-12 of the largest of their block of 32, and below that to within 2^-21 of
-    that largest (float16: 2^-25): what is far smaller than a loud neighbour loses bits. Sums are held in 32 bits and rounded once to ``dtype``
-    (default: a's, bfloat16 for an MX4). A NaN or an infinity in a block of ``a`` makes its row NaN."""
+    that largest (float16: 2^-25): what is far smaller than a loud neighbour loses bits. Sums are held in 32 bits
+    and rounded once to ``dtype`` (default: a's, bfloat16 for an MX4). A NaN or an infinity in a block of ``a``
+    makes its row NaN."""
     if not isinstance(w, MX4) or w.layout != "operand":
         raise ValueError("w must be an MX4 in operand layout (quantize or pack)")
     lib, n, device = _lib or _library(), w.rows, w.device
